@@ -199,8 +199,11 @@ typedef enum {
     dnnl_query_prop_kind = 11,
     dnnl_query_strides = 14,
     dnnl_query_src_md = 129,
+    dnnl_query_diff_src_md = 130,
     dnnl_query_weights_md = 131,
+    dnnl_query_diff_weights_md = 132,
     dnnl_query_dst_md = 133,
+    dnnl_query_diff_dst_md = 134,
     dnnl_query_workspace_md = 135,
     dnnl_query_scratchpad_md = 136,
     dnnl_query_exec_arg_md = 255,
@@ -605,6 +608,89 @@ dnnl_status_t dnnl_cuda_interop_peer_wait(dnnl_stream_t stream, int world, const
  * off.  dnnl_unimplemented for other implementations (use dnnl_cuda_interop_peer_scatter). */
 dnnl_status_t dnnl_cuda_interop_primitive_replicate_dst(dnnl_primitive_t primitive, int world, int rank,
         void *const *dst_bases, size_t buffer_bytes, unsigned *const *peer_flags, unsigned *done, unsigned epoch);
+
+/* ---- around the experts' products of a mixture-of-experts layer, and dropout (no counterpart in the reference) ----
+ * dnnl_matmul on grouped memory multiplies the rows of several experts in one call.  These primitives make that memory
+ * from tokens and bring its rows back, forward and backward.  They are created, queried, executed and destroyed as every
+ * other primitive (dnnl_primitive_create, dnnl_primitive_execute with the argument ids named below); an engine without a
+ * device creates their descriptors.  T tokens, E experts (1 to 1024), K choices per token (1 to 32, T K <= 2^30), H columns.
+ *   Matrices are [rows, cols] with neighbouring columns beside one another and any row pitch; an output's pitch is at least
+ *   its width; an input's may be 0 (one row for all).  Grouped memory is [T K, H] with E groups along dim 0 and s32
+ *   cumulative END offsets in its second buffer, as the grouped matmul has it.
+ *   Dims may be DNNL_RUNTIME_DIM_VAL: they are taken from the memory objects at each execution, one primitive serves
+ *   batches of any size.  T and H may be zero.
+ *   An attribute may set the scratchpad mode and nothing else (dnnl_unimplemented).
+ *   Errors: dims that contradict one another, a wrong rank, K > E, p or scale out of range: dnnl_invalid_arguments; data types, layouts
+ *   and sizes that are not built: dnnl_unimplemented.  Contents of index tensors never lead out of the buffers: an index or
+ *   a position that names nothing is skipped. */
+typedef enum {
+    dnnl_cuda_interop_moe_route = 0x10001,
+    dnnl_cuda_interop_moe_route_backward,
+    dnnl_cuda_interop_moe_dispatch,
+    dnnl_cuda_interop_moe_combine,
+    dnnl_cuda_interop_moe_combine_backward,
+    dnnl_cuda_interop_dropout
+} dnnl_cuda_interop_primitive_kind_t; /* what dnnl_query_primitive_kind answers for them */
+
+typedef enum {
+    dnnl_cuda_interop_scoring_softmax = 0, /* exp(l) over the sum of all experts' exp(l) */
+    dnnl_cuda_interop_scoring_sigmoid = 1 /* 1 / (1 + exp(-l)) */
+} dnnl_cuda_interop_scoring_t;
+
+#ifndef DNNL_ARG_DST_1
+#define DNNL_ARG_DST_1 18
+#define DNNL_ARG_DIFF_SRC 129
+#define DNNL_ARG_DIFF_DST 145
+#define DNNL_ARG_DIFF_WEIGHTS 161
+#define DNNL_ARG_ATTR_DROPOUT_SEED 510
+#endif
+
+/* Router.  SRC logits [T, E] (f32, bf16, f16) -> DST weights [T, K] (f32), DST_1 indices [T, K] (s32), by falling logit,
+ * ties to the lowest index.  Logits of -inf and NaN are masked: never chosen, without a share in any sum; a choice with
+ * nothing left has index -1 and weight 0.  normalize: weights are divided by their sum over the K choices.  Then they are
+ * multiplied by `scale`. */
+dnnl_status_t dnnl_cuda_interop_moe_route_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t logits_desc, const_dnnl_memory_desc_t weights_desc, const_dnnl_memory_desc_t indices_desc,
+        dnnl_cuda_interop_scoring_t scoring, int normalize, float scale, const_dnnl_primitive_attr_t attr);
+/* Its gradient.  SRC logits, SRC_1 the indices that the router chose, DIFF_DST the weights' gradient [T, K] (f32) ->
+ * DIFF_SRC [T, E], of the logits' type. */
+dnnl_status_t dnnl_cuda_interop_moe_route_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
+        dnnl_engine_t engine, const_dnnl_memory_desc_t logits_desc, const_dnnl_memory_desc_t indices_desc,
+        const_dnnl_memory_desc_t diff_weights_desc, const_dnnl_memory_desc_t diff_logits_desc,
+        dnnl_cuda_interop_scoring_t scoring, int normalize, float scale, const_dnnl_primitive_attr_t attr);
+/* Tokens into grouped memory.  SRC [T, H] (any type of 8, 16 or 32 bits), SRC_1 indices [T, K] (s32; one outside [0, E)
+ * gets no row) -> DST grouped [T K, H] of the same type: values, and the offsets, which this primitive writes; DST_1
+ * positions [T, K] (s32): the row of each (token, choice), -1 without one.  Rows of an expert stand in the order of their
+ * tokens.  Rows behind the last group are zero.  Its gradient is moe_combine without weights. */
+dnnl_status_t dnnl_cuda_interop_moe_dispatch_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
+        dnnl_engine_t engine, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t indices_desc,
+        const_dnnl_memory_desc_t dst_desc, const_dnnl_memory_desc_t positions_desc, const_dnnl_primitive_attr_t attr);
+/* Rows back to their tokens.  SRC grouped [T K, H], SRC_1 positions, WEIGHTS [T, K] (f32; weights_desc may be NULL: 1),
+ * SRC_2 residual [T, H] (NULL: none), ATTR_DROPOUT_SEED (dropout_p > 0) -> DST [T, H]:
+ *   residual + dropout(sum over K of weight x row).
+ * SRC and DST are f32, bf16 or f16, the residual of DST's type; sums are f32. */
+dnnl_status_t dnnl_cuda_interop_moe_combine_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
+        dnnl_engine_t engine, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t positions_desc,
+        const_dnnl_memory_desc_t weights_desc, const_dnnl_memory_desc_t residual_desc, const_dnnl_memory_desc_t dst_desc,
+        float dropout_p, const_dnnl_primitive_attr_t attr);
+/* Its gradient.  DIFF_DST [T, H], SRC, SRC_1, WEIGHTS and ATTR_DROPOUT_SEED as forward -> DIFF_SRC grouped, of SRC's type (its
+ * offsets are not written; rows behind SRC's last group are zero), DIFF_WEIGHTS [T, K] (f32).  (The residual's gradient is
+ * DIFF_DST itself.) */
+dnnl_status_t dnnl_cuda_interop_moe_combine_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
+        dnnl_engine_t engine, const_dnnl_memory_desc_t diff_dst_desc, const_dnnl_memory_desc_t src_desc,
+        const_dnnl_memory_desc_t positions_desc, const_dnnl_memory_desc_t weights_desc,
+        const_dnnl_memory_desc_t diff_src_desc, const_dnnl_memory_desc_t diff_weights_desc, float dropout_p,
+        const_dnnl_primitive_attr_t attr);
+/* Dropout.  SRC [M, N] (f32, bf16, f16), SRC_2 residual (NULL: none), ATTR_DROPOUT_SEED -> DST:
+ *   residual + (kept ? src / (1 - p) : 0);
+ * a dropped element counts as zero whatever it is.  DST may be SRC's or the residual's memory.  The gradient is this
+ * primitive on the gradient, without a residual.
+ *   ATTR_DROPOUT_SEED: [2] s64 in device memory, (seed, offset): read by the kernel, so a captured graph can move on.  No
+ *   mask is stored.  Element i (row-major index in the logical dims, whatever the strides) is kept where word i % 4 of block i / 4 of
+ *   Philox4x32-10 - key seed, counter (i / 4, offset), 64 bits each, low word first - is >= floor(p 2^32).  0 <= p <= 1. */
+dnnl_status_t dnnl_cuda_interop_dropout_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t residual_desc, const_dnnl_memory_desc_t dst_desc,
+        float p, const_dnnl_primitive_attr_t attr);
 
 #ifdef __cplusplus
 }

@@ -24,6 +24,7 @@ _STATUS_NAME = ["success", "out_of_memory", "invalid_arguments", "unimplemented"
 # exec-arg ids (dnnl_types.h:2542-2786)
 ARG_SRC, ARG_SRC_1, ARG_DST, ARG_WEIGHTS, ARG_BIAS, ARG_SCRATCHPAD = 1, 2, 17, 33, 41, 80
 ARG_FROM, ARG_TO = ARG_SRC, ARG_DST
+ARG_SRC_2, ARG_DST_1, ARG_DIFF_SRC, ARG_DIFF_DST, ARG_DIFF_WEIGHTS, ARG_ATTR_DROPOUT_SEED = 3, 18, 129, 145, 161, 510
 SCRATCHPAD_MODE_LIBRARY, SCRATCHPAD_MODE_USER = 0, 1  # dnnl_scratchpad_mode_t
 ARG_ATTR_SCALES, ARG_ATTR_ZERO_POINTS, ARG_ATTR_PRECOMPUTED_REDUCTIONS = 4096, 8192, 512
 
@@ -88,6 +89,13 @@ def lib():
         L.dnnl_version.restype = C.c_void_p
         L.dnnl_post_ops_append_eltwise.argtypes = [C.c_void_p, C.c_int, C.c_float, C.c_float]
         L.dnnl_post_ops_append_sum.argtypes = [C.c_void_p, C.c_float, C.c_int32, C.c_int]
+        v, i, f = C.c_void_p, C.c_int, C.c_float
+        L.dnnl_cuda_interop_moe_route_primitive_desc_create.argtypes = [v, v, v, v, v, i, i, f, v]
+        L.dnnl_cuda_interop_moe_route_backward_primitive_desc_create.argtypes = [v, v, v, v, v, v, i, i, f, v]
+        L.dnnl_cuda_interop_moe_dispatch_primitive_desc_create.argtypes = [v, v, v, v, v, v, v]
+        L.dnnl_cuda_interop_moe_combine_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, f, v]
+        L.dnnl_cuda_interop_moe_combine_backward_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, v, f, v]
+        L.dnnl_cuda_interop_dropout_primitive_desc_create.argtypes = [v, v, v, v, v, f, v]
         L.dnnl_engine_create.argtypes = [C.c_void_p, C.c_int, C.c_size_t]
         _lib = L
     return _lib
@@ -437,6 +445,101 @@ class reorder(matmul):
                 C.byref(self._h), src_md._h, src_eng._h, dst_md._h, dst_eng._h,
                 attr._h if attr is not None else None),
                 "could not create a primitive descriptor for a reorder primitive")
+
+
+class scoring:
+    softmax, sigmoid = 0, 1
+
+
+def _handle(obj):
+    return obj._h if obj is not None else None
+
+
+class moe_route(matmul):
+    """The router of a mixture-of-experts layer: the k experts of the largest logits of each token and their weights.
+    ``{ARG_SRC: logits [T, E], ARG_DST: weights [T, k] f32, ARG_DST_1: indices [T, k] s32}``"""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, logits_md, weights_md, indices_md, scoring=scoring.softmax, normalize=True, scale=1.0,
+                     attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_moe_route_primitive_desc_create(
+                C.byref(self._h), eng._h, logits_md._h, weights_md._h, indices_md._h, scoring, int(normalize), scale,
+                _handle(attr)), "could not create a primitive descriptor for the moe_route primitive")
+
+
+class moe_route_backward(matmul):
+    """Its gradient: ``{ARG_SRC: logits, ARG_SRC_1: indices, ARG_DIFF_DST: gradient of the weights,
+    ARG_DIFF_SRC: gradient of the logits}``"""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, logits_md, indices_md, diff_weights_md, diff_logits_md, scoring=scoring.softmax,
+                     normalize=True, scale=1.0, attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_moe_route_backward_primitive_desc_create(
+                C.byref(self._h), eng._h, logits_md._h, indices_md._h, diff_weights_md._h, diff_logits_md._h, scoring,
+                int(normalize), scale, _handle(attr)),
+                "could not create a primitive descriptor for the moe_route_backward primitive")
+
+
+class moe_dispatch(matmul):
+    """Tokens into grouped memory: ``{ARG_SRC: tokens [T, H], ARG_SRC_1: indices [T, k], ARG_DST: grouped memory
+    [T k, H] (values and offsets are written), ARG_DST_1: positions [T, k]}``.  Its gradient is :class:`moe_combine`
+    without weights."""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, src_md, indices_md, dst_md, positions_md, attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_moe_dispatch_primitive_desc_create(
+                C.byref(self._h), eng._h, src_md._h, indices_md._h, dst_md._h, positions_md._h, _handle(attr)),
+                "could not create a primitive descriptor for the moe_dispatch primitive")
+
+
+class moe_combine(matmul):
+    """Rows back to their tokens, residual + dropout(weighted sum): ``{ARG_SRC: grouped memory [T k, H],
+    ARG_SRC_1: positions, ARG_WEIGHTS: weights [T, k] f32, ARG_SRC_2: residual, ARG_ATTR_DROPOUT_SEED: (seed, offset),
+    ARG_DST: [T, H]}``; weights, residual and dropout are optional."""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, src_md, positions_md, dst_md, weights_md=None, residual_md=None, dropout_p=0.0, attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_moe_combine_primitive_desc_create(
+                C.byref(self._h), eng._h, src_md._h, positions_md._h, _handle(weights_md), _handle(residual_md),
+                dst_md._h, dropout_p, _handle(attr)),
+                "could not create a primitive descriptor for the moe_combine primitive")
+
+
+class moe_combine_backward(matmul):
+    """Its gradient: ``{ARG_DIFF_DST: [T, H], ARG_SRC: grouped memory, ARG_SRC_1: positions, ARG_WEIGHTS: weights,
+    ARG_ATTR_DROPOUT_SEED: (seed, offset), ARG_DIFF_SRC: grouped memory, ARG_DIFF_WEIGHTS: [T, k] f32}``"""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, diff_dst_md, src_md, positions_md, weights_md, diff_src_md, diff_weights_md,
+                     dropout_p=0.0, attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_moe_combine_backward_primitive_desc_create(
+                C.byref(self._h), eng._h, diff_dst_md._h, src_md._h, positions_md._h, weights_md._h, diff_src_md._h,
+                diff_weights_md._h, dropout_p, _handle(attr)),
+                "could not create a primitive descriptor for the moe_combine_backward primitive")
+
+
+class dropout(matmul):
+    """residual + (kept ? src / (1 - p) : 0), the mask made from a counter and never stored: ``{ARG_SRC: [M, N],
+    ARG_SRC_2: residual (optional), ARG_ATTR_DROPOUT_SEED: [2] s64 (seed, offset), ARG_DST: [M, N]}``.  The gradient is
+    the same primitive on the gradient, without a residual."""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, src_md, dst_md, p, residual_md=None, attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_dropout_primitive_desc_create(
+                C.byref(self._h), eng._h, src_md._h, _handle(residual_md), dst_md._h, p, _handle(attr)),
+                "could not create a primitive descriptor for the dropout primitive")
 
 
 def launch_count():

@@ -847,7 +847,7 @@ dnnl_status_t dnnl_matmul_primitive_desc_create(dnnl_primitive_desc_t *primitive
 
 dnnl_status_t dnnl_primitive_desc_next_impl(dnnl_primitive_desc_t pd) {
     if (!pd) return dnnl_invalid_arguments;
-    if (pd->kind != dnnl_matmul) return dnnl_last_impl_reached; // one reorder implementation
+    if (pd->kind != dnnl_matmul) return dnnl_last_impl_reached; // one implementation of the other kinds
     dnnl_primitive_desc tmp = *pd;
     if (tmp.runtime_m) {
         apply_stand_ins(tmp);
@@ -882,6 +882,24 @@ dnnl_status_t dnnl_primitive_desc_destroy(dnnl_primitive_desc_t pd) {
 
 const_dnnl_memory_desc_t dnnl_primitive_desc_query_md(const_dnnl_primitive_desc_t pd, dnnl_query_t what, int index) {
     if (!pd) return nullptr;
+    if (is_token_op(pd->kind)) {
+        auto of = [&](int arg) { // null where the kind has no such tensor
+            const dnnl_memory_desc *md = arg == DNNL_ARG_SCRATCHPAD ? &pd->scratchpad : pd->token_op.find(arg);
+            return md;
+        };
+        switch ((int)what) {
+            case dnnl_query_src_md: return of(index == 0 ? DNNL_ARG_SRC : index == 1 ? DNNL_ARG_SRC_1 : index == 2 ? DNNL_ARG_SRC_2 : 0);
+            case dnnl_query_weights_md: return index == 0 ? of(DNNL_ARG_WEIGHTS) : nullptr;
+            case dnnl_query_dst_md: return of(index == 0 ? DNNL_ARG_DST : index == 1 ? DNNL_ARG_DST_1 : 0);
+            case dnnl_query_diff_src_md: return index == 0 ? of(DNNL_ARG_DIFF_SRC) : nullptr;
+            case dnnl_query_diff_weights_md: return index == 0 ? of(DNNL_ARG_DIFF_WEIGHTS) : nullptr;
+            case dnnl_query_diff_dst_md: return index == 0 ? of(DNNL_ARG_DIFF_DST) : nullptr;
+            case dnnl_query_scratchpad_md: return &pd->scratchpad;
+            case dnnl_query_workspace_md: return &g_zero_md;
+            case dnnl_query_exec_arg_md: return of(index) ? of(index) : &g_zero_md;
+            default: return nullptr;
+        }
+    }
     switch ((int)what) {
         case dnnl_query_src_md: return index == 0 ? &pd->src : nullptr;
         case dnnl_query_weights_md: return index == 0 ? &pd->wei : index == 1 ? &pd->bias : nullptr;
@@ -911,6 +929,13 @@ dnnl_status_t dnnl_primitive_desc_query(const_dnnl_primitive_desc_t pd, dnnl_que
     if (!pd || !result) return dnnl_invalid_arguments;
     int n_binary = 0;
     for (const auto &e : pd->attr.post_ops.entries) n_binary += e.kind == dnnl_binary;
+    if (is_token_op(pd->kind) && (what == dnnl_query_num_of_inputs_s32 || what == dnnl_query_num_of_outputs_s32)) {
+        int in = 0, out = 0;
+        for (const auto &kv : pd->token_op.args)
+            ++(kv.first == DNNL_ARG_DST || kv.first == DNNL_ARG_DST_1 || kv.first == DNNL_ARG_DIFF_SRC || kv.first == DNNL_ARG_DIFF_WEIGHTS ? out : in);
+        *(int *)result = what == dnnl_query_num_of_inputs_s32 ? in : out;
+        return dnnl_success;
+    }
     switch ((int)what) {
         case dnnl_query_engine:
         case dnnl_query_scratchpad_engine: *(dnnl_engine_t *)result = pd->engine; break;
@@ -1217,6 +1242,7 @@ extern "C" dnnl_status_t dnnl_primitive_execute(const_dnnl_primitive_t primitive
         return dnnl_invalid_arguments;
     for (int i = 0; i < nargs; ++i)
         if (!args[i].memory) return dnnl_invalid_arguments;
+    if (is_token_op(primitive->pd.kind)) return execute_token_op(*primitive, stream, nargs, args);
     if (primitive->pd.kind == dnnl_reorder) return execute_reorder(primitive->pd, stream, nargs, args);
     arg_map_t am {args, nargs};
     // A primitive created with dims left open takes them from the memory objects: every descriptor

@@ -100,6 +100,12 @@ const char *arg_name(int arg) {
         case DNNL_ARG_WEIGHTS: return "wei";
         case DNNL_ARG_DST: return "dst";
         case DNNL_ARG_BIAS: return "bia";
+        case DNNL_ARG_SRC_2: return "src2";
+        case DNNL_ARG_DST_1: return "dst1";
+        case DNNL_ARG_DIFF_SRC: return "diff_src";
+        case DNNL_ARG_DIFF_DST: return "diff_dst";
+        case DNNL_ARG_DIFF_WEIGHTS: return "diff_wei";
+        case DNNL_ARG_ATTR_DROPOUT_SEED: return "seed";
         default: return "arg";
     }
 }
@@ -174,6 +180,21 @@ std::string pd_info_string(const dnnl_primitive_desc &pd) {
         s += "reorder," + pd.impl_name + ",undef," + md_str("src", pd.src) + " " + md_str("dst", pd.dst) + ","
                 + attr_str(pd.attr) + ",," + dims_str(pd.src.dims, pd.src.ndims);
         return s;
+    }
+    if (is_token_op(pd.kind)) {
+        s += std::string(token_op_name(pd.kind)) + "," + pd.impl_name + ",undef,";
+        bool first = true;
+        for (const auto &kv : pd.token_op.args) {
+            s += (first ? "" : " ") + md_str(arg_name(kv.first), kv.second);
+            first = false;
+        }
+        std::ostringstream aux;
+        if (pd.token_op.p != 0.f) aux << "p:" << pd.token_op.p;
+        else if (pd.kind == (int)dnnl_cuda_interop_moe_route || pd.kind == (int)dnnl_cuda_interop_moe_route_backward)
+            aux << "scoring:" << (pd.token_op.scoring ? "sigmoid" : "softmax") << " normalize:" << pd.token_op.normalize
+                << " scale:" << pd.token_op.scale;
+        const dnnl_memory_desc *x = pd.token_op.find(DNNL_ARG_DIFF_DST) ? pd.token_op.find(DNNL_ARG_DIFF_DST) : pd.token_op.find(DNNL_ARG_SRC);
+        return s + "," + attr_str(pd.attr) + "," + aux.str() + "," + dims_str(x->dims, x->ndims);
     }
     s += "matmul," + pd.impl_name + ",undef," + md_str("src", pd.src) + " " + md_str("wei", pd.wei) + " ";
     if (pd.bias.ndims) {
@@ -320,6 +341,7 @@ const char *dnnl_prim_kind2str(dnnl_primitive_kind_t v) {
             "eltwise", "lrn", "batch_normalization", "inner_product", "rnn", "gemm", "binary", "matmul", "resampling",
             "pooling", "reduction", "prelu", "softmax", "layer_normalization", "group_normalization"};
     const int i = (int)v;
+    if (is_token_op(i)) return token_op_name(i);
     return i >= 0 && i < (int)(sizeof(names) / sizeof(*names)) ? names[i] : "unknown prim_kind";
 }
 const char *dnnl_alg_kind2str(dnnl_alg_kind_t v) { return alg_name((int)v); }

@@ -1,0 +1,209 @@
+// The router's choice: the k experts of the largest logits of each token and their weights, and the gradient.
+//   chosen   ties go to the lowest index; logits of -inf and NaN are masked, never chosen and without a share in any sum;
+//            a choice with nothing left has index -1 and weight 0
+//   softmax  w_j = scale exp(l_j - m) / sum_i exp(l_i - m), i over all unmasked experts, or over the chosen (normalize)
+//   sigmoid  w_j = scale s(l_j), or scale s(l_j) / sum over the chosen (normalize): the softmax of log s, which cannot
+//            divide zero by zero however low the logits
+// A warp keeps a row in registers (one read of the logits) and takes the largest value k times: a redux.sync over the keys,
+// then one over the indices that have it.  Keys are the logits' bits in the order of their values, so the choice is exact.
+// Sums are held in 32 bits.
+#include "launch.h"
+#include "token_rows.cuh"
+
+namespace qmm {
+
+namespace {
+
+constexpr int WARPS = 4; // rows per CTA
+
+// Bits in the order of the values; -0 as +0; 0 for a masked value.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    const uint32_t u = __float_as_uint(v + 0.f);
+    const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return v > -INFINITY ? k : 0u; // (false for a NaN too)
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    const float v = __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+    return fminf(v, 3.402823466e38f); // +inf counts as the largest finite value
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) v += __shfl_xor_sync(0xffffffffu, v, s);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
+    return v;
+}
+__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
+__device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
+
+template <typename T, int PER_LANE>
+__global__ void __launch_bounds__(WARPS * 32) route_kernel(const __grid_constant__ RouteArgs a) {
+    ptx::grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t t = (int64_t)blockIdx.x * WARPS + threadIdx.x / 32;
+    if (t >= a.tokens) return;
+    const T *row = (const T *)a.logits + t * a.logits_ld;
+    uint32_t key[PER_LANE]; // of experts lane, lane + 32, ...
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) {
+        const int e = 32 * i + lane;
+        key[i] = e < a.experts ? order_key(to_f32(row[e])) : 0u;
+    }
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) best = max(best, key[i]);
+    float sum = 0.f, top = 0.f;
+    if (a.scoring == SCORING_SOFTMAX && !a.normalize) {
+        top = key_value(__reduce_max_sync(0xffffffffu, best));
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i) sum += key[i] ? expf(key_value(key[i]) - top) : 0.f;
+        sum = warp_sum(sum);
+    }
+    uint32_t mine = 0; // key and index of choice `lane`
+    int index = -1;
+    for (int j = 0; j < a.choices; ++j) {
+        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+        if (most == 0) break;
+        int at = 0x7fffffff;
+        if (best == most) {
+#pragma unroll
+            for (int i = PER_LANE - 1; i >= 0; --i)
+                if (key[i] == most) at = 32 * i + lane;
+        }
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == j) {
+            mine = most;
+            index = at;
+        }
+        if (lane == (at & 31)) { // taken: out of the running
+            best = 0;
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) {
+                if (i == at >> 5) key[i] = 0u;
+                best = max(best, key[i]);
+            }
+        }
+    }
+    const bool chosen = index >= 0;
+    float w;
+    if (a.scoring == SCORING_SOFTMAX) {
+        if (a.normalize) top = key_value(__shfl_sync(0xffffffffu, mine, 0)); // the first choice is the largest
+        w = chosen ? expf(key_value(mine) - top) : 0.f;
+        if (a.normalize) sum = warp_sum(w);
+        w = chosen ? w / sum : 0.f;
+    } else if (a.normalize) {
+        const float l = chosen ? log_sigmoid(key_value(mine)) : -INFINITY;
+        const float m = __shfl_sync(0xffffffffu, l, 0);
+        w = chosen ? expf(l - m) : 0.f;
+        sum = warp_sum(w);
+        w = chosen ? w / sum : 0.f;
+    } else {
+        w = chosen ? sigmoid(key_value(mine)) : 0.f;
+    }
+    if (lane < a.choices) {
+        a.weights[t * a.weights_ld + lane] = w * a.scale;
+        a.indices[t * a.indices_ld + lane] = index;
+    }
+}
+
+// Gradient of the logits.  With g the weights' gradient times scale:
+//   softmax            dl_i = p_i (g_i - sum_j g_j p_j), over all experts; normalize: over the chosen, zero elsewhere
+//   sigmoid            dl_j = g_j s_j (1 - s_j); normalize, q_j = s_j / sum: dl_j = q_j (1 - s_j) (g_j - sum_i g_i q_i)
+// Lane j works on choice j; only the first form needs the logits of the experts that were not chosen.
+template <typename T>
+__global__ void __launch_bounds__(WARPS * 32) route_backward_kernel(const __grid_constant__ RouteArgs a) {
+    extern __shared__ float shared[];
+    ptx::grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t t = (int64_t)blockIdx.x * WARPS + threadIdx.x / 32;
+    if (t >= a.tokens) return;
+    float *grad = shared + threadIdx.x / 32 * a.experts;
+    const T *row = (const T *)a.logits + t * a.logits_ld;
+    T *out = (T *)a.diff_logits + t * a.diff_logits_ld;
+    int index = lane < a.choices ? a.indices[t * a.indices_ld + lane] : -1;
+    uint32_t key = (unsigned)index < (unsigned)a.experts ? order_key(to_f32(row[index])) : 0u;
+    const bool chosen = key != 0;
+    const float l = key_value(key);
+    float g = chosen ? a.weights[t * a.weights_ld + lane] * a.scale : 0.f;
+    const bool dense = a.scoring == SCORING_SOFTMAX && !a.normalize;
+    float top = 0.f, inverse = 0.f, inner = 0.f, d;
+    for (int e = lane; e < a.experts; e += 32) grad[e] = 0.f;
+    if (dense) {
+        float m = -INFINITY, sum = 0.f;
+        for (int e = lane; e < a.experts; e += 32) {
+            const uint32_t k = order_key(to_f32(row[e]));
+            if (k) m = fmaxf(m, key_value(k));
+        }
+        top = warp_max(m);
+        for (int e = lane; e < a.experts; e += 32) {
+            const uint32_t k = order_key(to_f32(row[e]));
+            if (k) sum += expf(key_value(k) - top);
+        }
+        inverse = 1.f / warp_sum(sum); // (unused where every expert is masked)
+        const float p = chosen ? expf(l - top) * inverse : 0.f;
+        inner = warp_sum(g * p);
+        d = g * p; // and - p * inner below, with all the others
+    } else if (a.scoring == SCORING_SOFTMAX) {
+        top = warp_max(chosen ? l : -INFINITY);
+        const float e = chosen ? expf(l - top) : 0.f;
+        const float sum = warp_sum(e), q = chosen ? e / sum : 0.f;
+        d = q * (g - warp_sum(g * q));
+    } else if (a.normalize) {
+        const float ls = chosen ? log_sigmoid(l) : -INFINITY;
+        const float m = warp_max(ls);
+        const float e = chosen ? expf(ls - m) : 0.f;
+        const float sum = warp_sum(e), q = chosen ? e / sum : 0.f;
+        d = q * sigmoid(-l) * (g - warp_sum(g * q));
+    } else {
+        d = g * sigmoid(l) * sigmoid(-l);
+    }
+    __syncwarp();
+    if (chosen) atomicAdd(&grad[index], d); // the choices of a row differ; a caller's own may not
+    __syncwarp();
+    for (int e = lane; e < a.experts; e += 32) {
+        float v = grad[e];
+        if (dense) {
+            const uint32_t k = order_key(to_f32(row[e]));
+            if (k) v -= expf(key_value(k) - top) * inverse * inner;
+        }
+        out[e] = from_f32<T>(v);
+    }
+}
+
+template <typename T> int launch_typed(const RouteArgs &a, bool backward, cudaStream_t st) {
+    const int64_t grid = (a.tokens + WARPS - 1) / WARPS;
+    if (grid > 0x7fffffff) return 3;
+    int rc;
+    if (backward) {
+        rc = launch_dependent(route_backward_kernel<T>, a, (unsigned)grid, WARPS * 32, WARPS * a.experts * sizeof(float), st);
+    } else {
+        void (*kernel)(RouteArgs) = a.experts <= 64 ? route_kernel<T, 2>
+                : a.experts <= 128                  ? route_kernel<T, 4>
+                : a.experts <= 256                  ? route_kernel<T, 8>
+                : a.experts <= 512                  ? route_kernel<T, 16>
+                                                    : route_kernel<T, 32>;
+        rc = launch_dependent(kernel, a, (unsigned)grid, WARPS * 32, 0, st);
+    }
+    if (rc == 0) count_launch();
+    return rc;
+}
+
+int launch_any(const RouteArgs &a, bool backward, cudaStream_t st) {
+    if (a.tokens == 0) return 0;
+    switch (a.dt) {
+        case DT_F32: return launch_typed<float>(a, backward, st);
+        case DT_BF16: return launch_typed<__nv_bfloat16>(a, backward, st);
+        case DT_F16: return launch_typed<__half>(a, backward, st);
+        default: return 3;
+    }
+}
+
+} // namespace
+
+int launch_route(const RouteArgs &a, cudaStream_t st) { return launch_any(a, false, st); }
+int launch_route_backward(const RouteArgs &a, cudaStream_t st) { return launch_any(a, true, st); }
+
+} // namespace qmm

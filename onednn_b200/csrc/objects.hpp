@@ -145,8 +145,22 @@ enum impl_id_t : int {
     IMPL_COUNT
 };
 
+// The operators around an expert layer's products, and dropout (api_token_ops.cu): every tensor by its argument id.
+struct token_op_t {
+    int scoring = 0, normalize = 0; // router
+    float scale = 1.f;
+    float p = 0.f; // dropout probability
+    std::map<int, dnnl_memory_desc> args;
+    const dnnl_memory_desc *find(int arg) const {
+        auto it = args.find(arg);
+        return it == args.end() ? nullptr : &it->second;
+    }
+};
+
 struct dnnl_primitive_desc {
-    dnnl_primitive_kind_t kind = dnnl_matmul; // dnnl_reorder: only src, dst and attr are used
+    // dnnl_reorder: only src, dst and attr are used; the kinds of dnnl_cuda_interop_primitive_kind_t: attr and token_op
+    dnnl_primitive_kind_t kind = dnnl_matmul;
+    token_op_t token_op;
     dnnl_engine_t engine = nullptr;
     dnnl_memory_desc src, wei, bias, dst, scratchpad;
     dnnl_primitive_attr attr;
@@ -192,6 +206,10 @@ void verbose_line(const char *operation, const dnnl_primitive_desc &pd, double m
 void profiling_begin(dnnl_stream_t s);
 void profiling_end(dnnl_stream_t s);
 void profiling_clear(dnnl_stream_t s);
+// api_token_ops.cu: the kinds of dnnl_cuda_interop_primitive_kind_t
+bool is_token_op(int kind);
+const char *token_op_name(int kind);
+dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t stream, int nargs, const dnnl_exec_arg_t *args);
 // reorder.cu: enqueues the reorder described by pd on the stream
 dnnl_status_t execute_reorder(const dnnl_primitive_desc &pd, dnnl_stream_t stream, int nargs,
         const dnnl_exec_arg_t *args);
