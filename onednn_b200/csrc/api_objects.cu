@@ -96,16 +96,19 @@ dnnl_status_t dnnl_engine_create(dnnl_engine_t *engine, dnnl_engine_kind_t kind,
         return dnnl_success;
     }
     if (index >= dnnl_engine_get_count(kind)) return dnnl_invalid_arguments;
-    cudaDeviceProp prop;
-    if (!cuda_ok(cudaGetDeviceProperties(&prop, (int)index), "cudaGetDeviceProperties")) return dnnl_runtime_error;
-    if (prop.major != 10) {
+    // (two attributes: all of the device's properties take milliseconds)
+    int major = 0, sm_count = 0;
+    if (!cuda_ok(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, (int)index), "cudaDeviceGetAttribute")
+            || !cuda_ok(cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, (int)index), "cudaDeviceGetAttribute"))
+        return dnnl_runtime_error;
+    if (major != 10) {
         set_last_error("the CUDA engine requires a compute capability 10.x device");
         return dnnl_unimplemented;
     }
     if (!cuda_ok(cudaSetDevice((int)index), "cudaSetDevice")) return dnnl_runtime_error;
     auto *e = new dnnl_engine;
     e->device = (int)index;
-    e->sm_count = prop.multiProcessorCount;
+    e->sm_count = sm_count;
     if (!cuda_ok(cudaMalloc(&e->status_word, sizeof(int)), "cudaMalloc")
             || !cuda_ok(cudaMemset(e->status_word, 0, sizeof(int)), "cudaMemset")) {
         delete e;
