@@ -186,7 +186,7 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
 
 int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, const std::map<int, char *> &at,
         const std::map<int, const int *> &offsets, void *scratch, cudaStream_t stream) {
-    const dnnl_engine &engine = *primitive.pd.engine;
+    const int sms = primitive.pd.engine->sm_count > 0 ? primitive.pd.engine->sm_count : 148;
     auto ptr = [&](int arg) -> void * { auto it = at.find(arg); return it == at.end() ? nullptr : it->second; };
     auto ends = [&](int arg) { auto it = offsets.find(arg); return it == offsets.end() ? nullptr : it->second; };
     // row pitch in elements (of a single row: its width)
@@ -229,7 +229,8 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             a.dst = (char *)ptr(DNNL_ARG_DST);
             a.offsets = const_cast<int *>(ends(DNNL_ARG_DST));
             a.positions = (int *)ptr(DNNL_ARG_DST_1); a.positions_ld = ld(DNNL_ARG_DST_1);
-            return launch_dispatch(a, (int *)scratch, engine.sm_count > 0 ? engine.sm_count : 148, stream);
+            a.status = primitive.pd.engine->status_word;
+            return launch_dispatch(a, (int *)scratch, sms, stream);
         }
         case dnnl_cuda_interop_moe_combine:
         case dnnl_cuda_interop_moe_combine_backward: {
@@ -246,10 +247,11 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             a.residual = ptr(DNNL_ARG_SRC_2); a.residual_ld = ld(DNNL_ARG_SRC_2);
             a.dst = ptr(DNNL_ARG_DST); a.dst_ld = ld(DNNL_ARG_DST);
             a.drop = drop;
+            a.status = primitive.pd.engine->status_word;
             a.diff_dst = ptr(DNNL_ARG_DIFF_DST); a.diff_dst_ld = ld(DNNL_ARG_DIFF_DST);
             a.diff_src = ptr(DNNL_ARG_DIFF_SRC);
             a.diff_weights = (float *)ptr(DNNL_ARG_DIFF_WEIGHTS); a.diff_weights_ld = ld(DNNL_ARG_DIFF_WEIGHTS);
-            return backward ? launch_combine_backward(a, stream) : launch_combine(a, stream);
+            return backward ? launch_combine_backward(a, sms, stream) : launch_combine(a, sms, stream);
         }
         default: {
             const auto *src = op.find(DNNL_ARG_SRC);
@@ -259,7 +261,7 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             a.residual = ptr(DNNL_ARG_SRC_2); a.residual_ld = ld(DNNL_ARG_SRC_2);
             a.dst = ptr(DNNL_ARG_DST); a.dst_ld = ld(DNNL_ARG_DST);
             a.drop = drop;
-            return launch_dropout(a, engine.sm_count > 0 ? engine.sm_count : 148, stream);
+            return launch_dropout(a, sms, stream);
         }
     }
 }

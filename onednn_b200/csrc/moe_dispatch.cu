@@ -19,12 +19,65 @@ namespace {
 
 constexpr int THREADS = 1024, WARPS = THREADS / 32;
 constexpr int TILE = 1024; // slots ranked at a time
+constexpr int SHARED_BYTES = 220 * 1024; // dynamic, at most
 constexpr int DIRECT_SLOTS = 2048; // up to here every CTA ranks all slots
+
+// Rows that bulk copies can move: some warps of a CTA each stream segments of rows through a ring of their own in shared
+// memory, one load in and a store to every place out, so that no register or instruction stands between.
+constexpr int MOVERS = 8, SLOTS = 3;
+constexpr int SLOT_BYTES = 8192;
 
 struct Plan {
     DispatchArgs a;
     int *counts; // [ranges][experts], of the ranges of tokens
     int ranges, range_tokens;
+    int segment, segments; // bulk copies: bytes of a segment (0: none), segments of a row
+    int ring; // where their rings begin in the dynamic shared memory
+};
+
+// One mover's ring; the whole warp calls it.
+struct Mover {
+    const Plan &p;
+    char *ring;
+    uint64_t *full; // [SLOTS]
+    int lane, mover;
+    int slot = 0; // next to be used
+    uint32_t phases = 0; // parity of each slot
+    bool failed = false;
+
+    __device__ __forceinline__ void load(int64_t item, int64_t t0, int at) {
+        if (lane != 0) return;
+        const int64_t t = t0 + item / p.segments;
+        const int from = (int)(item % p.segments) * p.segment, bytes = (int)min((int64_t)p.segment, p.a.row_bytes - from);
+        ptx::mbar_arrive_expect_tx(&full[at], bytes);
+        ptx::bulk_load(ring + at * p.segment, p.a.src + t * p.a.src_pitch + from, bytes, &full[at]);
+    }
+    // the loads of a tile's first items
+    __device__ __forceinline__ void begin(int64_t t0, int64_t items) {
+#pragma unroll
+        for (int q = 0; q < SLOTS - 1; ++q)
+            if (mover + q * MOVERS < items && !failed) load(mover + q * MOVERS, t0, (slot + q) % SLOTS);
+    }
+    __device__ __forceinline__ void move(int64_t t0, int64_t items, const int *place) {
+        for (int64_t i = mover; i < items && !failed; i += MOVERS) {
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], (phases >> slot) & 1))) {
+                failed = true;
+                break;
+            }
+            phases ^= 1u << slot;
+            const int t = (int)(i / p.segments), from = (int)(i % p.segments) * p.segment;
+            const int to = lane < p.a.choices ? place[t * p.a.choices + lane] : -1;
+            if (to >= 0)
+                ptx::bulk_store(p.a.dst + (int64_t)to * p.a.row_bytes + from, ring + slot * p.segment, (uint32_t)min((int64_t)p.segment, p.a.row_bytes - from));
+            ptx::bulk_commit();
+            // the slot of the item before is free once its stores have read it
+            ptx::bulk_wait_read<1>();
+            __syncwarp();
+            const int64_t ahead = i + (SLOTS - 1) * MOVERS;
+            if (ahead < items) load(ahead, t0, (slot + SLOTS - 1) % SLOTS);
+            slot = (slot + 1) % SLOTS;
+        }
+    }
 };
 
 __device__ __forceinline__ int slot_expert(const DispatchArgs &a, int slot) {
@@ -55,16 +108,29 @@ template <typename U> __device__ __forceinline__ void store_unit(const DispatchA
         if (place[j] >= 0) *((U *)(a.dst + (int64_t)place[j] * a.row_bytes) + u) = v;
 }
 
-template <typename U, bool DIRECT> __global__ void __launch_bounds__(THREADS) dispatch_kernel(const __grid_constant__ Plan p) {
-    extern __shared__ __align__(16) int shared[];
+template <typename U, bool DIRECT, bool BULK> __global__ void __launch_bounds__(THREADS) dispatch_kernel(const __grid_constant__ Plan p) {
+    extern __shared__ __align__(128) int shared[];
     __shared__ int scan[WARPS], kept;
+    __shared__ uint64_t full[MOVERS][SLOTS];
     const DispatchArgs &a = p.a;
     int *base = shared, *total = base + a.experts; // per expert: next free place, number of slots
     int *place = total + a.experts; // positions of a tile's slots (DIRECT: of all slots)
     unsigned short *table = (unsigned short *)(place + (DIRECT ? DIRECT_SLOTS : TILE)); // [warp][expert]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
     const int n = a.tokens * a.choices;
+    // the tokens whose positions this CTA writes down, and (not DIRECT) whose rows it moves
+    const int first = DIRECT ? (int)((int64_t)a.tokens * blockIdx.x / gridDim.x) : blockIdx.x * p.range_tokens;
+    const int last = DIRECT ? (int)((int64_t)a.tokens * (blockIdx.x + 1) / gridDim.x)
+                            : (int)min((int64_t)a.tokens, (int64_t)first + p.range_tokens);
+    const int tile_tokens = TILE / a.choices;
+    if (BULK && tid == 0) {
+        for (int i = 0; i < MOVERS * SLOTS; ++i) ptx::mbar_init(&full[0][0] + i, 1);
+        ptx::fence_barrier_init();
+    }
+    __syncthreads();
     ptx::grid_dependency_wait();
+    Mover mover {p, (char *)shared + p.ring + warp * (SLOTS * p.segment), full[BULK ? warp % MOVERS : 0], lane, warp};
+    if (BULK && warp < MOVERS) mover.begin(first, (int64_t)min(tile_tokens, last - first) * p.segments);
 
     for (int e = tid; e < a.experts; e += THREADS) base[e] = total[e] = 0;
     __syncthreads();
@@ -118,11 +184,6 @@ template <typename U, bool DIRECT> __global__ void __launch_bounds__(THREADS) di
     __syncthreads();
 
     const int64_t units = a.row_bytes / sizeof(U);
-    // the tokens whose positions this CTA writes down, and (not DIRECT) whose rows it moves
-    const int first = DIRECT ? (int)((int64_t)a.tokens * blockIdx.x / gridDim.x) : blockIdx.x * p.range_tokens;
-    const int last = DIRECT ? (int)((int64_t)a.tokens * (blockIdx.x + 1) / gridDim.x)
-                            : (int)min((int64_t)a.tokens, (int64_t)first + p.range_tokens);
-    const int tile_tokens = TILE / a.choices;
     for (int t0 = DIRECT ? 0 : first; t0 < (DIRECT ? a.tokens : last); t0 += tile_tokens) {
         const int t1 = min(t0 + tile_tokens, DIRECT ? a.tokens : last), slots = (t1 - t0) * a.choices;
         const int warps = (slots + 31) / 32;
@@ -150,7 +211,13 @@ template <typename U, bool DIRECT> __global__ void __launch_bounds__(THREADS) di
         }
         __syncthreads();
         if (tid < a.experts) base[tid] += tile_count;
-        if constexpr (!DIRECT) {
+        if constexpr (BULK) {
+            if (warp < MOVERS) {
+                const int64_t items = (int64_t)(t1 - t0) * p.segments;
+                if (t0 != first) mover.begin(t0, items);
+                mover.move(t0, items, place);
+            }
+        } else if constexpr (!DIRECT) {
             const int64_t work = (int64_t)(t1 - t0) * units;
             constexpr int FLIGHT = 4;
             for (int64_t i0 = tid; i0 < work; i0 += (int64_t)THREADS * FLIGHT) {
@@ -182,15 +249,42 @@ template <typename U, bool DIRECT> __global__ void __launch_bounds__(THREADS) di
     const int64_t tail = (int64_t)(n - kept) * units;
     U *behind = (U *)(a.dst + (int64_t)kept * a.row_bytes);
     for (int64_t i = (int64_t)blockIdx.x * THREADS + tid; i < tail; i += (int64_t)gridDim.x * THREADS) behind[i] = zero;
+    if (BULK && warp < MOVERS) {
+        ptx::bulk_wait_all();
+        if (mover.failed) { // a load may still be on its way: it lands before the memory goes
+            for (int s = 0; s < SLOTS; ++s)
+                for (int parity = 0; parity < 2; ++parity) (void)ptx::mbar_wait(&mover.full[s], parity, 500000000ull);
+            if (lane == 0 && a.status) atomicExch(a.status, 5);
+        }
+    }
 }
 
-template <typename U> int launch_unit(const Plan &p, bool direct, unsigned grid, cudaStream_t st) {
-    const size_t smem = p.a.experts * (2 * sizeof(int) + WARPS * sizeof(short)) + (direct ? DIRECT_SLOTS : TILE) * sizeof(int);
-    static std::atomic<unsigned long long> done_direct, done_ranges;
-    const int most = TOKEN_MAX_EXPERTS * (2 * sizeof(int) + WARPS * sizeof(short)) + DIRECT_SLOTS * sizeof(int);
-    auto kernel = direct ? dispatch_kernel<U, true> : dispatch_kernel<U, false>;
-    if (!opt_in_dynamic_smem(kernel, most, direct ? done_direct : done_ranges)) return 5;
-    return launch_dependent(kernel, p, grid, THREADS, smem, st);
+size_t plan_bytes(int experts, bool direct) {
+    return experts * (2 * sizeof(int) + WARPS * sizeof(short)) + (direct ? DIRECT_SLOTS : TILE) * sizeof(int);
+}
+
+template <typename U, bool DIRECT, bool BULK> int launch_kernel(const Plan &p, size_t smem, unsigned grid, cudaStream_t st) {
+    static std::atomic<unsigned long long> done;
+    if (!opt_in_dynamic_smem(dispatch_kernel<U, DIRECT, BULK>, SHARED_BYTES, done)) return 5;
+    return launch_dependent(dispatch_kernel<U, DIRECT, BULK>, p, grid, THREADS, smem, st);
+}
+
+template <typename U> int launch_unit(Plan &p, bool direct, unsigned grid, cudaStream_t st) {
+    const size_t plan = plan_bytes(p.a.experts, direct);
+    if (direct) return launch_kernel<U, true, false>(p, plan, grid, st);
+    if constexpr (sizeof(U) == 16) {
+        if (p.a.row_bytes >= 512) {
+            p.ring = (int)((plan + 127) / 128 * 128);
+            const int64_t most = std::min<int64_t>(SLOT_BYTES, (SHARED_BYTES - p.ring) / (MOVERS * SLOTS) / 128 * 128);
+            // rows in equal segments, and segments enough for every mover of a short range
+            const int64_t wanted = std::max<int64_t>((p.a.row_bytes + most - 1) / most,
+                    std::min<int64_t>((MOVERS + p.range_tokens - 1) / p.range_tokens, p.a.row_bytes / 1024));
+            p.segment = (int)(((p.a.row_bytes + wanted - 1) / wanted + 127) / 128 * 128);
+            p.segments = (int)((p.a.row_bytes + p.segment - 1) / p.segment);
+            return launch_kernel<U, false, true>(p, p.ring + MOVERS * SLOTS * p.segment, grid, st);
+        }
+    }
+    return launch_kernel<U, false, false>(p, plan, grid, st);
 }
 
 } // namespace

@@ -43,6 +43,7 @@ struct DispatchArgs {
     int *offsets; // [experts], cumulative ends
     int *positions;
     int64_t positions_ld;
+    int *status; // the engine's status word
 };
 int launch_dispatch(const DispatchArgs &a, int *scratch, int sm_count, cudaStream_t st);
 size_t dispatch_scratch_bytes(int experts, int sm_count);
@@ -70,6 +71,7 @@ struct CombineArgs {
     void *dst;
     int64_t dst_ld;
     DropoutState drop;
+    int *status; // the engine's status word
     // backward
     const void *diff_dst;
     int64_t diff_dst_ld;
@@ -77,8 +79,8 @@ struct CombineArgs {
     float *diff_weights;
     int64_t diff_weights_ld;
 };
-int launch_combine(const CombineArgs &a, cudaStream_t st);
-int launch_combine_backward(const CombineArgs &a, cudaStream_t st);
+int launch_combine(const CombineArgs &a, int sm_count, cudaStream_t st);
+int launch_combine_backward(const CombineArgs &a, int sm_count, cudaStream_t st);
 
 struct DropoutArgs {
     int64_t rows, cols;

@@ -57,6 +57,10 @@ template <typename T> struct Cols<T, true> {
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4 *>(part)[i];
         }
     }
+    __device__ __forceinline__ void load_shared(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4 *>(p)[i];
+    }
     __device__ __forceinline__ void get(float (&v)[8]) const {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
