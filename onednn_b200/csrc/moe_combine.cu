@@ -73,26 +73,38 @@ __device__ __forceinline__ void fma2(float &a0, float &a1, float w, float v0, fl
         : "+f"(a0), "+f"(a1) : "f"(w), "f"(v0), "f"(v1));
 }
 
-// The same sum for many tokens: one CTA per SM, whose first warp streams the rows' segments through a ring of stages in
+// The same sum for many tokens: one CTA per SM, whose first warps stream rows (and residuals) through a ring of stages in
 // shared memory with bulk copies - as many bytes in flight as the ring holds, whatever the other warps do - and whose
-// others sum them.  An item is a segment of up to 2048 columns of one token, a stage its rows' segments.
-constexpr int BULK_WARPS = 8; // that sum an item: 8 columns a thread
-constexpr int BULK_GROUPS = 3; // of such warps, which take the items in turn
-constexpr int BULK_THREADS = 32 + BULK_GROUPS * BULK_WARPS * 32;
-constexpr int BULK_COLS = BULK_WARPS * 32 * 8;
-constexpr int BULK_MAX_STAGES = 16;
-constexpr int BULK_RING = 200 * 1024;
+// others sum them.  An item fills a stage: a segment of up to 2048 columns of one token, or several tokens whose rows are
+// shorter.  A group of four warps works on an item, 16 columns a thread; the groups take the items in turn.
+// Three warps issue the copies: one takes about 0.4 us an item and 0.04 us a row, which held 8192 tokens x 8 rows x 4096 bf16
+// with dropout at 116 us and 4096 x 8 x 512 at 14.6 (three: 101 and 9.0; four: no better).
+constexpr int BULK_WARPS = 4, BULK_GROUPS = 6;
+constexpr int PRODUCERS = 3;
+constexpr int BULK_THREADS = (PRODUCERS + BULK_GROUPS * BULK_WARPS) * 32;
+constexpr int WARP_COLS = 512;
+constexpr int BULK_MAX_STAGES = 24;
+constexpr int BULK_RING = 208 * 1024;
 
 struct BulkPlan {
     CombineArgs a;
-    int segment; // columns of an item
-    int stages;
+    int warps; // of a token's segment
+    uint32_t segments; // of a token's columns
+    uint32_t items;
+    int tokens; // of an item
+    int stride; // elements from row to row of a stage
+    int residuals; // bytes from a stage's beginning to its residuals
+    int stage_bytes;
+    int stages; // a multiple of the groups: a stage always serves the same group
+    int groups; // at work
 };
 
 template <typename S, typename D, bool DROP>
 __global__ void __launch_bounds__(BULK_THREADS, 1) combine_bulk_kernel(const __grid_constant__ BulkPlan p) {
     extern __shared__ __align__(128) char ring[];
     __shared__ uint64_t full[BULK_MAX_STAGES], empty[BULK_MAX_STAGES];
+    __shared__ float weights[BULK_MAX_STAGES][32]; // of an item's rows
+    __shared__ uint32_t present[BULK_MAX_STAGES]; // its rows that are there
     __shared__ int late; // a wait ran out
     const CombineArgs &a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -106,38 +118,74 @@ __global__ void __launch_bounds__(BULK_THREADS, 1) combine_bulk_kernel(const __g
     }
     __syncthreads();
     ptx::grid_dependency_wait();
-    const uint32_t segments = (uint32_t)((a.cols + p.segment - 1) / p.segment);
-    const int64_t items = a.tokens * segments;
-    const int row_bytes = p.segment * (int)sizeof(S), stage_bytes = a.choices * row_bytes;
-    auto token_of = [&](int64_t i) { return items <= 0xffffffff ? (int64_t)((uint32_t)i / segments) : i / segments; };
-    // lane j: position (and weight) of choice j, fetched an item ahead
-    auto position = [&](int64_t t) { return lane < a.choices ? ptx::ld_dependent(a.positions + t * a.positions_ld + lane) : -1; };
-    auto weight = [&](int64_t t) { return lane < a.choices && a.weights ? ptx::ld_dependent(a.weights + t * a.weights_ld + lane) : 1.f; };
-    int64_t item = blockIdx.x;
-    int stage = 0;
-    uint32_t phase = 0;
+    const uint32_t segments = p.segments, items = p.items;
+    const int segment = p.warps * WARP_COLS;
     bool failed = false;
-    if (warp == 0) {
-        int pos = item < items ? position(token_of(item)) : -1;
-        for (; item < items; item += gridDim.x) {
-            const int64_t next = item + gridDim.x, t = token_of(item);
-            const int next_pos = next < items ? position(token_of(next)) : -1;
-            const int64_t col = (item - t * segments) * p.segment;
-            const uint32_t bytes = (uint32_t)min((int64_t)p.segment, a.cols - col) * (uint32_t)sizeof(S);
+    if (warp < PRODUCERS) {
+        // Serves every PRODUCERS-th group, in the order of their items.  A lane holds position and weight of a row; as many
+        // items as have lanes are fetched together, two batches ahead.
+        const int k = a.choices, rows = p.tokens * k, batch = 32 / rows;
+        const int of = lane / rows, row = lane - of * rows; // the lane's item of a batch, and its row there
+        const uint32_t served = max(1, (p.groups - warp + PRODUCERS - 1) / PRODUCERS), depth = p.stages / p.groups;
+        auto item_of = [&](uint32_t turn, uint32_t &group, uint32_t &round) {
+            round = turn / served;
+            group = warp + PRODUCERS * (turn - round * served);
+            return blockIdx.x + gridDim.x * (round * p.groups + group);
+        };
+        auto fetch = [&](uint32_t first, int &pos, float &w) {
+            uint32_t group, round;
+            const uint32_t item = item_of(first + of, group, round);
+            const int64_t t = (int64_t)(item / segments) * p.tokens + row / k;
+            pos = -1;
+            w = 1.f;
+            if (of < batch && item < items && t < a.tokens) {
+                pos = ptx::ld_dependent(a.positions + t * a.positions_ld + row % k);
+                if (a.weights) w = ptx::ld_dependent(a.weights + t * a.weights_ld + row % k);
+            }
+        };
+        int pos, next_pos, last_pos;
+        float w, next_w, last_w;
+        fetch(0, pos, w);
+        fetch(batch, next_pos, next_w);
+        bool more = warp < p.groups;
+        for (uint32_t first = 0; more; first += batch) {
+            fetch(first + 2 * batch, last_pos, last_w);
             const bool there = (uint32_t)pos < a.rows;
-            if (!__all_sync(0xffffffffu, ptx::mbar_wait(&empty[stage], phase ^ 1))) {
-                failed = true;
-                break;
+            const uint32_t all = __ballot_sync(0xffffffffu, there);
+            for (int b = 0; b < batch; ++b) {
+                uint32_t group, round;
+                const uint32_t item = item_of(first + b, group, round), part = item / segments;
+                if (item >= items) {
+                    more = false;
+                    break;
+                }
+                const uint32_t turns = round / depth, stage = group + p.groups * (round - turns * depth);
+                const int64_t t0 = (int64_t)part * p.tokens, col = (int64_t)(item - part * segments) * segment;
+                const uint32_t cols = (uint32_t)min((int64_t)segment, a.cols - col);
+                const int tokens = (int)min((int64_t)p.tokens, a.tokens - t0);
+                const uint32_t mask = (all >> (b * rows)) & (rows == 32 ? 0xffffffffu : (1u << rows) - 1);
+                if (!__all_sync(0xffffffffu, ptx::mbar_wait(&empty[stage], ~turns & 1))) {
+                    failed = true;
+                    more = false;
+                    break;
+                }
+                if (of == b) weights[stage][row] = DROP ? w * a.drop.scale : w; // (one product a row instead of one an element)
+                if (lane == 0) present[stage] = mask;
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive_expect_tx(&full[stage], __popc(mask) * cols * (uint32_t)sizeof(S) + (a.residual ? tokens * cols * (uint32_t)sizeof(D) : 0));
+                __syncwarp();
+                char *at = ring + stage * p.stage_bytes;
+                if (of == b && there)
+                    ptx::bulk_load(at + row * p.stride * (int)sizeof(S), (const S *)a.src + (int64_t)pos * a.cols + col, cols * (uint32_t)sizeof(S), &full[stage]);
+                if (a.residual && lane < tokens)
+                    ptx::bulk_load(at + p.residuals + lane * p.stride * (int)sizeof(D), (const D *)a.residual + (t0 + lane) * a.residual_ld + col,
+                            cols * (uint32_t)sizeof(D), &full[stage]);
             }
-            const uint32_t rows = __popc(__ballot_sync(0xffffffffu, there));
-            if (lane == 0) ptx::mbar_arrive_expect_tx(&full[stage], rows * bytes);
-            __syncwarp();
-            if (there) ptx::bulk_load(ring + stage * stage_bytes + lane * row_bytes, (const S *)a.src + (int64_t)pos * a.cols + col, bytes, &full[stage]);
             pos = next_pos;
-            if (++stage == p.stages) {
-                stage = 0;
-                phase ^= 1;
-            }
+            w = next_w;
+            next_pos = last_pos;
+            next_w = last_w;
         }
     } else {
         uint64_t seed = 0, offset = 0;
@@ -145,79 +193,88 @@ __global__ void __launch_bounds__(BULK_THREADS, 1) combine_bulk_kernel(const __g
             seed = ld_dependent_u64(a.drop.seed);
             offset = ld_dependent_u64(a.drop.seed + 1);
         }
-        const int group = (warp - 1) / BULK_WARPS;
-        const int mine = ((warp - 1) % BULK_WARPS * 32 + lane) * 8; // first column within the segment
-        const bool active = mine < p.segment;
-        auto column = [&](int64_t i, int64_t t) { return (i - t * segments) * p.segment + mine; };
-        Cols<D, true> res, next_res;
-        int64_t t = 0, tn = 0;
-        int pos = -1;
-        float w = 1.f;
-        const int64_t step = (int64_t)gridDim.x * BULK_GROUPS;
-        item += (int64_t)gridDim.x * group;
-        stage = group;
-        while (stage >= p.stages) {
-            stage -= p.stages;
-            phase ^= 1;
-        }
-        if (item < items) {
-            t = token_of(item);
-            pos = position(t);
-            w = weight(t);
-            if (a.residual && active) res.load((const D *)a.residual + t * a.residual_ld, column(item, t), a.cols);
-        }
-        for (; item < items; item += step) {
-            const int64_t next = item + step, col = column(item, t);
-            int next_pos = -1;
-            float next_w = 1.f;
-            if (next < items) {
-                tn = token_of(next);
-                next_pos = position(tn);
-                next_w = weight(tn);
-                if (a.residual && active) next_res.load((const D *)a.residual + tn * a.residual_ld, column(next, tn), a.cols);
-            }
-            const uint32_t there = __ballot_sync(0xffffffffu, (uint32_t)pos < a.rows);
-            float acc[8];
+        const int group = (warp - PRODUCERS) / BULK_WARPS, part = (warp - PRODUCERS) % BULK_WARPS;
+        const int token = part / p.warps; // the warp's token of an item
+        const int mine = (part - token * p.warps) * WARP_COLS + lane * 8; // and its first column of the segment; more 256 on
+        // A wait knows a phase by its parity only, so nobody may come to a stage's next phase before its last has ended: the
+        // stages of a group are its own, and it has seen them end.
+        int stage = group;
+        uint32_t phase = 0;
+        for (uint32_t item = group < p.groups ? blockIdx.x + gridDim.x * group : items; item < items; item += gridDim.x * p.groups) {
+            const uint32_t q = item / segments;
+            const int64_t t = (int64_t)q * p.tokens + token, col = (int64_t)(item - q * segments) * segment + mine;
+            const bool work = token < p.tokens && t < a.tokens;
+            const bool on[2] = {work && col < a.cols, work && col + 256 < a.cols};
+            float acc[2][8];
 #pragma unroll
-            for (int n = 0; n < 8; ++n) acc[n] = 0.f;
+            for (int n = 0; n < 16; ++n) acc[n / 8][n % 8] = 0.f;
+            Cols<D, true> res[2];
             if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[stage], phase))) {
                 failed = true;
                 break;
             }
-            const S *rows = (const S *)(ring + stage * stage_bytes) + mine;
-            for (int j0 = 0; j0 < a.choices; j0 += GROUP) {
+            if (work) {
+                const char *at = ring + stage * p.stage_bytes;
+                const S *rows = (const S *)at + token * a.choices * p.stride + mine;
+                const float *w = &weights[stage][token * a.choices];
+                const uint32_t there = present[stage] >> (token * a.choices);
+                auto add = [&](int j) {
+                    const float wj = w[j];
 #pragma unroll
-                for (int j = 0; j < GROUP; ++j) {
-                    const float wj = __shfl_sync(0xffffffffu, w, (j0 + j) & 31);
-                    if (j0 + j < 32 && (there >> (j0 + j)) & 1) {
-                        Cols<S, true> x;
-                        if (active) x.load_shared(rows + (j0 + j) * p.segment);
-                        float v[8];
-                        x.get(v);
+                    for (int h = 0; h < 2; ++h)
+                        if (on[h]) {
+                            Cols<S, true> x;
+                            x.load_shared(rows + j * p.stride + 256 * h);
+                            float v[8];
+                            x.get(v);
 #pragma unroll
-                        for (int n = 0; n < 8; n += 2) fma2(acc[n], acc[n + 1], wj, v[n], v[n + 1]);
+                            for (int n = 0; n < 8; n += 2) fma2(acc[h][n], acc[h][n + 1], wj, v[n], v[n + 1]);
+                        }
+                };
+                const uint32_t every = a.choices == 32 ? 0xffffffffu : (1u << a.choices) - 1;
+                if ((there & every) == every) {
+                    int j = 0;
+                    for (; j + 4 <= a.choices; j += 4) {
+                        add(j);
+                        add(j + 1);
+                        add(j + 2);
+                        add(j + 3);
                     }
+                    for (; j < a.choices; ++j) add(j);
+                } else {
+                    for (int j = 0; j < a.choices; ++j)
+                        if ((there >> j) & 1) add(j);
                 }
+                if (a.residual)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (on[h]) res[h].load_shared((const D *)(at + p.residuals) + token * p.stride + mine + 256 * h);
             }
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&empty[stage]);
-            if (active && col < a.cols) {
-                if constexpr (DROP) apply_dropout<true>(acc, a.drop, seed, offset, t, a.cols, col, nullptr);
-                if (a.residual) {
-                    float v[8];
-                    res.get(v);
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) acc[n] += v[n];
+            if constexpr (DROP) {
+                if (on[0]) {
+                    uint32_t u[2][8];
+                    random_words<true>(u[0], seed, offset, t, a.cols, col, nullptr);
+                    random_words<true>(u[1], seed, offset, t, a.cols, col + 256, nullptr);
+                    drop(acc[0], u[0], a.drop);
+                    drop(acc[1], u[1], a.drop);
                 }
-                Cols<D, true>::store((D *)a.dst + t * a.dst_ld, col, a.cols, acc);
             }
-            t = tn;
-            pos = next_pos;
-            w = next_w;
-            res = next_res;
-            stage += BULK_GROUPS;
-            while (stage >= p.stages) {
-                stage -= p.stages;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (on[h]) {
+                    if (a.residual) {
+                        float v[8];
+                        res[h].get(v);
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) acc[h][n] += v[n];
+                    }
+                    Cols<D, true>::store((D *)a.dst + t * a.dst_ld, col + 256 * h, a.cols, acc[h]);
+                }
+            stage += p.groups;
+            if (stage >= p.stages) {
+                stage = group;
                 phase ^= 1;
             }
         }
@@ -323,21 +380,34 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const __grid_cons
 template <typename S, typename D, bool DROP> int launch_bulk(const CombineArgs &a, int sm_count, cudaStream_t st) {
     BulkPlan p {};
     p.a = a;
-    // stages of at least four to the ring, segments of whole warps' shares
-    const int most = BULK_RING / 4 / (a.choices * (int)sizeof(S)) / 256 * 256;
-    const int wide = (int)std::min<int64_t>(BULK_COLS, (a.cols + 255) / 256 * 256);
-    p.segment = std::max(256, std::min(most, wide));
-    p.stages = std::min(BULK_MAX_STAGES, BULK_RING / (a.choices * p.segment * (int)sizeof(S)));
-    const int64_t items = a.tokens * ((a.cols + p.segment - 1) / p.segment);
+    const int row = a.choices * (int)sizeof(S) + (a.residual ? (int)sizeof(D) : 0); // bytes per column of a token
+    const int most = BULK_RING / 4; // four stages at least
+    p.warps = (int)std::min<int64_t>(BULK_WARPS, (a.cols + WARP_COLS - 1) / WARP_COLS);
+    while (p.warps > 1 && row * p.warps * WARP_COLS > most) --p.warps;
+    p.segments = (uint32_t)((a.cols + p.warps * WARP_COLS - 1) / (p.warps * WARP_COLS));
+    p.stride = p.segments == 1 ? (int)((a.cols + 7) / 8 * 8) : p.warps * WARP_COLS;
+    p.tokens = p.segments == 1 ? std::min(BULK_WARPS / p.warps, 32 / a.choices) : 1;
+    while (p.tokens > 1 && row * p.tokens * p.stride > most) --p.tokens;
+    p.residuals = p.tokens * a.choices * p.stride * (int)sizeof(S);
+    p.stage_bytes = p.tokens * row * p.stride;
+    const int room = std::min(BULK_MAX_STAGES, BULK_RING / p.stage_bytes);
+    p.groups = std::min(room, BULK_GROUPS);
+    for (int g = p.groups - 1; g >= 4 && g > p.groups - 6; --g) // as many as leave the least of the ring unused
+        if (room / g * g > room / p.groups * p.groups) p.groups = g;
+    p.stages = room / p.groups * p.groups;
+    p.items = (uint32_t)((a.tokens + p.tokens - 1) / p.tokens * p.segments);
     static std::atomic<unsigned long long> done;
     if (!opt_in_dynamic_smem(combine_bulk_kernel<S, D, DROP>, BULK_RING, done)) return 5;
-    return launch_dependent(combine_bulk_kernel<S, D, DROP>, p, (unsigned)std::min<int64_t>(items, sm_count), BULK_THREADS, BULK_RING, st);
+    return launch_dependent(combine_bulk_kernel<S, D, DROP>, p, std::min<unsigned>(p.items, sm_count), BULK_THREADS, BULK_RING, st);
 }
 
 template <typename S, typename D, bool DROP> int launch_forward(const CombineArgs &a, bool vec, int sm_count, cudaStream_t st) {
     const int64_t total = a.tokens * (vec ? row_units<true>(a.cols, DROP) : row_units<false>(a.cols, DROP));
     const int64_t grid = (total + 255) / 256;
-    if (vec && a.cols * (int64_t)sizeof(S) % 16 == 0 && a.cols * (int64_t)sizeof(S) >= 1024 && a.tokens >= 4 * sm_count)
+    // Below 2 KB a row or 2^21 sums the ring's start and the copies' number cost more than they give.  us a call, thread by
+    // thread / bulk, bf16, k = 8: 600 x 4096 7.9 / 7.5, 400 x 4096 5.8 / 6.0, 4096 x 512 7.4 / 9.0; k = 1: 4096 x 1024 8.3 / 6.7.
+    if (vec && a.cols % 8 == 0 && a.cols * (int64_t)sizeof(S) >= 2048 && a.tokens * a.cols >= (1 << 21)
+            && a.tokens * ((a.cols + WARP_COLS - 1) / WARP_COLS) < (1 << 30) && !a.drop.drop_all)
         return launch_bulk<S, D, DROP>(a, sm_count, st);
     if (grid > 0x7fffffff) return 3;
     return launch_dependent(vec ? combine_kernel<S, D, true, DROP> : combine_kernel<S, D, false, DROP>, a, (unsigned)grid, 256, 0, st);

@@ -151,9 +151,8 @@ __device__ __forceinline__ uint4 philox(uint64_t seed, uint64_t offset, uint64_t
 // logical dims) uses word i % 4 of block i / 4.  A dropped element is zero whatever it was, infinities and NaN included.
 // `words`: 128 words of shared memory of this warp's own (unused by VEC); the whole warp calls it.
 template <bool VEC, int N>
-__device__ __forceinline__ void apply_dropout(float (&v)[N], const DropoutState &d, uint64_t seed, uint64_t offset, int64_t t,
-        int64_t cols, int64_t col, uint32_t *words) {
-    uint32_t u[N];
+__device__ __forceinline__ void random_words(uint32_t (&u)[N], uint64_t seed, uint64_t offset, int64_t t, int64_t cols, int64_t col,
+        uint32_t *words) {
     if constexpr (VEC) {
         const uint64_t block = (uint64_t)(t * cols + col) >> 2;
         const uint4 a = philox(seed, offset, block), b = philox(seed, offset, block + 1);
@@ -168,8 +167,24 @@ __device__ __forceinline__ void apply_dropout(float (&v)[N], const DropoutState 
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = words[32 * i + lane];
     }
+}
+template <int N> __device__ __forceinline__ void drop(float (&v)[N], const uint32_t (&u)[N], const DropoutState &d) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = u[i] >= d.threshold && !d.drop_all ? v[i] * d.scale : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = u[i] >= d.threshold ? v[i] : 0.f;
+}
+template <bool VEC, int N>
+__device__ __forceinline__ void apply_dropout(float (&v)[N], const DropoutState &d, uint64_t seed, uint64_t offset, int64_t t,
+        int64_t cols, int64_t col, uint32_t *words) {
+    if (d.drop_all) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = 0.f;
+        return;
+    }
+    uint32_t u[N];
+    random_words<VEC>(u, seed, offset, t, cols, col, words);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= d.scale;
+    drop(v, u, d);
 }
 
 __device__ __forceinline__ uint64_t ld_dependent_u64(const int64_t *p) {
