@@ -1,6 +1,13 @@
 // Dropout on the way into a residual stream: dst = residual + (kept ? src / (1 - p) : 0), with the mask made from a counter
 // (token_rows.cuh) and never stored.  The gradient is the same operator on the gradient, without a residual: the same
-// (seed, offset) makes the same mask.  Elementwise, so the floor is one read of src and residual and one write of dst.
+// (seed, offset) makes the same mask.
+//
+// The floor is one read of src and residual and one write of dst; beside it stands the generator, whose 20 wide products a
+// block of four elements leave the SM at 32 a clock: 19 us for 8192 x 4096 elements, whatever their type.  Both run side by
+// side as long as nothing else fills the issue slots, so the usual form - dense tensors, one long row - computes one address
+// a tensor and keeps or drops with one comparison and one predicated multiply-add.
+#include <algorithm>
+
 #include "launch.h"
 #include "token_rows.cuh"
 
@@ -8,59 +15,150 @@ namespace qmm {
 
 namespace {
 
-constexpr int SHARES = 2; // of a thread: their loads leave together, their generators run side by side
+__device__ __forceinline__ float keep_add(uint32_t u, const DropoutState &d, float v, float residual) {
+    return u >= d.threshold ? fmaf(v, d.scale, residual) : residual;
+}
 
-template <typename T, bool VEC, bool RES>
-__global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutArgs a) {
-    __shared__ __align__(16) uint32_t shared_words[VEC ? 4 : 8 * 128];
-    uint32_t *words = shared_words + (VEC ? 0 : threadIdx.x / 32 * 128);
+// Rows that start on 16-byte boundaries, and on multiples of four elements: eight neighbouring columns a share, two shares a
+// thread at a time.  The loads leave before the generator runs, which takes longer than they do.  Where 16-bit elements leave
+// the generator in front, the grid stays, four CTAs an SM: a thread that ended after its first shares would wait for the seed
+// as often (8192 x 4096 with residual 38.6 us gone / 32.3 us staying; five CTAs 33.8, six 34.5, one share 38.1).  32-bit
+// elements wait for memory, and more CTAs on their way bring it sooner (59.2 us gone / 69 staying).
+constexpr int SHARES = 2;
+constexpr int CTAS = 4;
+
+template <typename T, bool RES, bool WHOLE>
+__device__ __forceinline__ void drop_piece(const DropoutArgs &a, uint64_t seed, uint64_t offset, const T *src, const T *residual, T *dst,
+        int64_t col, uint64_t block) {
+    constexpr int SPREAD = 256 * 8; // columns from one share of a thread to the next
+    Cols<T, true> x[SHARES], res[SHARES];
+    const int64_t end = WHOLE ? INT64_MAX : a.cols;
+#pragma unroll
+    for (int s = 0; s < SHARES; ++s)
+        if (WHOLE || col + SPREAD * s < end) {
+            x[s].load(src + SPREAD * s, 0, WHOLE ? 8 : end - col - SPREAD * s);
+            if constexpr (RES) res[s].load(residual + SPREAD * s, 0, WHOLE ? 8 : end - col - SPREAD * s);
+        }
+    uint32_t u[SHARES][8];
+#pragma unroll
+    for (int s = 0; s < SHARES; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 r = philox(seed, offset, block + SPREAD / 4 * s + h);
+            u[s][4 * h] = r.x; u[s][4 * h + 1] = r.y; u[s][4 * h + 2] = r.z; u[s][4 * h + 3] = r.w;
+        }
+#pragma unroll
+    for (int s = 0; s < SHARES; ++s)
+        if (WHOLE || col + SPREAD * s < end) {
+            float v[8], r[8];
+            x[s].get(v);
+            if constexpr (RES) res[s].get(r);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) v[n] = keep_add(u[s][n], a.drop, v[n], RES ? r[n] : 0.f);
+            Cols<T, true>::store(dst + SPREAD * s, 0, WHOLE ? 8 : end - col - SPREAD * s, v);
+        }
+}
+
+template <typename T, bool RES, bool DENSE> __global__ void __launch_bounds__(256, CTAS) dropout_rows_kernel(const __grid_constant__ DropoutArgs a) {
     ptx::grid_dependency_wait();
-    const int64_t units = row_units<VEC>(a.cols, true), total = a.rows * units;
-    const int64_t first = (int64_t)blockIdx.x * (256 * SHARES) + threadIdx.x;
-    int64_t t[SHARES], col[SHARES];
-    bool on[SHARES]; // (whole warps, where a warp works together)
-    Cols<T, VEC> x[SHARES], res[SHARES];
-#pragma unroll
-    for (int s = 0; s < SHARES; ++s) {
-        const int64_t i = first + 256 * s;
-        t[s] = a.rows == 1 ? 0 : total <= 0xffffffff ? (int64_t)((uint32_t)i / (uint32_t)units) : i / units;
-        col[s] = unit_column<VEC>(i - t[s] * units, t[s], a.cols, true);
-        on[s] = i < total;
-        if (on[s]) {
-            x[s].load((const T *)a.src + t[s] * a.src_ld, col[s], a.cols);
-            if constexpr (RES) res[s].load((const T *)a.residual + t[s] * a.residual_ld, col[s], a.cols);
+    constexpr int PIECE = 256 * 8 * SHARES; // columns of a CTA at a time
+    const uint64_t seed = same_in_warp(ld_dependent_u64(a.drop.seed)), offset = ld_dependent_u64(a.drop.seed + 1);
+    const int mine = threadIdx.x * 8;
+    if constexpr (DENSE) {
+        const int64_t step = (int64_t)gridDim.x * PIECE;
+        int64_t col = (int64_t)blockIdx.x * PIECE + mine;
+        const T *src = (const T *)a.src + col, *residual = RES ? (const T *)a.residual + col : nullptr;
+        T *dst = (T *)a.dst + col;
+        int64_t left = a.cols - (int64_t)blockIdx.x * PIECE; // from the piece's beginning
+        for (; left >= PIECE; left -= step) {
+            drop_piece<T, RES, true>(a, seed, offset, src, residual, dst, 0, (uint64_t)col >> 2);
+            col += step;
+            src += step;
+            if constexpr (RES) residual += step;
+            dst += step;
         }
-    }
-    const uint64_t seed = ld_dependent_u64(a.drop.seed), offset = ld_dependent_u64(a.drop.seed + 1);
-    constexpr int N = Cols<T, VEC>::N;
-    uint32_t u[SHARES][N];
-#pragma unroll
-    for (int s = 0; s < SHARES; ++s) random_words<VEC>(u[s], seed, offset, t[s], a.cols, col[s], words);
-#pragma unroll
-    for (int s = 0; s < SHARES; ++s) {
-        if (!on[s]) continue;
-        float v[N], r[N];
-        x[s].get(v);
-#pragma unroll
-        for (int n = 0; n < N; ++n) v[n] = a.drop.drop_all ? 0.f : v[n] * a.drop.scale;
-        drop(v, u[s], a.drop);
-        if constexpr (RES) {
-            res[s].get(r);
-#pragma unroll
-            for (int n = 0; n < N; ++n) v[n] += r[n];
+        if (left > 0) drop_piece<T, RES, false>(a, seed, offset, src, residual, dst, col, (uint64_t)col >> 2);
+    } else {
+        const int64_t pieces = (a.cols + PIECE - 1) / PIECE, total = a.rows * pieces;
+        for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+            const int64_t t = total <= 0xffffffff ? (int64_t)((uint32_t)i / (uint32_t)pieces) : i / pieces;
+            const int64_t col = (i - t * pieces) * PIECE + mine;
+            const T *src = (const T *)a.src + t * a.src_ld + col, *residual = (const T *)a.residual + t * a.residual_ld + col;
+            T *dst = (T *)a.dst + t * a.dst_ld + col;
+            const uint64_t block = (uint64_t)(t * a.cols + col) >> 2;
+            if (col - mine + PIECE <= a.cols) drop_piece<T, RES, true>(a, seed, offset, src, residual, dst, col, block);
+            else drop_piece<T, RES, false>(a, seed, offset, src, residual, dst, col, block);
         }
-        Cols<T, VEC>::store((T *)a.dst + t[s] * a.dst_ld, col[s], a.cols, v);
     }
 }
 
-template <typename T> int launch_typed(const DropoutArgs &a, cudaStream_t st) {
+// Rows that start anywhere: a warp takes 256 columns, 32 beside one another at a time, so that its accesses stay contiguous;
+// the 256 begin at a multiple of four elements of the whole tensor, up to three columns before the row, and the words of
+// their 64 blocks go through shared memory to the lanes that need them.
+constexpr int SPAN = 256;
+
+template <typename T, bool RES> __global__ void __launch_bounds__(256) dropout_any_kernel(const __grid_constant__ DropoutArgs a) {
+    __shared__ __align__(16) uint32_t shared_words[8 * SPAN];
+    ptx::grid_dependency_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    uint32_t *words = shared_words + warp * SPAN;
+    const int64_t spans = (a.cols + 3 + SPAN - 1) / SPAN, item = (int64_t)blockIdx.x * 8 + warp;
+    const int64_t t = a.rows * spans <= 0xffffffff ? (int64_t)((uint32_t)item / (uint32_t)spans) : item / spans;
+    if (t >= a.rows) return;
+    const int64_t start = t * a.cols, begin = (item - t * spans) * SPAN - (start & 3); // the span's first column
+    const T *src = (const T *)a.src + t * a.src_ld + begin, *residual = (const T *)a.residual + t * a.residual_ld + begin;
+    T *dst = (T *)a.dst + t * a.dst_ld + begin;
+    // columns of the span that are there: [low, high)
+    const int low = begin < 0 ? (int)-begin : 0, high = (int)min((int64_t)SPAN, a.cols - begin);
+    T x[SPAN / 32], res[SPAN / 32];
+#pragma unroll
+    for (int i = 0; i < SPAN / 32; ++i) {
+        const int c = 32 * i + lane;
+        if (c >= low && c < high) {
+            x[i] = src[c];
+            if constexpr (RES) res[i] = residual[c];
+        }
+    }
+    const uint64_t seed = ld_dependent_u64(a.drop.seed), offset = ld_dependent_u64(a.drop.seed + 1);
+    const uint64_t block = (uint64_t)(start + begin) >> 2;
+    reinterpret_cast<uint4 *>(words)[lane] = philox(seed, offset, block + lane);
+    reinterpret_cast<uint4 *>(words)[lane + 32] = philox(seed, offset, block + lane + 32);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < SPAN / 32; ++i) {
+        const int c = 32 * i + lane;
+        if (c >= low && c < high) dst[c] = from_f32<T>(keep_add(words[c], a.drop, to_f32(x[i]), RES ? to_f32(res[i]) : 0.f));
+    }
+}
+
+// p = 1: nothing is kept, and no comparison with a 32-bit word says so
+template <typename T> __global__ void __launch_bounds__(256) dropout_all_kernel(const __grid_constant__ DropoutArgs a) {
+    ptx::grid_dependency_wait();
+    const int64_t total = a.rows * a.cols;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / a.cols, c = i - t * a.cols;
+        ((T *)a.dst)[t * a.dst_ld + c] = a.residual ? ((const T *)a.residual)[t * a.residual_ld + c] : from_f32<T>(0.f);
+    }
+}
+
+template <typename T> int launch_typed(const DropoutArgs &a, int sm_count, cudaStream_t st) {
     const bool vec = rows_aligned(a.src, a.src_ld * sizeof(T), a.rows) && rows_aligned(a.dst, a.dst_ld * sizeof(T), a.rows)
             && (!a.residual || rows_aligned(a.residual, a.residual_ld * sizeof(T), a.rows)) && (a.cols % 4 == 0 || a.rows == 1);
-    const int64_t total = a.rows * (vec ? row_units<true>(a.cols, true) : row_units<false>(a.cols, true));
-    const int64_t grid = (total + 256 * SHARES - 1) / (256 * SHARES);
+    void (*kernel)(DropoutArgs);
+    int64_t grid;
+    if (a.drop.drop_all) {
+        kernel = dropout_all_kernel<T>;
+        grid = std::min<int64_t>((a.rows * a.cols + 255) / 256, (int64_t)sm_count * 16);
+    } else if (vec) {
+        kernel = a.rows == 1 ? (a.residual ? dropout_rows_kernel<T, true, true> : dropout_rows_kernel<T, false, true>)
+                             : (a.residual ? dropout_rows_kernel<T, true, false> : dropout_rows_kernel<T, false, false>);
+        grid = a.rows * ((a.cols + 256 * SHARES * 8 - 1) / (256 * SHARES * 8));
+        if (sizeof(T) == 2) grid = std::min(grid, (int64_t)sm_count * CTAS);
+    } else {
+        kernel = a.residual ? dropout_any_kernel<T, true> : dropout_any_kernel<T, false>;
+        grid = (a.rows * ((a.cols + 3 + SPAN - 1) / SPAN) + 7) / 8;
+    }
     if (grid > 0x7fffffff) return 3;
-    void (*kernel)(DropoutArgs) = vec ? (a.residual ? dropout_kernel<T, true, true> : dropout_kernel<T, true, false>)
-                                      : (a.residual ? dropout_kernel<T, false, true> : dropout_kernel<T, false, false>);
     const int rc = launch_dependent(kernel, a, (unsigned)grid, 256, 0, st);
     if (rc == 0) count_launch();
     return rc;
@@ -77,9 +175,9 @@ int launch_dropout(const DropoutArgs &args, int sm_count, cudaStream_t st) {
         a.rows = 1;
     }
     switch (a.dt) {
-        case DT_F32: return launch_typed<float>(a, st);
-        case DT_BF16: return launch_typed<__nv_bfloat16>(a, st);
-        case DT_F16: return launch_typed<__half>(a, st);
+        case DT_F32: return launch_typed<float>(a, sm_count, st);
+        case DT_BF16: return launch_typed<__nv_bfloat16>(a, sm_count, st);
+        case DT_F16: return launch_typed<__half>(a, sm_count, st);
         default: return 3;
     }
 }
