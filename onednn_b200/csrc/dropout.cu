@@ -7,6 +7,7 @@
 // side as long as nothing else fills the issue slots, so the usual form - dense tensors, one long row - computes one address
 // a tensor and keeps or drops with one comparison and one predicated multiply-add.
 #include <algorithm>
+#include <type_traits>
 
 #include "launch.h"
 #include "token_rows.cuh"
@@ -27,10 +28,12 @@ __device__ __forceinline__ float keep_add(uint32_t u, const DropoutState &d, flo
 constexpr int SHARES = 2;
 constexpr int CTAS = 4;
 
+constexpr int SPREAD = 256 * 8, PIECE = SPREAD * SHARES; // columns from share to share of a thread; of a CTA at a time
+
+// Dense tensors: one row.
 template <typename T, bool RES, bool WHOLE>
 __device__ __forceinline__ void drop_piece(const DropoutArgs &a, uint64_t seed, uint64_t offset, const T *src, const T *residual, T *dst,
         int64_t col, uint64_t block) {
-    constexpr int SPREAD = 256 * 8; // columns from one share of a thread to the next
     Cols<T, true> x[SHARES], res[SHARES];
     const int64_t end = WHOLE ? INT64_MAX : a.cols;
 #pragma unroll
@@ -59,36 +62,78 @@ __device__ __forceinline__ void drop_piece(const DropoutArgs &a, uint64_t seed, 
         }
 }
 
-template <typename T, bool RES, bool DENSE> __global__ void __launch_bounds__(256, CTAS) dropout_rows_kernel(const __grid_constant__ DropoutArgs a) {
+// A thread's shares begin at src[s], with left[s] columns of the row from there (WHOLE: eight at least).
+template <typename T, bool RES, bool WHOLE>
+__device__ __forceinline__ void drop_shares(const DropoutArgs &a, uint64_t seed, uint64_t offset, const T *const (&src)[SHARES],
+        const T *const (&residual)[SHARES], T *const (&dst)[SHARES], const int64_t (&left)[SHARES], const uint64_t (&block)[SHARES]) {
+    Cols<T, true> x[SHARES], res[SHARES];
+#pragma unroll
+    for (int s = 0; s < SHARES; ++s)
+        if (WHOLE || left[s] > 0) {
+            x[s].load(src[s], 0, WHOLE ? 8 : left[s]);
+            if constexpr (RES) res[s].load(residual[s], 0, WHOLE ? 8 : left[s]);
+        }
+    uint32_t u[SHARES][8];
+#pragma unroll
+    for (int s = 0; s < SHARES; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 r = philox(seed, offset, block[s] + h);
+            u[s][4 * h] = r.x; u[s][4 * h + 1] = r.y; u[s][4 * h + 2] = r.z; u[s][4 * h + 3] = r.w;
+        }
+#pragma unroll
+    for (int s = 0; s < SHARES; ++s)
+        if (WHOLE || left[s] > 0) {
+            float v[8], r[8];
+            x[s].get(v);
+            if constexpr (RES) res[s].get(r);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) v[n] = keep_add(u[s][n], a.drop, v[n], RES ? r[n] : 0.f);
+            Cols<T, true>::store(dst[s], 0, WHOLE ? 8 : left[s], v);
+        }
+}
+
+// DENSE: one row.  Otherwise shares are counted over all rows, and each finds its own.
+template <typename T, bool RES> __global__ void __launch_bounds__(256, CTAS) dropout_dense_kernel(const __grid_constant__ DropoutArgs a) {
     ptx::grid_dependency_wait();
-    constexpr int PIECE = 256 * 8 * SHARES; // columns of a CTA at a time
     const uint64_t seed = same_in_warp(ld_dependent_u64(a.drop.seed)), offset = ld_dependent_u64(a.drop.seed + 1);
-    const int mine = threadIdx.x * 8;
-    if constexpr (DENSE) {
-        const int64_t step = (int64_t)gridDim.x * PIECE;
-        int64_t col = (int64_t)blockIdx.x * PIECE + mine;
-        const T *src = (const T *)a.src + col, *residual = RES ? (const T *)a.residual + col : nullptr;
-        T *dst = (T *)a.dst + col;
-        int64_t left = a.cols - (int64_t)blockIdx.x * PIECE; // from the piece's beginning
-        for (; left >= PIECE; left -= step) {
-            drop_piece<T, RES, true>(a, seed, offset, src, residual, dst, 0, (uint64_t)col >> 2);
-            col += step;
-            src += step;
-            if constexpr (RES) residual += step;
-            dst += step;
+    const int64_t step = (int64_t)gridDim.x * PIECE;
+    int64_t col = (int64_t)blockIdx.x * PIECE + threadIdx.x * 8;
+    const T *src = (const T *)a.src + col, *residual = RES ? (const T *)a.residual + col : nullptr;
+    T *dst = (T *)a.dst + col;
+    int64_t left = a.cols - (int64_t)blockIdx.x * PIECE; // from the piece's beginning
+    for (; left >= PIECE; left -= step) {
+        drop_piece<T, RES, true>(a, seed, offset, src, residual, dst, 0, (uint64_t)col >> 2);
+        col += step;
+        src += step;
+        if constexpr (RES) residual += step;
+        dst += step;
+    }
+    if (left > 0) drop_piece<T, RES, false>(a, seed, offset, src, residual, dst, col, (uint64_t)col >> 2);
+}
+
+// Several rows: shares are counted over all of them, and each finds its own.
+template <typename T, bool RES> __global__ void __launch_bounds__(256, CTAS) dropout_rows_kernel(const __grid_constant__ DropoutArgs a) {
+    ptx::grid_dependency_wait();
+    const uint64_t seed = same_in_warp(ld_dependent_u64(a.drop.seed)), offset = ld_dependent_u64(a.drop.seed + 1);
+    const int64_t units = (a.cols + 7) / 8, total = a.rows * units;
+    for (int64_t first = (int64_t)blockIdx.x * (256 * SHARES); first < total; first += (int64_t)gridDim.x * (256 * SHARES)) {
+        const T *src[SHARES], *residual[SHARES];
+        T *dst[SHARES];
+        int64_t left[SHARES];
+        uint64_t block[SHARES];
+#pragma unroll
+        for (int s = 0; s < SHARES; ++s) {
+            const int64_t i = first + threadIdx.x + 256 * s;
+            const int64_t t = total <= 0xffffffff ? (int64_t)((uint32_t)i / (uint32_t)units) : i / units, col = (i - t * units) * 8;
+            src[s] = (const T *)a.src + t * a.src_ld + col;
+            residual[s] = (const T *)a.residual + t * a.residual_ld + col;
+            dst[s] = (T *)a.dst + t * a.dst_ld + col;
+            left[s] = i < total ? a.cols - col : 0;
+            block[s] = (uint64_t)(t * a.cols + col) >> 2;
         }
-        if (left > 0) drop_piece<T, RES, false>(a, seed, offset, src, residual, dst, col, (uint64_t)col >> 2);
-    } else {
-        const int64_t pieces = (a.cols + PIECE - 1) / PIECE, total = a.rows * pieces;
-        for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
-            const int64_t t = total <= 0xffffffff ? (int64_t)((uint32_t)i / (uint32_t)pieces) : i / pieces;
-            const int64_t col = (i - t * pieces) * PIECE + mine;
-            const T *src = (const T *)a.src + t * a.src_ld + col, *residual = (const T *)a.residual + t * a.residual_ld + col;
-            T *dst = (T *)a.dst + t * a.dst_ld + col;
-            const uint64_t block = (uint64_t)(t * a.cols + col) >> 2;
-            if (col - mine + PIECE <= a.cols) drop_piece<T, RES, true>(a, seed, offset, src, residual, dst, col, block);
-            else drop_piece<T, RES, false>(a, seed, offset, src, residual, dst, col, block);
-        }
+        if (a.cols % 8 == 0 && first + 256 * SHARES <= total) drop_shares<T, RES, true>(a, seed, offset, src, residual, dst, left, block);
+        else drop_shares<T, RES, false>(a, seed, offset, src, residual, dst, left, block);
     }
 }
 
@@ -102,32 +147,38 @@ template <typename T, bool RES> __global__ void __launch_bounds__(256) dropout_a
     ptx::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     uint32_t *words = shared_words + warp * SPAN;
-    const int64_t spans = (a.cols + 3 + SPAN - 1) / SPAN, item = (int64_t)blockIdx.x * 8 + warp;
-    const int64_t t = a.rows * spans <= 0xffffffff ? (int64_t)((uint32_t)item / (uint32_t)spans) : item / spans;
-    if (t >= a.rows) return;
-    const int64_t start = t * a.cols, begin = (item - t * spans) * SPAN - (start & 3); // the span's first column
-    const T *src = (const T *)a.src + t * a.src_ld + begin, *residual = (const T *)a.residual + t * a.residual_ld + begin;
-    T *dst = (T *)a.dst + t * a.dst_ld + begin;
-    // columns of the span that are there: [low, high)
-    const int low = begin < 0 ? (int)-begin : 0, high = (int)min((int64_t)SPAN, a.cols - begin);
-    T x[SPAN / 32], res[SPAN / 32];
+    const uint64_t seed = same_in_warp(ld_dependent_u64(a.drop.seed)), offset = ld_dependent_u64(a.drop.seed + 1);
+    const int64_t spans = (a.cols + 3 + SPAN - 1) / SPAN, total = a.rows * spans;
+    for (int64_t item = (int64_t)blockIdx.x * 8 + warp; item < total; item += (int64_t)gridDim.x * 8) {
+        const int64_t t = total <= 0xffffffff ? (int64_t)((uint32_t)item / (uint32_t)spans) : item / spans;
+        const int64_t start = t * a.cols, begin = (item - t * spans) * SPAN - (start & 3); // the span's first column
+        const T *src = (const T *)a.src + t * a.src_ld + begin, *residual = (const T *)a.residual + t * a.residual_ld + begin;
+        T *dst = (T *)a.dst + t * a.dst_ld + begin;
+        // columns of the span that are there: [low, high)
+        const int low = begin < 0 ? (int)-begin : 0, high = (int)min((int64_t)SPAN, a.cols - begin);
+        const uint64_t block = (uint64_t)(start + begin) >> 2;
+        auto span = [&](auto whole) {
+            T x[SPAN / 32], res[SPAN / 32];
 #pragma unroll
-    for (int i = 0; i < SPAN / 32; ++i) {
-        const int c = 32 * i + lane;
-        if (c >= low && c < high) {
-            x[i] = src[c];
-            if constexpr (RES) res[i] = residual[c];
-        }
-    }
-    const uint64_t seed = ld_dependent_u64(a.drop.seed), offset = ld_dependent_u64(a.drop.seed + 1);
-    const uint64_t block = (uint64_t)(start + begin) >> 2;
-    reinterpret_cast<uint4 *>(words)[lane] = philox(seed, offset, block + lane);
-    reinterpret_cast<uint4 *>(words)[lane + 32] = philox(seed, offset, block + lane + 32);
-    __syncwarp();
+            for (int i = 0; i < SPAN / 32; ++i) {
+                const int c = 32 * i + lane;
+                if (whole || (c >= low && c < high)) {
+                    x[i] = src[c];
+                    if constexpr (RES) res[i] = residual[c];
+                }
+            }
+            __syncwarp();
+            reinterpret_cast<uint4 *>(words)[lane] = philox(seed, offset, block + lane);
+            reinterpret_cast<uint4 *>(words)[lane + 32] = philox(seed, offset, block + lane + 32);
+            __syncwarp();
 #pragma unroll
-    for (int i = 0; i < SPAN / 32; ++i) {
-        const int c = 32 * i + lane;
-        if (c >= low && c < high) dst[c] = from_f32<T>(keep_add(words[c], a.drop, to_f32(x[i]), RES ? to_f32(res[i]) : 0.f));
+            for (int i = 0; i < SPAN / 32; ++i) {
+                const int c = 32 * i + lane;
+                if (whole || (c >= low && c < high)) dst[c] = from_f32<T>(keep_add(words[c], a.drop, to_f32(x[i]), RES ? to_f32(res[i]) : 0.f));
+            }
+        };
+        if (low == 0 && high == SPAN) span(std::true_type());
+        else span(std::false_type());
     }
 }
 
@@ -150,13 +201,13 @@ template <typename T> int launch_typed(const DropoutArgs &a, int sm_count, cudaS
         kernel = dropout_all_kernel<T>;
         grid = std::min<int64_t>((a.rows * a.cols + 255) / 256, (int64_t)sm_count * 16);
     } else if (vec) {
-        kernel = a.rows == 1 ? (a.residual ? dropout_rows_kernel<T, true, true> : dropout_rows_kernel<T, false, true>)
-                             : (a.residual ? dropout_rows_kernel<T, true, false> : dropout_rows_kernel<T, false, false>);
-        grid = a.rows * ((a.cols + 256 * SHARES * 8 - 1) / (256 * SHARES * 8));
+        kernel = a.rows == 1 ? (a.residual ? dropout_dense_kernel<T, true> : dropout_dense_kernel<T, false>)
+                             : (a.residual ? dropout_rows_kernel<T, true> : dropout_rows_kernel<T, false>);
+        grid = (a.rows * ((a.cols + 7) / 8) + 256 * SHARES - 1) / (256 * SHARES);
         if (sizeof(T) == 2) grid = std::min(grid, (int64_t)sm_count * CTAS);
     } else {
         kernel = a.residual ? dropout_any_kernel<T, true> : dropout_any_kernel<T, false>;
-        grid = (a.rows * ((a.cols + 3 + SPAN - 1) / SPAN) + 7) / 8;
+        grid = std::min((a.rows * ((a.cols + 3 + SPAN - 1) / SPAN) + 7) / 8, (int64_t)sm_count * 6);
     }
     if (grid > 0x7fffffff) return 3;
     const int rc = launch_dependent(kernel, a, (unsigned)grid, 256, 0, st);
