@@ -4,9 +4,14 @@
 //   softmax  w_j = scale exp(l_j - m) / sum_i exp(l_i - m), i over all unmasked experts, or over the chosen (normalize)
 //   sigmoid  w_j = scale s(l_j), or scale s(l_j) / sum over the chosen (normalize): the softmax of log s, which cannot
 //            divide zero by zero however low the logits
-// A warp keeps a row in registers (one read of the logits) and takes the largest value k times: a redux.sync over the keys,
-// then one over the indices that have it.  Keys are the logits' bits in the order of their values, so the choice is exact.
-// Sums are held in 32 bits.
+// A warp keeps a row in registers (one read of the logits) and takes the largest value k times.  Values stand as unsigned
+// keys in the order of the values, so the choice is exact; 16-bit logits share a word with their index, which makes keys
+// differ and one redux.sync say both.  What is chosen is never removed: the next largest is the largest below it, which one
+// addition and maximum a value finds (8192 x 256 bf16, k = 8: removing 11.1 us, this 6.1).  Sums are held in 32 bits.
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
 #include "launch.h"
 #include "token_rows.cuh"
 
@@ -39,69 +44,118 @@ __device__ __forceinline__ float warp_max(float v) {
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
 __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
 
+// The largest key below `most`, 0 if there is none: key - most wraps for those below, beyond any difference of the others,
+// and the largest wrapped difference is the nearest.
+template <int N> __device__ __forceinline__ uint32_t next_below(const uint32_t (&key)[N], uint32_t most) {
+    uint32_t d = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) d = max(d, key[i] - most);
+    const uint32_t next = d + most;
+    return next < most ? next : 0u;
+}
+
 template <typename T, int PER_LANE>
 __global__ void __launch_bounds__(WARPS * 32) route_kernel(const __grid_constant__ RouteArgs a) {
     ptx::grid_dependency_wait();
+    constexpr int V = PER_LANE * sizeof(T) < 16 ? PER_LANE : 16 / (int)sizeof(T); // neighbours that a lane reads at once
     const int lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * WARPS + threadIdx.x / 32;
     if (t >= a.tokens) return;
     const T *row = (const T *)a.logits + t * a.logits_ld;
-    uint32_t key[PER_LANE]; // of experts lane, lane + 32, ...
+    auto expert = [&](int i) { return i / V * (32 * V) + lane * V + i % V; }; // of the lane's value i
+    T raw[PER_LANE];
+    if (a.aligned) { // rows start on, and hold a multiple of, V values
+        struct alignas(V * sizeof(T)) Group { T v[V]; };
+#pragma unroll
+        for (int i = 0; i < PER_LANE; i += V)
+            if (expert(i) < a.experts) {
+                const Group g = *reinterpret_cast<const Group *>(row + expert(i));
+#pragma unroll
+                for (int j = 0; j < V; ++j) raw[i + j] = g.v[j];
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i)
+            if (expert(i) < a.experts) raw[i] = row[expert(i)];
+    }
+    uint32_t key[PER_LANE];
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) {
-        const int e = 32 * i + lane;
-        key[i] = e < a.experts ? order_key(to_f32(row[e])) : 0u;
+        key[i] = expert(i) < a.experts ? order_key(to_f32(raw[i])) : 0u;
+        // the value's bits are the upper 16 of its key (bf16) or of its own (f16)
+        if constexpr (sizeof(T) == 2) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const uint32_t u = __half_as_ushort(raw[i]), k = (u & 0x7fffu) == 0 ? 0x8000u : u & 0x8000u ? ~u & 0xffffu : u | 0x8000u;
+                key[i] = key[i] ? k << 16 : 0u;
+            }
+            key[i] = key[i] ? (key[i] & 0xffff0000u) | (0xffffu - expert(i)) : 0u;
+        }
     }
+    constexpr float LIMIT = std::is_same<T, __half>::value ? 65504.f : 3.402823466e38f; // +inf counts as the largest finite value
+    auto value = [&](uint32_t k) { // of a key
+        if constexpr (std::is_same<T, __half>::value) {
+            const uint32_t u = k >> 16;
+            return fminf(__half2float(__ushort_as_half((unsigned short)(u & 0x8000u ? u & 0x7fffu : ~u))), LIMIT);
+        } else {
+            return key_value(sizeof(T) == 2 ? (k & 0x80000000u ? k & 0xffff0000u : k | 0xffffu) : k);
+        }
+    };
     uint32_t best = 0;
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) best = max(best, key[i]);
     float sum = 0.f, top = 0.f;
     if (a.scoring == SCORING_SOFTMAX && !a.normalize) {
-        top = key_value(__reduce_max_sync(0xffffffffu, best));
+        top = value(__reduce_max_sync(0xffffffffu, best));
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i) sum += key[i] ? expf(key_value(key[i]) - top) : 0.f;
+        for (int i = 0; i < PER_LANE; ++i) sum += key[i] ? expf(fminf(to_f32(raw[i]), LIMIT) - top) : 0.f;
         sum = warp_sum(sum);
     }
     uint32_t mine = 0; // key and index of choice `lane`
     int index = -1;
-    for (int j = 0; j < a.choices; ++j) {
-        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-        if (most == 0) break;
-        int at = 0x7fffffff;
-        if (best == most) {
-#pragma unroll
-            for (int i = PER_LANE - 1; i >= 0; --i)
-                if (key[i] == most) at = 32 * i + lane;
+    if constexpr (sizeof(T) == 2) {
+        for (int j = 0; j < a.choices; ++j) {
+            const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+            if (most == 0) break;
+            if (lane == j) mine = most;
+            best = next_below(key, most);
         }
-        at = __reduce_min_sync(0xffffffffu, at);
-        if (lane == j) {
-            mine = most;
-            index = at;
-        }
-        if (lane == (at & 31)) { // taken: out of the running
-            best = 0;
+        if (mine) index = 0xffff - (int)(mine & 0xffffu);
+    } else {
+        for (int j = 0; j < a.choices;) {
+            const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+            if (most == 0) break;
+            uint32_t equal = 0; // the lane's values with this key, lowest index first
+            if (best == most) {
 #pragma unroll
-            for (int i = 0; i < PER_LANE; ++i) {
-                if (i == at >> 5) key[i] = 0u;
-                best = max(best, key[i]);
+                for (int i = 0; i < PER_LANE; ++i) equal |= key[i] == most ? 1u << i : 0u;
             }
+            for (; j < a.choices; ++j) {
+                const int i = __ffs(equal) - 1, own = equal ? expert(i) : INT_MAX, at = __reduce_min_sync(0xffffffffu, own);
+                if (at == INT_MAX) break;
+                if (own == at) equal &= equal - 1;
+                if (lane == j) {
+                    mine = most;
+                    index = at;
+                }
+            }
+            best = next_below(key, most);
         }
     }
     const bool chosen = index >= 0;
     float w;
     if (a.scoring == SCORING_SOFTMAX) {
-        if (a.normalize) top = key_value(__shfl_sync(0xffffffffu, mine, 0)); // the first choice is the largest
-        w = chosen ? expf(key_value(mine) - top) : 0.f;
+        if (a.normalize) top = value(__shfl_sync(0xffffffffu, mine, 0)); // the first choice is the largest
+        w = chosen ? expf(value(mine) - top) : 0.f;
         if (a.normalize) sum = warp_sum(w);
         w = chosen ? w / sum : 0.f;
     } else if (a.normalize) {
-        const float l = chosen ? log_sigmoid(key_value(mine)) : -INFINITY;
+        const float l = chosen ? log_sigmoid(value(mine)) : -INFINITY;
         const float m = __shfl_sync(0xffffffffu, l, 0);
         w = chosen ? expf(l - m) : 0.f;
         sum = warp_sum(w);
         w = chosen ? w / sum : 0.f;
     } else {
-        w = chosen ? sigmoid(key_value(mine)) : 0.f;
+        w = chosen ? sigmoid(value(mine)) : 0.f;
     }
     if (lane < a.choices) {
         a.weights[t * a.weights_ld + lane] = w * a.scale;
@@ -180,12 +234,16 @@ template <typename T> int launch_typed(const RouteArgs &a, bool backward, cudaSt
     if (backward) {
         rc = launch_dependent(route_backward_kernel<T>, a, (unsigned)grid, WARPS * 32, WARPS * a.experts * sizeof(float), st);
     } else {
-        void (*kernel)(RouteArgs) = a.experts <= 64 ? route_kernel<T, 2>
-                : a.experts <= 128                  ? route_kernel<T, 4>
-                : a.experts <= 256                  ? route_kernel<T, 8>
-                : a.experts <= 512                  ? route_kernel<T, 16>
-                                                    : route_kernel<T, 32>;
-        rc = launch_dependent(kernel, a, (unsigned)grid, WARPS * 32, 0, st);
+        RouteArgs r = a;
+        const int per_lane = a.experts <= 64 ? 2 : a.experts <= 128 ? 4 : a.experts <= 256 ? 8 : a.experts <= 512 ? 16 : 32;
+        const int bytes = std::min(per_lane * (int)sizeof(T), 16), values = bytes / (int)sizeof(T);
+        r.aligned = (uintptr_t)a.logits % bytes == 0 && a.experts % values == 0 && (a.tokens == 1 || a.logits_ld % values == 0);
+        void (*kernel)(RouteArgs) = per_lane == 2 ? route_kernel<T, 2>
+                : per_lane == 4                   ? route_kernel<T, 4>
+                : per_lane == 8                   ? route_kernel<T, 8>
+                : per_lane == 16                  ? route_kernel<T, 16>
+                                                  : route_kernel<T, 32>;
+        rc = launch_dependent(kernel, r, (unsigned)grid, WARPS * 32, 0, st);
     }
     if (rc == 0) count_launch();
     return rc;

@@ -21,6 +21,7 @@ struct RouteArgs {
     int dt; // of the logits and of their gradient
     const void *logits;
     int64_t logits_ld;
+    int aligned; // the launcher's: rows can be read several values at a time
     // forward: outputs; backward: indices and the weights' gradient are inputs
     float *weights;
     int64_t weights_ld;
