@@ -184,11 +184,24 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
     return dnnl_success;
 }
 
-int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, const std::map<int, char *> &at,
-        const std::map<int, const int *> &offsets, void *scratch, cudaStream_t stream) {
+// where an execution's tensors are
+struct bound_t {
+    struct { int arg; char *values; const int *offsets; } t[8];
+    int n = 0;
+};
+
+int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, const bound_t &bound, void *scratch, cudaStream_t stream) {
     const int sms = primitive.pd.engine->sm_count > 0 ? primitive.pd.engine->sm_count : 148;
-    auto ptr = [&](int arg) -> void * { auto it = at.find(arg); return it == at.end() ? nullptr : it->second; };
-    auto ends = [&](int arg) { auto it = offsets.find(arg); return it == offsets.end() ? nullptr : it->second; };
+    auto ptr = [&](int arg) -> void * {
+        for (int i = 0; i < bound.n; ++i)
+            if (bound.t[i].arg == arg) return bound.t[i].values;
+        return nullptr;
+    };
+    auto ends = [&](int arg) -> const int * {
+        for (int i = 0; i < bound.n; ++i)
+            if (bound.t[i].arg == arg) return bound.t[i].offsets;
+        return nullptr;
+    };
     // row pitch in elements (of a single row: its width)
     auto ld = [&](int arg) -> int64_t {
         const auto *md = op.find(arg);
@@ -223,13 +236,13 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             DispatchArgs a {};
             a.tokens = (int)src->dims[0]; a.choices = (int)op.find(DNNL_ARG_SRC_1)->dims[1];
             a.experts = (int)op.find(DNNL_ARG_DST)->group_count;
+            a.element = (int)size;
             a.row_bytes = src->dims[1] * size;
             a.src = (const char *)ptr(DNNL_ARG_SRC); a.src_pitch = ld(DNNL_ARG_SRC) * size;
             a.indices = (const int *)ptr(DNNL_ARG_SRC_1); a.indices_ld = ld(DNNL_ARG_SRC_1);
             a.dst = (char *)ptr(DNNL_ARG_DST);
             a.offsets = const_cast<int *>(ends(DNNL_ARG_DST));
             a.positions = (int *)ptr(DNNL_ARG_DST_1); a.positions_ld = ld(DNNL_ARG_DST_1);
-            a.status = primitive.pd.engine->status_word;
             return launch_dispatch(a, (int *)scratch, sms, stream);
         }
         case dnnl_cuda_interop_moe_combine:
@@ -312,17 +325,19 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
         if (st != dnnl_success) return st;
         op = &settled;
     }
-    std::map<int, char *> at;
-    std::map<int, const int *> offsets;
+    bound_t bound;
     for (const auto &kv : op->args) {
         const dnnl_memory_t m = find(kv.first);
         if (m->is_host_scalar) return dnnl_invalid_arguments;
-        char *p = (char *)m->handles[0];
-        if (!p && !kv.second.has_zero_dim()) return dnnl_invalid_arguments;
-        at[kv.first] = p ? p + kv.second.offset0 * (dnnl_dim_t)dt_bits(kv.second.data_type) / 8 : p;
+        auto &b = bound.t[bound.n++]; // (no kind has more than seven tensors)
+        b.arg = kv.first;
+        b.values = (char *)m->handles[0];
+        b.offsets = nullptr;
+        if (!b.values && !kv.second.has_zero_dim()) return dnnl_invalid_arguments;
+        if (b.values) b.values += kv.second.offset0 * (dnnl_dim_t)dt_bits(kv.second.data_type) / 8;
         if (kv.second.is_grouped()) {
             if (!m->md.is_grouped() || !m->handles[1]) return dnnl_invalid_arguments;
-            offsets[kv.first] = (const int *)m->handles[1];
+            b.offsets = (const int *)m->handles[1];
         }
     }
     if (pd.engine->device < 0) {
@@ -343,7 +358,7 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
         cudaEventRecord(ev0, stream->stream);
     }
     profiling_begin(stream);
-    const int rc = launch(primitive, (int)pd.kind, *op, at, offsets, scratch, stream->stream);
+    const int rc = launch(primitive, (int)pd.kind, *op, bound, scratch, stream->stream);
     profiling_end(stream);
     if (verbose) {
         cudaEventRecord(ev1, stream->stream);

@@ -39,8 +39,8 @@ __device__ __forceinline__ void drop_piece(const DropoutArgs &a, uint64_t seed, 
 #pragma unroll
     for (int s = 0; s < SHARES; ++s)
         if (WHOLE || col + SPREAD * s < end) {
-            x[s].load(src + SPREAD * s, 0, WHOLE ? 8 : end - col - SPREAD * s);
-            if constexpr (RES) res[s].load(residual + SPREAD * s, 0, WHOLE ? 8 : end - col - SPREAD * s);
+            x[s].load_ragged(src + SPREAD * s, WHOLE ? 8 : end - col - SPREAD * s);
+            if constexpr (RES) res[s].load_ragged(residual + SPREAD * s, WHOLE ? 8 : end - col - SPREAD * s);
         }
     uint32_t u[SHARES][8];
 #pragma unroll
@@ -58,7 +58,7 @@ __device__ __forceinline__ void drop_piece(const DropoutArgs &a, uint64_t seed, 
             if constexpr (RES) res[s].get(r);
 #pragma unroll
             for (int n = 0; n < 8; ++n) v[n] = keep_add(u[s][n], a.drop, v[n], RES ? r[n] : 0.f);
-            Cols<T, true>::store(dst + SPREAD * s, 0, WHOLE ? 8 : end - col - SPREAD * s, v);
+            Cols<T, true>::store_ragged(dst + SPREAD * s, WHOLE ? 8 : end - col - SPREAD * s, v);
         }
 }
 
@@ -70,8 +70,8 @@ __device__ __forceinline__ void drop_shares(const DropoutArgs &a, uint64_t seed,
 #pragma unroll
     for (int s = 0; s < SHARES; ++s)
         if (WHOLE || left[s] > 0) {
-            x[s].load(src[s], 0, WHOLE ? 8 : left[s]);
-            if constexpr (RES) res[s].load(residual[s], 0, WHOLE ? 8 : left[s]);
+            x[s].load_ragged(src[s], WHOLE ? 8 : left[s]);
+            if constexpr (RES) res[s].load_ragged(residual[s], WHOLE ? 8 : left[s]);
         }
     uint32_t u[SHARES][8];
 #pragma unroll
@@ -89,7 +89,7 @@ __device__ __forceinline__ void drop_shares(const DropoutArgs &a, uint64_t seed,
             if constexpr (RES) res[s].get(r);
 #pragma unroll
             for (int n = 0; n < 8; ++n) v[n] = keep_add(u[s][n], a.drop, v[n], RES ? r[n] : 0.f);
-            Cols<T, true>::store(dst[s], 0, WHOLE ? 8 : left[s], v);
+            Cols<T, true>::store_ragged(dst[s], WHOLE ? 8 : left[s], v);
         }
 }
 

@@ -13,9 +13,10 @@ namespace qmm {
 
 namespace {
 
-constexpr int GROUP = 8; // rows of a token in flight at a time: their loads leave before the first is used
+// rows of a token in flight at a time: their loads leave before the first is used.  Two where a token has no more, eight
+// otherwise: what eight take in registers costs a token of two rows half its warps (gradient, 4096 x 2 x 4096 55 / 39 us).
 
-template <typename S, typename D, bool VEC, bool DROP>
+template <typename S, typename D, bool VEC, bool DROP, int GROUP>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineArgs a) {
     __shared__ __align__(16) uint32_t words[DROP && !VEC ? 8 * 128 : 4];
     ptx::grid_dependency_wait();
@@ -303,7 +304,7 @@ template <typename S, bool VEC> __device__ __forceinline__ void zero_tail(const 
 }
 
 // THREADS of the 256 of a CTA work on a token: all of them, or a warp where rows are short.
-template <typename S, typename D, bool VEC, bool DROP, int THREADS>
+template <typename S, typename D, bool VEC, bool DROP, int THREADS, int GROUP>
 __global__ void __launch_bounds__(256) combine_backward_kernel(const __grid_constant__ CombineArgs a) {
     __shared__ __align__(16) uint32_t words[DROP && !VEC ? 8 * 128 : 4];
     __shared__ float partial[8][GROUP];
@@ -406,27 +407,31 @@ template <typename S, typename D, bool DROP> int launch_forward(const CombineArg
     const int64_t grid = (total + 255) / 256;
     // Below 2 KB a row or 2^21 sums the ring's start and the copies' number cost more than they give.  us a call, thread by
     // thread / bulk, bf16, k = 8: 600 x 4096 7.9 / 7.5, 400 x 4096 5.8 / 6.0, 4096 x 512 7.4 / 9.0; k = 1: 4096 x 1024 8.3 / 6.7.
-    if (vec && a.cols % 8 == 0 && a.cols * (int64_t)sizeof(S) >= 2048 && a.tokens * a.cols >= (1 << 21)
+    if (vec && a.cols * (int64_t)sizeof(S) >= 2048 && a.tokens * a.cols >= (1 << 21)
             && a.tokens * ((a.cols + WARP_COLS - 1) / WARP_COLS) < (1 << 30) && !a.drop.drop_all)
         return launch_bulk<S, D, DROP>(a, sm_count, st);
     if (grid > 0x7fffffff) return 3;
-    return launch_dependent(vec ? combine_kernel<S, D, true, DROP> : combine_kernel<S, D, false, DROP>, a, (unsigned)grid, 256, 0, st);
+    void (*kernel)(CombineArgs) = a.choices <= 2 ? (vec ? combine_kernel<S, D, true, DROP, 2> : combine_kernel<S, D, false, DROP, 2>)
+                                                 : (vec ? combine_kernel<S, D, true, DROP, 8> : combine_kernel<S, D, false, DROP, 8>);
+    return launch_dependent(kernel, a, (unsigned)grid, 256, 0, st);
 }
 
-template <typename S, typename D, bool DROP> int launch_backward(const CombineArgs &a, bool vec, cudaStream_t st) {
-    const int64_t units = vec ? row_units<true>(a.cols, DROP) : row_units<false>(a.cols, DROP);
-    const bool wide = units > 64;
+template <typename S, typename D, bool VEC, bool DROP, int GROUP> int launch_backward(const CombineArgs &a, cudaStream_t st) {
+    const bool wide = row_units<VEC>(a.cols, DROP) > 64;
     const int64_t grid = wide ? a.tokens : (a.tokens + 7) / 8;
     if (grid > 0x7fffffff) return 3;
-    void (*kernel)(CombineArgs) = vec ? (wide ? combine_backward_kernel<S, D, true, DROP, 256> : combine_backward_kernel<S, D, true, DROP, 32>)
-                                      : (wide ? combine_backward_kernel<S, D, false, DROP, 256> : combine_backward_kernel<S, D, false, DROP, 32>);
-    return launch_dependent(kernel, a, (unsigned)grid, 256, 0, st);
+    return launch_dependent(wide ? combine_backward_kernel<S, D, VEC, DROP, 256, GROUP> : combine_backward_kernel<S, D, VEC, DROP, 32, GROUP>, a,
+            (unsigned)grid, 256, 0, st);
+}
+template <typename S, typename D, bool DROP> int launch_backward(const CombineArgs &a, bool vec, cudaStream_t st) {
+    if (a.choices <= 2) return vec ? launch_backward<S, D, true, DROP, 2>(a, st) : launch_backward<S, D, false, DROP, 2>(a, st);
+    return vec ? launch_backward<S, D, true, DROP, 8>(a, st) : launch_backward<S, D, false, DROP, 8>(a, st);
 }
 
 template <typename S, typename D> int launch_types(const CombineArgs &a, bool backward, int sm_count, cudaStream_t st) {
     const bool drop = a.drop.seed != nullptr;
     const int64_t ds = sizeof(D);
-    bool vec = rows_aligned(a.src, a.cols * (int64_t)sizeof(S), a.rows) && (!drop || a.cols % 4 == 0 || a.tokens == 1);
+    bool vec = a.cols % 8 == 0 && rows_aligned(a.src, a.cols * (int64_t)sizeof(S), a.rows);
     int rc;
     if (backward) {
         vec = vec && rows_aligned(a.diff_src, a.cols * (int64_t)sizeof(S), a.rows) && rows_aligned(a.diff_dst, a.diff_dst_ld * ds, a.tokens);

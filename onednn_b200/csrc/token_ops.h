@@ -35,6 +35,7 @@ int launch_route_backward(const RouteArgs &a, cudaStream_t st);
 
 struct DispatchArgs {
     int tokens, choices, experts;
+    int element; // bytes of one: 1, 2 or 4
     int64_t row_bytes; // of a token's row; the grouped rows are dense
     const char *src;
     int64_t src_pitch; // bytes
@@ -44,7 +45,6 @@ struct DispatchArgs {
     int *offsets; // [experts], cumulative ends
     int *positions;
     int64_t positions_ld;
-    int *status; // the engine's status word
 };
 int launch_dispatch(const DispatchArgs &a, int *scratch, int sm_count, cudaStream_t st);
 size_t dispatch_scratch_bytes(int experts, int sm_count);

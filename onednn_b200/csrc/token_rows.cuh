@@ -1,8 +1,8 @@
 // What the kernels that move and sum rows of tokens share: a thread's share of a row's columns, in two forms, and the
 // random words of dropout.
 //
-// VEC: eight neighbouring columns, 16-byte accesses; every row of every tensor starts on a 16-byte boundary (and, with
-// dropout, on a multiple of four elements of the whole tensor).  Otherwise: four columns, 32 apart, so that a warp covers
+// VEC: eight neighbouring columns, 16-byte accesses; every row of every tensor starts on a 16-byte boundary and holds a
+// multiple of eight columns.  Otherwise: four columns, 32 apart, so that a warp covers
 // 128 neighbouring ones and its accesses stay contiguous wherever the rows start; with dropout the 128 begin at a
 // multiple of four elements of the whole tensor, up to three columns before the row.
 #pragma once
@@ -45,14 +45,23 @@ template <typename T, bool VEC> struct Cols;
 template <typename T> struct Cols<T, true> {
     static constexpr int N = 8;
     uint4 raw[sizeof(T) / 2];
+    // of a row with a multiple of eight columns (one predicate and no branch: rows' loads stay together); zeros beyond it
     __device__ __forceinline__ void load(const T *row, int64_t col, int64_t cols) {
-        if (col + 8 <= cols) {
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = ptx::ld_dependent((const uint4 *)(row + col) + i);
-        } else { // the ragged end of a row
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (col < cols) raw[i] = ptx::ld_dependent((const uint4 *)(row + col) + i);
+        }
+    }
+    // of the `left` columns that a row still has from p on
+    __device__ __forceinline__ void load_ragged(const T *p, int64_t left) {
+        if (left >= 8) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = ptx::ld_dependent((const uint4 *)p + i);
+        } else {
             T part[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) part[i] = col + i < cols ? row[col + i] : from_f32<T>(0.f);
+            for (int i = 0; i < 8; ++i) part[i] = i < left ? p[i] : from_f32<T>(0.f);
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4 *>(part)[i];
         }
@@ -78,19 +87,22 @@ template <typename T> struct Cols<T, true> {
         }
     }
     static __device__ __forceinline__ void store(T *row, int64_t col, int64_t cols, const float (&v)[8]) {
-        if (col + 8 <= cols) {
+        if (col < cols) store_ragged(row + col, 8, v);
+    }
+    static __device__ __forceinline__ void store_ragged(T *p, int64_t left, const float (&v)[8]) {
+        if (left >= 8) {
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    reinterpret_cast<float4 *>(row + col)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    reinterpret_cast<float4 *>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             } else {
-                *reinterpret_cast<uint4 *>(row + col) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()),
+                *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()),
                         pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (col + i < cols) row[col + i] = from_f32<T>(v[i]);
+                if (i < left) p[i] = from_f32<T>(v[i]);
         }
     }
 };
@@ -98,23 +110,24 @@ template <typename T> struct Cols<T, true> {
 template <typename T> struct Cols<T, false> {
     static constexpr int N = 4;
     T raw[4];
+    // of 32 i: the columns that are there (those below 0 are among the first 32)
+    static __device__ __forceinline__ bool there(int i, int64_t col, int64_t cols) {
+        return (i > 0 || col >= 0) && 32 * i < (int)min((int64_t)128, cols - col);
+    }
     __device__ __forceinline__ void load(const T *row, int64_t col, int64_t cols) {
+        const T *p = row + col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t c = col + 32 * i;
-            raw[i] = c >= 0 && c < cols ? row[c] : from_f32<T>(0.f);
-        }
+        for (int i = 0; i < 4; ++i) raw[i] = there(i, col, cols) ? p[32 * i] : from_f32<T>(0.f);
     }
     __device__ __forceinline__ void get(float (&v)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = to_f32(raw[i]);
     }
     static __device__ __forceinline__ void store(T *row, int64_t col, int64_t cols, const float (&v)[4]) {
+        T *p = row + col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t c = col + 32 * i;
-            if (c >= 0 && c < cols) row[c] = from_f32<T>(v[i]);
-        }
+        for (int i = 0; i < 4; ++i)
+            if (there(i, col, cols)) p[32 * i] = from_f32<T>(v[i]);
     }
 };
 
