@@ -13,8 +13,9 @@ namespace qmm {
 
 namespace {
 
-// rows of a token in flight at a time: their loads leave before the first is used.  Two where a token has no more, eight
-// otherwise: what eight take in registers costs a token of two rows half its warps (gradient, 4096 x 2 x 4096 55 / 39 us).
+// GROUP rows of a token are in flight at a time: their loads leave before the first is used.  As many as a token has, up to
+// eight: what eight take in registers costs a token of fewer rows its warps (gradient, 4096 x 4096, two rows 55 us with
+// eight / 34 with two, four rows 72 / 56).
 
 template <typename S, typename D, bool VEC, bool DROP, int GROUP>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineArgs a) {
@@ -303,9 +304,15 @@ template <typename S, bool VEC> __device__ __forceinline__ void zero_tail(const 
     }
 }
 
+// CTAs per SM that the gradient's registers are cut to (0: the compiler's choice), by what 4096 tokens took: bf16, eight rows
+// of 4096 100 us uncut / 103 two / 95 three, of 512 (a warp a token) 12 / - / 16, four rows of 4096 56 / 65 / 60; f32, eight
+// rows 220 / 173 / 238; rows that start anywhere 102 / 102 / 154.
+template <typename S, bool VEC, int GROUP, int THREADS>
+constexpr int GRADIENT_CTAS = !VEC || sizeof(S) == 4 ? 2 : GROUP == 8 && THREADS == 256 ? 3 : 0;
+
 // THREADS of the 256 of a CTA work on a token: all of them, or a warp where rows are short.
 template <typename S, typename D, bool VEC, bool DROP, int THREADS, int GROUP>
-__global__ void __launch_bounds__(256) combine_backward_kernel(const __grid_constant__ CombineArgs a) {
+__global__ void __launch_bounds__(256, GRADIENT_CTAS<S, VEC, GROUP, THREADS>) combine_backward_kernel(const __grid_constant__ CombineArgs a) {
     __shared__ __align__(16) uint32_t words[DROP && !VEC ? 8 * 128 : 4];
     __shared__ float partial[8][GROUP];
     ptx::grid_dependency_wait();
@@ -425,6 +432,7 @@ template <typename S, typename D, bool VEC, bool DROP, int GROUP> int launch_bac
 }
 template <typename S, typename D, bool DROP> int launch_backward(const CombineArgs &a, bool vec, cudaStream_t st) {
     if (a.choices <= 2) return vec ? launch_backward<S, D, true, DROP, 2>(a, st) : launch_backward<S, D, false, DROP, 2>(a, st);
+    if (a.choices <= 4) return vec ? launch_backward<S, D, true, DROP, 4>(a, st) : launch_backward<S, D, false, DROP, 4>(a, st);
     return vec ? launch_backward<S, D, true, DROP, 8>(a, st) : launch_backward<S, D, false, DROP, 8>(a, st);
 }
 
