@@ -1,6 +1,8 @@
 // Descriptors and execution of the operators around an expert layer's products and of dropout (dnnl_b200.h).  One check
 // serves creation and, where dims were left open, each execution: it skips what an open dim leaves unsaid.
 #include <initializer_list>
+#include <memory>
+#include <new>
 
 #include "launch.h"
 #include "objects.hpp"
@@ -137,11 +139,10 @@ dnnl_status_t check(int kind, const token_op_t &op) {
     return c.status;
 }
 
-// An output may not be left open to the primitive's choice, nor may a bias-like zero descriptor stand for a tensor; a null
-// or zero descriptor of an optional tensor leaves it out.
+// A null or zero descriptor leaves an optional tensor out, and is an error for the others.
 dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind, token_op_t op,
         std::initializer_list<std::pair<int, const_dnnl_memory_desc_t>> tensors,
-        std::initializer_list<std::pair<int, const_dnnl_memory_desc_t>> optional, const_dnnl_primitive_attr_t attr) {
+        std::initializer_list<std::pair<int, const_dnnl_memory_desc_t>> optional, const_dnnl_primitive_attr_t attr) try {
     if (!out || !engine) return dnnl_invalid_arguments;
     for (const auto &t : tensors) {
         if (!t.second) return dnnl_invalid_arguments;
@@ -165,7 +166,7 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
         seed.format_kind = dnnl_blocked;
         op.args[DNNL_ARG_ATTR_DROPOUT_SEED] = seed;
     }
-    auto *pd = new dnnl_primitive_desc;
+    std::unique_ptr<dnnl_primitive_desc> pd(new dnnl_primitive_desc);
     pd->kind = (dnnl_primitive_kind_t)kind;
     pd->engine = engine;
     if (attr) pd->attr = *attr;
@@ -180,8 +181,10 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
         pd->scratchpad.format_kind = dnnl_blocked;
     }
     pd->token_op = std::move(op);
-    *out = pd;
+    *out = pd.release();
     return dnnl_success;
+} catch (const std::bad_alloc &) { // no exception leaves a C entry
+    return dnnl_out_of_memory;
 }
 
 // where an execution's tensors are
@@ -290,7 +293,7 @@ const char *token_op_name(int kind) {
     return is_token_op(kind) ? names[kind - dnnl_cuda_interop_moe_route] : "unknown";
 }
 
-dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t stream, int nargs, const dnnl_exec_arg_t *args) {
+dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t stream, int nargs, const dnnl_exec_arg_t *args) try {
     const dnnl_primitive_desc &pd = primitive.pd;
     auto find = [&](int key) -> dnnl_memory_t {
         for (int i = 0; i < nargs; ++i)
@@ -370,6 +373,8 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
     }
     if (rc == 5) set_last_error(std::string("kernel launch: ") + cudaGetErrorString(cudaGetLastError()));
     return (dnnl_status_t)rc;
+} catch (const std::bad_alloc &) {
+    return dnnl_out_of_memory;
 }
 
 } // namespace qmm

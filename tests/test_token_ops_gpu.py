@@ -250,7 +250,13 @@ COMBINE = [
     (33, 40, 32, 64, "f32", "bf16", True, True, 0.0, 0, 0), (64, 3, 3, 7, "f32", "f32", False, True, 0.25, 0, 0.5),
     (130, 8, 2, 1024, "bf16", "f16", False, False, 0.0, 0, 0.1), (11, 8, 4, 512, "f32", "f16", True, True, 1.0, 0, 0),
     (5, 8, 2, 2050, "bf16", "bf16", True, True, 0.2, 0, 1.0), (777, 32, 6, 8, "f16", "bf16", True, True, 0.1, 0, 0),
-    (3, 4, 2, 1001, "f16", "f32", True, True, 0.4, 0, 0)]
+    (3, 4, 2, 1001, "f16", "f32", True, True, 0.4, 0, 0),
+    # many tokens of wide rows: the form that streams them through shared memory (several tokens an item, several
+    # segments a token, few and many stages, ragged last items and segments)
+    (2050, 16, 8, 1024, "bf16", "bf16", True, True, 0.2, 0, 0.1), (2101, 16, 3, 1032, "f16", "f32", True, True, 0.0, 1040, 0.3),
+    (700, 40, 32, 3080, "f32", "f16", True, True, 0.1, 0, 0), (1000, 8, 1, 2600, "bf16", "f16", False, False, 0.3, 0, 0),
+    (601, 16, 8, 4104, "bf16", "bf16", True, True, 0.0, 0, 1.0), (530, 8, 5, 4352, "f32", "f32", True, False, 0.5, 0, 0.2),
+    (1201, 32, 17, 1800, "bf16", "bf16", True, True, 0.0, 0, 0.05)]
 
 
 @pytest.mark.parametrize("T,E,k,H,dtype,out,weighted,res,p,pitch,dropped", COMBINE)
@@ -366,6 +372,47 @@ def test_positions_outside_the_rows_are_skipped(gpu):
     offsets = torch.tensor([8], dtype=torch.int32, device="cuda:0")
     pos = torch.tensor([[0, 8], [2 ** 31 - 1, -2 ** 31], [3, -1], [7, 7]], dtype=torch.int32, device="cuda:0")
     assert run_combine(gpu[0], rows, offsets, pos, "f32")[:, 0].tolist() == [1, 0, 1, 2]
+
+
+@pytest.mark.parametrize("T,H,p", [(40, 104, 0.2), (40, 103, 0.2), (3000, 1024, 0.2), (3000, 1024, 0.0), (600, 4096, 0.5)])
+def test_inputs_of_one_row_for_all_and_results_in_place(gpu, T, H, p):
+    """residual, weights, tokens and the gradient with a row pitch of 0; dst in the residual's memory"""
+    import torch
+    r = rng(T, H)
+    E, k, seed = 8, 2, (99, 5)
+    rows, offsets, dpos, pos = make_rows(r, T, E, k, H, "bf16", 0.1)
+    one, w1 = device_matrix(r.standard_normal((1, H)), "bf16"), r.random((1, k)).astype(np.float32)
+    weights = torch.from_numpy(w1).cuda().expand(T, k)
+    drop = dict(p=p, seed=seed if p else None)
+    got = run_combine(gpu[0], rows, offsets, dpos, "bf16", weights, one.expand(T, H), **drop)
+    want, size = combine_want(rows, pos, np.where(pos >= 0, w1, 0).astype(np.float64), np.repeat(host(one), T, 0), p, seed)
+    check(got, want, size * EPS * (k + 4) + out_slack(want, "bf16"))
+    y = device_matrix(np.repeat(host(one), T, 0), "bf16")
+    c = Call(gpu[0])
+    a = c.api
+    if p:
+        c.bind(a.ARG_ATTR_DROPOUT_SEED, torch.tensor(seed, dtype=torch.int64, device="cuda:0"))
+    pd = a.moe_combine.primitive_desc(gpu[0], c.grouped(a.ARG_SRC, rows, offsets), c.bind(a.ARG_SRC_1, dpos), c.bind(a.ARG_DST, y),
+                                      weights_md=c.bind(a.ARG_WEIGHTS, weights), residual_md=c.bind(a.ARG_SRC_2, y), dropout_p=p)
+    c.run(a.moe_combine, pd).strm.wait()
+    assert np.array_equal(host(y), got)
+    c = Call(gpu[0])
+    drows, dw = torch.empty_like(rows), torch.empty((T, k), device="cuda:0")
+    if p:
+        c.bind(a.ARG_ATTR_DROPOUT_SEED, torch.tensor(seed, dtype=torch.int64, device="cuda:0"))
+    pd = a.moe_combine_backward.primitive_desc(
+        gpu[0], c.bind(a.ARG_DIFF_DST, one.expand(T, H)), c.grouped(a.ARG_SRC, rows, offsets), c.bind(a.ARG_SRC_1, dpos),
+        c.bind(a.ARG_WEIGHTS, weights), c.grouped(a.ARG_DIFF_SRC, drows, offsets), c.bind(a.ARG_DIFF_WEIGHTS, dw), dropout_p=p)
+    c.run(a.moe_combine_backward, pd).strm.wait()
+    g = np.repeat(host(one), T, 0)
+    g = R.dropout(g, p, *seed) if p else g
+    x = host(rows)
+    dots = np.where(pos >= 0, np.einsum("th,tkh->tk", g, x[np.maximum(pos, 0)]), 0.0)
+    sizes = np.einsum("th,tkh->tk", np.abs(g), np.abs(x[np.maximum(pos, 0)]))
+    check(host(dw), dots, sizes * EPS * (H + 16) + 2.0 ** -140)
+    idx = choices(r, T, E, k, 0)
+    got_rows, _, got_pos = run_dispatch(gpu[0], one.expand(T, H), idx, E)
+    assert np.array_equal(host(got_rows), np.repeat(host(one), T * k, 0)) and np.array_equal(host(got_pos), R.sort_slots(idx, E)[1])
 
 
 # ----------------------------------------------------------------------------------------------- dropout
@@ -553,3 +600,19 @@ def test_rows_beyond_32_bit_offsets(gpu):
     pd = a.moe_combine.primitive_desc(gpu[0], c.grouped(a.ARG_SRC, rows, offsets), c.bind(a.ARG_SRC_1, pos), c.bind(a.ARG_DST, y))
     c.run(a.moe_combine, pd).strm.wait()
     assert torch.equal(y, x * k)
+
+
+@pytest.mark.parametrize("tokens,dropout", [(512, 0.1), (1, 0.0), (37, 0.0), (1300, 0.3)])
+def test_a_layer_of_all_of_them(gpu, tokens, dropout):
+    """router, dispatch, the experts' products, combine and the gradients in one stream, each reading what the one before
+    wrote (examples/moe_layer.py).  The sums of 2048 bf16 products round to 8 bits on the way (2^-8 of a row's size, a row's
+    largest values being a few times its usual ones): 2 % of the largest result."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import moe_layer
+    difference, layer = moe_layer.run(tokens=tokens, dropout=dropout)
+    assert max(difference.values()) < 0.02, difference
+    want = R.choose(host(layer.logits), 4)
+    assert np.array_equal(host(layer.idx), want)
+    assert np.array_equal(host(layer.offsets), R.sort_slots(want, 16)[0])
