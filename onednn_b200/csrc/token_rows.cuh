@@ -217,6 +217,5 @@ __device__ __forceinline__ uint64_t ld_dependent_u64(const int64_t *p) {
 inline bool rows_aligned(const void *p, int64_t pitch_bytes, int64_t rows) {
     return (uintptr_t)p % 16 == 0 && (rows <= 1 || pitch_bytes % 16 == 0);
 }
-inline int64_t dt_bytes(int dt) { return dt == DT_F32 || dt == DT_S32 ? 4 : dt == DT_BF16 || dt == DT_F16 ? 2 : 1; }
 
 } // namespace qmm
