@@ -304,9 +304,9 @@ template <typename S, bool VEC> __device__ __forceinline__ void zero_tail(const 
     }
 }
 
-// CTAs per SM that the gradient's registers are cut to (0: the compiler's choice), by what 4096 tokens took: bf16, eight rows
-// of 4096 100 us uncut / 103 two / 95 three, of 512 (a warp a token) 12 / - / 16, four rows of 4096 56 / 65 / 60; f32, eight
-// rows 220 / 173 / 238; rows that start anywhere 102 / 102 / 154.
+// CTAs per SM that the gradient's registers are cut to (0: the compiler's choice).  4096 tokens, the same inputs every call: bf16,
+// eight rows of 4096 89 us three / 101 four (with positions and weights in every thread's registers 100 uncut / 103 two / 95
+// three); f32 220 uncut / 170 two / 238 three; rows that start anywhere 102 two / 154 three.
 template <typename S, bool VEC, int GROUP, int THREADS>
 constexpr int GRADIENT_CTAS = !VEC || sizeof(S) == 4 ? 2 : GROUP == 8 && THREADS == 256 ? 3 : 0;
 
@@ -326,38 +326,41 @@ __global__ void __launch_bounds__(256, GRADIENT_CTAS<S, VEC, GROUP, THREADS>) co
             seed = ld_dependent_u64(a.drop.seed);
             offset = ld_dependent_u64(a.drop.seed + 1);
         }
+        // lane j: position and weight of choice j
+        const int my_pos = lane < a.choices ? ptx::ld_dependent(a.positions + t * a.positions_ld + lane) : -1;
+        const float my_w = lane < a.choices ? ptx::ld_dependent(a.weights + t * a.weights_ld + lane) : 0.f;
         for (int j0 = 0; j0 < a.choices; j0 += GROUP) {
-            int pos[GROUP];
-            float w[GROUP], dot[GROUP];
+            float dot[GROUP];
 #pragma unroll
-            for (int j = 0; j < GROUP; ++j) {
-                pos[j] = j0 + j < a.choices ? ptx::ld_dependent(a.positions + t * a.positions_ld + j0 + j) : -1;
-                w[j] = j0 + j < a.choices ? ptx::ld_dependent(a.weights + t * a.weights_ld + j0 + j) : 0.f;
-                dot[j] = 0.f;
-            }
+            for (int j = 0; j < GROUP; ++j) dot[j] = 0.f;
             for (int64_t u = threadIdx.x % THREADS; u < units; u += THREADS) {
                 const int64_t col = unit_column<VEC>(u, t, a.cols, DROP);
                 Cols<D, VEC> g;
                 Cols<S, VEC> x[GROUP];
                 g.load((const D *)a.diff_dst + t * a.diff_dst_ld, col, a.cols);
 #pragma unroll
-                for (int j = 0; j < GROUP; ++j)
-                    if ((uint32_t)pos[j] < (uint64_t)a.rows) x[j].load((const S *)a.src + (int64_t)pos[j] * a.cols, col, a.cols);
+                for (int j = 0; j < GROUP; ++j) {
+                    const uint32_t pos = __shfl_sync(0xffffffffu, my_pos, j0 + j);
+                    if (pos < (uint64_t)a.rows) x[j].load((const S *)a.src + (int64_t)pos * a.cols, col, a.cols);
+                }
                 float dy[N];
                 g.get(dy);
                 if constexpr (DROP) apply_dropout<VEC>(dy, a.drop, seed, offset, t, a.cols, col, words + (VEC ? 0 : warp * 128));
 #pragma unroll
-                for (int j = 0; j < GROUP; ++j)
-                    if ((uint32_t)pos[j] < (uint64_t)a.rows) {
+                for (int j = 0; j < GROUP; ++j) {
+                    const uint32_t pos = __shfl_sync(0xffffffffu, my_pos, j0 + j);
+                    const float w = __shfl_sync(0xffffffffu, my_w, j0 + j);
+                    if (pos < (uint64_t)a.rows) {
                         float v[N], d[N];
                         x[j].get(v);
 #pragma unroll
                         for (int n = 0; n < N; ++n) {
                             dot[j] = fmaf(dy[n], v[n], dot[j]);
-                            d[n] = w[j] * dy[n];
+                            d[n] = w * dy[n];
                         }
-                        Cols<S, VEC>::store((S *)a.diff_src + (int64_t)pos[j] * a.cols, col, a.cols, d);
+                        Cols<S, VEC>::store((S *)a.diff_src + (int64_t)pos * a.cols, col, a.cols, d);
                     }
+                }
             }
 #pragma unroll
             for (int j = 0; j < GROUP; ++j)
