@@ -647,8 +647,8 @@ typedef enum {
 
 /* Router.  SRC logits [T, E] (f32, bf16, f16) -> DST weights [T, K] (f32), DST_1 indices [T, K] (s32), by falling logit,
  * ties to the lowest index.  Logits of -inf and NaN are masked: never chosen, without a share in any sum; a choice with
- * nothing left has index -1 and weight 0.  normalize: weights are divided by their sum over the K choices.  Then they are
- * multiplied by `scale`. */
+ * nothing left has index -1 and weight 0.  +inf is chosen first and counts as the largest finite value of the logits' type.
+ * normalize: weights are divided by their sum over the K choices.  Then they are multiplied by `scale`. */
 dnnl_status_t dnnl_cuda_interop_moe_route_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
         const_dnnl_memory_desc_t logits_desc, const_dnnl_memory_desc_t weights_desc, const_dnnl_memory_desc_t indices_desc,
         dnnl_cuda_interop_scoring_t scoring, int normalize, float scale, const_dnnl_primitive_attr_t attr);

@@ -27,9 +27,11 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
     return v > -INFINITY ? k : 0u; // (false for a NaN too)
 }
-__device__ __forceinline__ float key_value(uint32_t k) {
-    const float v = __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-    return fminf(v, 3.402823466e38f); // +inf counts as the largest finite value
+// +inf counts as the largest finite value of the logits' type, in the choice's weights and in their gradient alike.
+template <typename T>
+constexpr float LARGEST = std::is_same<T, __half>::value ? 65504.f : std::is_same<T, __nv_bfloat16>::value ? 3.38953139e38f : 3.402823466e38f;
+template <typename T> __device__ __forceinline__ float key_value(uint32_t k) {
+    return fminf(__uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k), LARGEST<T>);
 }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -91,13 +93,12 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const __grid_constant
             key[i] = key[i] ? (key[i] & 0xffff0000u) | (0xffffu - expert(i)) : 0u;
         }
     }
-    constexpr float LIMIT = std::is_same<T, __half>::value ? 65504.f : 3.402823466e38f; // +inf counts as the largest finite value
     auto value = [&](uint32_t k) { // of a key
         if constexpr (std::is_same<T, __half>::value) {
             const uint32_t u = k >> 16;
-            return fminf(__half2float(__ushort_as_half((unsigned short)(u & 0x8000u ? u & 0x7fffu : ~u))), LIMIT);
+            return fminf(__half2float(__ushort_as_half((unsigned short)(u & 0x8000u ? u & 0x7fffu : ~u))), LARGEST<T>);
         } else {
-            return key_value(sizeof(T) == 2 ? (k & 0x80000000u ? k & 0xffff0000u : k | 0xffffu) : k);
+            return key_value<T>(sizeof(T) == 2 ? (k & 0x80000000u ? k & 0xffff0000u : k | 0xffffu) : k);
         }
     };
     uint32_t best = 0;
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const __grid_constant
     if (a.scoring == SCORING_SOFTMAX && !a.normalize) {
         top = value(__reduce_max_sync(0xffffffffu, best));
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i) sum += key[i] ? expf(fminf(to_f32(raw[i]), LIMIT) - top) : 0.f;
+        for (int i = 0; i < PER_LANE; ++i) sum += key[i] ? expf(fminf(to_f32(raw[i]), LARGEST<T>) - top) : 0.f;
         sum = warp_sum(sum);
     }
     uint32_t mine = 0; // key and index of choice `lane`
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_backward_kernel(const __grid
     int index = lane < a.choices ? a.indices[t * a.indices_ld + lane] : -1;
     uint32_t key = (unsigned)index < (unsigned)a.experts ? order_key(to_f32(row[index])) : 0u;
     const bool chosen = key != 0;
-    const float l = key_value(key);
+    const float l = key_value<T>(key);
     float g = chosen ? a.weights[t * a.weights_ld + lane] * a.scale : 0.f;
     const bool dense = a.scoring == SCORING_SOFTMAX && !a.normalize;
     float top = 0.f, inverse = 0.f, inner = 0.f, d;
@@ -189,12 +190,12 @@ __global__ void __launch_bounds__(WARPS * 32) route_backward_kernel(const __grid
         float m = -INFINITY, sum = 0.f;
         for (int e = lane; e < a.experts; e += 32) {
             const uint32_t k = order_key(to_f32(row[e]));
-            if (k) m = fmaxf(m, key_value(k));
+            if (k) m = fmaxf(m, key_value<T>(k));
         }
         top = warp_max(m);
         for (int e = lane; e < a.experts; e += 32) {
             const uint32_t k = order_key(to_f32(row[e]));
-            if (k) sum += expf(key_value(k) - top);
+            if (k) sum += expf(key_value<T>(k) - top);
         }
         inverse = 1.f / warp_sum(sum); // (unused where every expert is masked)
         const float p = chosen ? expf(l - top) * inverse : 0.f;
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_backward_kernel(const __grid
         float v = grad[e];
         if (dense) {
             const uint32_t k = order_key(to_f32(row[e]));
-            if (k) v -= expf(key_value(k) - top) * inverse * inner;
+            if (k) v -= expf(key_value<T>(k) - top) * inverse * inner;
         }
         out[e] = from_f32<T>(v);
     }
