@@ -668,7 +668,7 @@ dnnl_status_t dnnl_cuda_interop_moe_dispatch_primitive_desc_create(dnnl_primitiv
 /* Rows back to their tokens.  SRC grouped [T K, H], SRC_1 positions, WEIGHTS [T, K] (f32; weights_desc may be NULL: 1),
  * SRC_2 residual [T, H] (NULL: none), ATTR_DROPOUT_SEED (dropout_p > 0) -> DST [T, H]:
  *   residual + dropout(sum over K of weight x row).
- * SRC and DST are f32, bf16 or f16, the residual of DST's type; sums are f32.  DST may be the residual's memory. */
+ * A position outside [0, SRC's last offset) names no row.  SRC and DST are f32, bf16 or f16, the residual of DST's type; sums are f32.  DST may be the residual's memory. */
 dnnl_status_t dnnl_cuda_interop_moe_combine_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
         dnnl_engine_t engine, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t positions_desc,
         const_dnnl_memory_desc_t weights_desc, const_dnnl_memory_desc_t residual_desc, const_dnnl_memory_desc_t dst_desc,

@@ -1,9 +1,10 @@
 // The experts' rows back to their tokens, and the gradient.
 //   y[t]  = residual[t] + D(sum_j w[t,j] rows[position[t,j]])
 //   drows[position[t,j]] = w[t,j] D(dy[t]),  dw[t,j] = <D(dy[t]), rows[position[t,j]]>
-// D is dropout (or nothing).  A slot whose position is outside the rows (-1: its token went to no expert there) adds
-// nothing, not even the product of its weight and an infinity, and its dw is zero.  Every row belongs to one slot, so the
-// sums have one order and no atomics.  Bytes bound both: each row is read once (and written once, backward).
+// D is dropout (or nothing).  A slot whose position is outside the groups' rows (-1: its token went to no expert there; at
+// or behind the last offset) adds nothing, not even the product of its weight and an infinity, and its dw is zero.  Every row
+// belongs to one slot, so the sums have one order and no atomics.  Bytes bound both: each row is read once (and written once,
+// backward).
 #include <algorithm>
 
 #include "launch.h"
@@ -12,6 +13,12 @@
 namespace qmm {
 
 namespace {
+
+// Rows that the groups hold.  What lies behind is nobody's: forward does not read it, backward zeroes it in one place.
+__device__ __forceinline__ uint32_t rows_of_groups(const CombineArgs &a) {
+    const int last = ptx::ld_dependent(a.offsets + a.experts - 1);
+    return last < 0 ? 0u : (uint32_t)min((int64_t)last, a.rows);
+}
 
 // GROUP rows of a token are in flight at a time: their loads leave before the first is used.  As many as a token has, up to
 // eight: what eight take in registers costs a token of fewer rows its warps (gradient, 4096 x 4096, two rows 55 us with
@@ -43,12 +50,17 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Co
             pos[j] = j0 + j < a.choices ? ptx::ld_dependent(positions + j0 + j) : -1;
             w[j] = a.weights && j0 + j < a.choices ? ptx::ld_dependent(weights + j0 + j) : 1.f;
         }
+        // (read here and not before the loop: held over it, the bound takes 10 registers and a CTA an SM where rows start anywhere,
+        // 3000 x 8 x 2047 bf16 with dropout 47 us this way / 86)
+        const uint32_t kept = rows_of_groups(a);
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) pos[j] = (uint32_t)pos[j] < kept ? pos[j] : -1;
 #pragma unroll
         for (int j = 0; j < GROUP; ++j)
-            if ((uint32_t)pos[j] < (uint64_t)a.rows) x[j].load((const S *)a.src + (int64_t)pos[j] * a.cols, col, a.cols);
+            if (pos[j] >= 0) x[j].load((const S *)a.src + (int64_t)pos[j] * a.cols, col, a.cols);
 #pragma unroll
         for (int j = 0; j < GROUP; ++j)
-            if ((uint32_t)pos[j] < (uint64_t)a.rows) {
+            if (pos[j] >= 0) {
                 float v[N];
                 x[j].get(v);
 #pragma unroll
@@ -127,6 +139,7 @@ __global__ void __launch_bounds__(BULK_THREADS, 1) combine_bulk_kernel(const __g
         // Serves every PRODUCERS-th group, in the order of their items.  A lane holds position and weight of a row; as many
         // items as have lanes are fetched together, two batches ahead.
         const int k = a.choices, rows = p.tokens * k, batch = 32 / rows;
+        const uint32_t kept = rows_of_groups(a);
         const int of = lane / rows, row = lane - of * rows; // the lane's item of a batch, and its row there
         const uint32_t served = max(1, (p.groups - warp + PRODUCERS - 1) / PRODUCERS), depth = p.stages / p.groups;
         auto item_of = [&](uint32_t turn, uint32_t &group, uint32_t &round) {
@@ -152,7 +165,7 @@ __global__ void __launch_bounds__(BULK_THREADS, 1) combine_bulk_kernel(const __g
         bool more = warp < p.groups;
         for (uint32_t first = 0; more; first += batch) {
             fetch(first + 2 * batch, last_pos, last_w);
-            const bool there = (uint32_t)pos < a.rows;
+            const bool there = (uint32_t)pos < kept;
             const uint32_t all = __ballot_sync(0xffffffffu, there);
             for (int b = 0; b < batch; ++b) {
                 uint32_t group, round;
@@ -293,8 +306,7 @@ __global__ void __launch_bounds__(BULK_THREADS, 1) combine_bulk_kernel(const __g
 
 // Zeros for the rows that belong to no slot, shared out over the grid.
 template <typename S, bool VEC> __device__ __forceinline__ void zero_tail(const CombineArgs &a) {
-    int64_t kept = ptx::ld_dependent(a.offsets + a.experts - 1);
-    kept = kept < 0 ? 0 : kept > a.rows ? a.rows : kept;
+    const int64_t kept = rows_of_groups(a);
     const int64_t end = a.rows * a.cols;
     S *p = (S *)a.diff_src;
     constexpr int STEP = VEC ? 16 / sizeof(S) : 1;
@@ -326,6 +338,7 @@ __global__ void __launch_bounds__(256, GRADIENT_CTAS<S, VEC, GROUP, THREADS>) co
             seed = ld_dependent_u64(a.drop.seed);
             offset = ld_dependent_u64(a.drop.seed + 1);
         }
+        const uint32_t kept = rows_of_groups(a);
         // lane j: position and weight of choice j
         const int my_pos = lane < a.choices ? ptx::ld_dependent(a.positions + t * a.positions_ld + lane) : -1;
         const float my_w = lane < a.choices ? ptx::ld_dependent(a.weights + t * a.weights_ld + lane) : 0.f;
@@ -341,7 +354,7 @@ __global__ void __launch_bounds__(256, GRADIENT_CTAS<S, VEC, GROUP, THREADS>) co
 #pragma unroll
                 for (int j = 0; j < GROUP; ++j) {
                     const uint32_t pos = __shfl_sync(0xffffffffu, my_pos, j0 + j);
-                    if (pos < (uint64_t)a.rows) x[j].load((const S *)a.src + (int64_t)pos * a.cols, col, a.cols);
+                    if (pos < kept) x[j].load((const S *)a.src + (int64_t)pos * a.cols, col, a.cols);
                 }
                 float dy[N];
                 g.get(dy);
@@ -350,7 +363,7 @@ __global__ void __launch_bounds__(256, GRADIENT_CTAS<S, VEC, GROUP, THREADS>) co
                 for (int j = 0; j < GROUP; ++j) {
                     const uint32_t pos = __shfl_sync(0xffffffffu, my_pos, j0 + j);
                     const float w = __shfl_sync(0xffffffffu, my_w, j0 + j);
-                    if (pos < (uint64_t)a.rows) {
+                    if (pos < kept) {
                         float v[N], d[N];
                         x[j].get(v);
 #pragma unroll

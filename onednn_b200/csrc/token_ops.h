@@ -62,7 +62,7 @@ struct CombineArgs {
     int choices, experts;
     int row_dt, tok_dt; // of the grouped rows; of dst, the residual and diff_dst
     const void *src; // grouped rows, dense
-    const int *offsets; // cumulative ends of the groups (backward: the rows behind the last one get no gradient)
+    const int *offsets; // cumulative ends of the groups (the rows behind the last one belong to no slot)
     const int *positions;
     int64_t positions_ld;
     const float *weights; // may be null: 1

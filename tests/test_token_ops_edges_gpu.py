@@ -60,3 +60,81 @@ def test_f16_masks_ties_and_lowest_values(gpu, scoring, normalize):
     base.check(w[~usual], want[~usual], np.abs(want[~usual]) * 64 * EPS + 2.0 ** -126)
     d = base.run_route_backward(gpu[0], logits, idx, np.ones((len(rows), 4)), scoring, normalize)
     assert np.isfinite(d).all() and not d[np.isnan(x) | (x == -inf)].any()
+
+
+# ----------------------------------------------------------------------------------------------- combine
+
+
+def run_combine_backward(eng, rows, offsets, pos, weights, dy, p=0.0, seed=None):
+    """gradients of the rows and of the weights, in memory that holds other values before"""
+    import torch
+    c = base.Call(eng)
+    a = c.api
+    drows, dw = torch.full_like(rows, 7.0), torch.full(tuple(pos.shape), 7.0, device="cuda:0")
+    if p:
+        c.bind(a.ARG_ATTR_DROPOUT_SEED, torch.tensor(seed, dtype=torch.int64, device="cuda:0"))
+    pd = a.moe_combine_backward.primitive_desc(
+        eng, c.bind(a.ARG_DIFF_DST, dy), c.grouped(a.ARG_SRC, rows, offsets), c.bind(a.ARG_SRC_1, pos), c.bind(a.ARG_WEIGHTS, weights),
+        c.grouped(a.ARG_DIFF_SRC, drows, offsets), c.bind(a.ARG_DIFF_WEIGHTS, dw), dropout_p=p)
+    c.run(a.moe_combine_backward, pd).strm.wait()
+    return host(drows), host(dw)
+
+
+def check_both_ways(eng, r, rows, offsets, pos, p):
+    """combine and its gradient for the positions in `pos`, those outside the groups' rows naming nothing"""
+    import torch
+    T, k = pos.shape
+    H, dtype, kept = rows.shape[1], base.Call(eng).name(rows), int(offsets[-1])
+    named = (pos >= 0) & (pos < kept)
+    at = np.where(named, pos, -1)
+    weights = r.standard_normal((T, k)).astype(np.float32)
+    dpos, dweights = torch.from_numpy(pos).cuda(), torch.from_numpy(weights).cuda()
+    seed = (int(r.integers(0, 2 ** 62)), int(r.integers(0, 2 ** 62))) if p else None
+    got = base.run_combine(eng, rows, offsets, dpos, dtype, dweights, None, p, seed)
+    want, size = base.combine_want(rows, at, np.where(named, weights, 0).astype(np.float64), None, p, seed)
+    base.check(got, want, size * EPS * (k + 4) + out_slack(want, dtype))
+    dy = device_matrix(r.standard_normal((T, H)), dtype)
+    drows, dw = run_combine_backward(eng, rows, offsets, dpos, dweights, dy, p, seed)
+    g = R.dropout(host(dy), p, *seed) if p else host(dy)
+    x, slots = host(rows), np.argwhere(named)
+    where = pos[named]
+    want, want_dw, size = np.zeros_like(x), np.zeros((T, k)), np.zeros((T, k))
+    want[where] = weights[named].astype(np.float64)[:, None] * g[slots[:, 0]]
+    terms = g[slots[:, 0]] * x[where]
+    want_dw[named], size[named] = terms.sum(1), np.abs(terms).sum(1)
+    base.check(drows, want, np.abs(want) * 3 * EPS + np.where(want != 0, out_slack(want, dtype), 0))
+    base.check(dw, want_dw, size * EPS * (H + 16) + np.where(named, 2.0 ** -140, 0))
+
+
+FORMS = [  # a warp and a CTA a token, rows on and off 16-byte boundaries, few and many choices, and the ring of bulk copies
+    (37, 8, 2, 104, "bf16", 0.0), (300, 64, 8, 2048, "bf16", 0.2), (300, 12, 3, 2047, "f16", 0.0), (64, 6, 4, 7, "f32", 0.25),
+    (150, 40, 32, 520, "f32", 0.0), (2101, 16, 3, 1032, "bf16", 0.0), (2050, 16, 8, 1024, "bf16", 0.2)]
+
+
+@pytest.mark.parametrize("T,E,k,H,dtype,p", FORMS)
+def test_positions_behind_the_last_group_name_nothing(gpu, T, E, k, H, dtype, p):
+    """the rows behind the last offset belong to no slot: forward leaves them out, backward zeroes them, whoever names them"""
+    import torch
+    r = rng(T, E, k, H)
+    rows, offsets, _, pos = base.make_rows(r, T, E, k, H, dtype, 0.3)
+    kept = int(offsets[-1])
+    assert kept < T * k
+    out = np.argwhere(pos < 0)
+    behind = out[r.random(len(out)) < 0.6]
+    pos[behind[:, 0], behind[:, 1]] = r.integers(kept, T * k, len(behind))
+    check_both_ways(gpu[0], r, rows, offsets, pos, p)
+
+
+@pytest.mark.parametrize("dtype,H", [("f32", 40), ("bf16", 41)])
+def test_offsets_beyond_the_memory_are_cut(gpu, dtype, H):
+    """a last offset above the number of rows, or below zero"""
+    import torch
+    r = rng(H)
+    rows, offsets, dpos, pos = base.make_rows(r, 20, 5, 2, H, dtype, 0)
+    for last, there in ((2 ** 31 - 1, 1.0), (-5, 0.0)):
+        offsets[-1] = last
+        y = base.run_combine(gpu[0], rows, offsets, dpos, "f32")
+        base.check(y, there * host(rows)[pos].sum(1), np.abs(host(rows)[pos]).sum(1) * EPS * 8)
+        drows, dw = run_combine_backward(gpu[0], rows, offsets, dpos, torch.ones((20, 2), device="cuda:0"),
+                                         device_matrix(np.ones((20, H)), dtype))
+        assert (drows == there).all() and (dw != 0).all() == bool(there)
