@@ -674,8 +674,8 @@ dnnl_status_t dnnl_cuda_interop_moe_combine_primitive_desc_create(dnnl_primitive
         const_dnnl_memory_desc_t weights_desc, const_dnnl_memory_desc_t residual_desc, const_dnnl_memory_desc_t dst_desc,
         float dropout_p, const_dnnl_primitive_attr_t attr);
 /* Its gradient.  DIFF_DST [T, H], SRC, SRC_1, WEIGHTS and ATTR_DROPOUT_SEED as forward -> DIFF_SRC grouped, of SRC's type (its
- * offsets are not written; rows behind SRC's last group are zero), DIFF_WEIGHTS [T, K] (f32).  (The residual's gradient is
- * DIFF_DST itself.) */
+ * offsets are not written; rows that no position names, in the groups or behind the last, are zero), DIFF_WEIGHTS [T, K]
+ * (f32).  No row may be named twice.  (The residual's gradient is DIFF_DST itself.) */
 dnnl_status_t dnnl_cuda_interop_moe_combine_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
         dnnl_engine_t engine, const_dnnl_memory_desc_t diff_dst_desc, const_dnnl_memory_desc_t src_desc,
         const_dnnl_memory_desc_t positions_desc, const_dnnl_memory_desc_t weights_desc,

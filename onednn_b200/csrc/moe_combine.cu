@@ -316,21 +316,92 @@ template <typename S, bool VEC> __device__ __forceinline__ void zero_tail(const 
     }
 }
 
+// Rows of the groups that no slot names - a program took their positions back after dispatch - have a gradient of zero.  The
+// first CTAs of the grid look for them while the others work on tokens: each goes through all positions and marks those of its
+// part of the rows in shared memory.  Marked rows are the tokens', unmarked ones its own, so nothing is written twice.
+// What a CTA takes grows with all positions, whatever its part: 32 CTAs, more only where the marks would not fit.  (us a call,
+// without / with: 4096 x 8 rows of 4096 bf16 89.0 / 88.4, of 512 12.6 / 12.3, of 128 7.9 / 9.1; 131072 x 8 of 128 214 / 223.)
+constexpr int MARK_ROWS = 32768; // of a CTA at most
+inline unsigned mark_ctas(int64_t rows) {
+    return (unsigned)std::max((rows + MARK_ROWS - 1) / MARK_ROWS, std::min<int64_t>(32, (rows + 255) / 256));
+}
+
+template <typename S, bool VEC> __device__ __forceinline__ void zero_unnamed(const CombineArgs &a, uint32_t *marks) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const uint32_t part = ((uint32_t)((a.rows + a.mark_ctas - 1) / a.mark_ctas) + 31) / 32 * 32, first = blockIdx.x * part;
+    const uint32_t kept = rows_of_groups(a); // (not waited for before the positions)
+    for (uint32_t i = threadIdx.x; i < part / 32; i += 256) marks[i] = 0;
+    __syncthreads();
+    auto mark = [&](uint32_t position) {
+        const uint32_t at = position - first;
+        if (at < part) atomicOr(&marks[at / 32], 1u << (at % 32));
+    };
+    const uint32_t slots = (uint32_t)(a.tokens * a.choices);
+    uint32_t done = 0;
+    if (a.positions_ld == a.choices && (uintptr_t)a.positions % 16 == 0) {
+        constexpr int FLIGHT = 8; // of four each
+        for (uint32_t q = threadIdx.x; q < slots / 4; q += 256 * FLIGHT) {
+            uint4 at[FLIGHT];
+#pragma unroll
+            for (int f = 0; f < FLIGHT; ++f) {
+                at[f] = make_uint4(~0u, ~0u, ~0u, ~0u);
+                if (q + 256 * f < slots / 4) at[f] = ptx::ld_dependent((const uint4 *)a.positions + q + 256 * f);
+            }
+#pragma unroll
+            for (int f = 0; f < FLIGHT; ++f) {
+                mark(at[f].x);
+                mark(at[f].y);
+                mark(at[f].z);
+                mark(at[f].w);
+            }
+        }
+        done = slots / 4 * 4;
+    }
+    constexpr int FLIGHT = 16;
+    for (uint32_t s0 = done + threadIdx.x; s0 < slots; s0 += 256 * FLIGHT) {
+        uint32_t at[FLIGHT];
+#pragma unroll
+        for (int f = 0; f < FLIGHT; ++f) {
+            const uint32_t s = s0 + 256 * f, t = s / (uint32_t)a.choices;
+            at[f] = ~0u;
+            if (s < slots) at[f] = (uint32_t)ptx::ld_dependent(a.positions + (int64_t)t * a.positions_ld + (s - t * (uint32_t)a.choices));
+        }
+#pragma unroll
+        for (int f = 0; f < FLIGHT; ++f) mark(at[f]);
+    }
+    __syncthreads();
+    const uint32_t count = kept > first ? min(part, kept - first) : 0;
+    for (uint32_t w = warp; w * 32 < count; w += 8) {
+        uint32_t gone = ~marks[w] & (count - w * 32 >= 32 ? 0xffffffffu : (1u << (count - w * 32)) - 1);
+        for (; gone; gone &= gone - 1) {
+            S *row = (S *)a.diff_src + (int64_t)(first + w * 32 + __ffs(gone) - 1) * a.cols;
+            constexpr int STEP = VEC ? 16 / sizeof(S) : 1;
+            for (int64_t c = lane * STEP; c < a.cols; c += 32 * STEP) {
+                if constexpr (VEC) *reinterpret_cast<uint4 *>(row + c) = make_uint4(0, 0, 0, 0);
+                else row[c] = from_f32<S>(0.f);
+            }
+        }
+    }
+}
+
 // CTAs per SM that the gradient's registers are cut to (0: the compiler's choice).  4096 tokens, the same inputs every call: bf16,
 // eight rows of 4096 89 us three / 101 four (with positions and weights in every thread's registers 100 uncut / 103 two / 95
-// three); f32 220 uncut / 170 two / 238 three; rows that start anywhere 102 two / 154 three.
-template <typename S, bool VEC, int GROUP, int THREADS>
-constexpr int GRADIENT_CTAS = !VEC || sizeof(S) == 4 ? 2 : GROUP == 8 && THREADS == 256 ? 3 : 0;
+// three), four rows of 4096 with dropout 51.5 uncut / 47.7 five, without 52.0 / 50.3; f32 220 uncut / 170 two / 238 three; rows
+// that start anywhere 102 two / 154 three, two rows of 2047 bf16 without dropout 21.9 four / 20.7 five.
+template <typename S, typename D, bool VEC, bool DROP, int GROUP, int THREADS>
+constexpr int GRADIENT_CTAS = !VEC && !DROP && GROUP == 2 ? 5 : !VEC || sizeof(S) == 4 ? 2 : THREADS == 32 || GROUP == 2 ? 0 : GROUP == 8 ? 3 : sizeof(D) == 2 ? 5 : 0;
 
 // THREADS of the 256 of a CTA work on a token: all of them, or a warp where rows are short.
 template <typename S, typename D, bool VEC, bool DROP, int THREADS, int GROUP>
-__global__ void __launch_bounds__(256, GRADIENT_CTAS<S, VEC, GROUP, THREADS>) combine_backward_kernel(const __grid_constant__ CombineArgs a) {
+__global__ void __launch_bounds__(256, GRADIENT_CTAS<S, D, VEC, DROP, GROUP, THREADS>) combine_backward_kernel(const __grid_constant__ CombineArgs a) {
     __shared__ __align__(16) uint32_t words[DROP && !VEC ? 8 * 128 : 4];
     __shared__ float partial[8][GROUP];
+    __shared__ uint32_t marks[MARK_ROWS / 32];
     ptx::grid_dependency_wait();
     constexpr int N = Cols<S, VEC>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    const int64_t t = THREADS == 256 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
+    const uint32_t block = blockIdx.x - a.mark_ctas; // (wraps beyond all tokens for the CTAs that mark)
+    const int64_t t = THREADS == 256 ? (int64_t)block : (int64_t)block * 8 + warp;
     const int64_t units = (row_units<VEC>(a.cols, DROP) + 31) / 32 * 32;
     if (t < a.tokens) {
         uint64_t seed = 0, offset = 0;
@@ -398,6 +469,7 @@ __global__ void __launch_bounds__(256, GRADIENT_CTAS<S, VEC, GROUP, THREADS>) co
             }
         }
     }
+    if (blockIdx.x < a.mark_ctas) zero_unnamed<S, VEC>(a, marks);
     zero_tail<S, VEC>(a);
 }
 
@@ -441,9 +513,11 @@ template <typename S, typename D, bool DROP> int launch_forward(const CombineArg
 
 template <typename S, typename D, bool VEC, bool DROP, int GROUP> int launch_backward(const CombineArgs &a, cudaStream_t st) {
     const bool wide = row_units<VEC>(a.cols, DROP) > 64;
-    const int64_t grid = wide ? a.tokens : (a.tokens + 7) / 8;
+    CombineArgs b = a;
+    b.mark_ctas = mark_ctas(a.rows);
+    const int64_t grid = (wide ? a.tokens : (a.tokens + 7) / 8) + b.mark_ctas;
     if (grid > 0x7fffffff) return 3;
-    return launch_dependent(wide ? combine_backward_kernel<S, D, VEC, DROP, 256, GROUP> : combine_backward_kernel<S, D, VEC, DROP, 32, GROUP>, a,
+    return launch_dependent(wide ? combine_backward_kernel<S, D, VEC, DROP, 256, GROUP> : combine_backward_kernel<S, D, VEC, DROP, 32, GROUP>, b,
             (unsigned)grid, 256, 0, st);
 }
 template <typename S, typename D, bool DROP> int launch_backward(const CombineArgs &a, bool vec, cudaStream_t st) {

@@ -79,6 +79,7 @@ struct CombineArgs {
     void *diff_src;
     float *diff_weights;
     int64_t diff_weights_ld;
+    unsigned mark_ctas; // the launcher's: CTAs that look for rows without a slot
 };
 int launch_combine(const CombineArgs &a, int sm_count, cudaStream_t st);
 int launch_combine_backward(const CombineArgs &a, int sm_count, cudaStream_t st);

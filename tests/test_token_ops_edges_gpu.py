@@ -138,3 +138,38 @@ def test_offsets_beyond_the_memory_are_cut(gpu, dtype, H):
         drows, dw = run_combine_backward(gpu[0], rows, offsets, dpos, torch.ones((20, 2), device="cuda:0"),
                                          device_matrix(np.ones((20, H)), dtype))
         assert (drows == there).all() and (dw != 0).all() == bool(there)
+
+
+@pytest.mark.parametrize("T,E,k,H,dtype,p", FORMS + [(9000, 64, 4, 16, "bf16", 0.0), (70001, 8, 4, 8, "f32", 0.0)])
+def test_rows_whose_slots_were_taken_back_have_no_gradient(gpu, T, E, k, H, dtype, p):
+    """positions a program set to -1 after dispatch (tokens over an expert's capacity): the rows stay in their groups, and
+    what the groups' products make of their gradient counts; it is zero"""
+    r = rng(T, E, k, H, 1)
+    rows, offsets, _, pos = base.make_rows(r, T, E, k, H, dtype, 0.1)
+    taken = r.random(pos.shape) < 0.3
+    taken[T // 2] = True
+    taken[:, 0] |= pos[:, 0] < r.integers(0, 40)  # whole words of rows
+    pos[taken] = -1
+    check_both_ways(gpu[0], r, rows, offsets, pos, p)
+
+
+@pytest.mark.parametrize("T,k,pitch,offset", [(3000, 3, 5, 1), (2000, 8, 8, 1), (41, 4, 9, 0)])
+def test_positions_inside_a_wider_buffer(gpu, T, k, pitch, offset):
+    r = rng(T, k)
+    rows, offsets, _, pos = base.make_rows(r, T, 11, k, 72, "bf16", 0.1)
+    pos[r.random(pos.shape) < 0.2] = -1
+    dpos = device_matrix(pos, "s32", pitch, offset)
+    w, dy = device_matrix(r.standard_normal((T, k)), "f32", pitch, offset), device_matrix(r.standard_normal((T, 72)), "bf16")
+    drows, dw = run_combine_backward(gpu[0], rows, offsets, dpos, w, dy)
+    named = pos >= 0
+    want, g = np.zeros(tuple(rows.shape)), host(dy)
+    want[pos[named]] = host(w)[named][:, None] * g[np.argwhere(named)[:, 0]]
+    base.check(drows, want, np.abs(want) * 3 * EPS + np.where(want != 0, out_slack(want, "bf16"), 0))
+    assert not dw[~named].any() and dw[named].all()
+
+
+def test_no_slot_names_a_row(gpu):
+    r = rng(2)
+    rows, offsets, _, pos = base.make_rows(r, 700, 6, 2, 264, "bf16", 0)
+    pos[:] = -1
+    check_both_ways(gpu[0], r, rows, offsets, pos, 0.0)
