@@ -661,7 +661,10 @@ dnnl_status_t dnnl_cuda_interop_moe_route_backward_primitive_desc_create(dnnl_pr
 /* Tokens into grouped memory.  SRC [T, H] (any type of 8, 16 or 32 bits), SRC_1 indices [T, K] (s32; one outside [0, E)
  * gets no row) -> DST grouped [T K, H] of the same type: values, and the offsets, which this primitive writes; DST_1
  * positions [T, K] (s32): the row of each (token, choice), -1 without one.  Rows of an expert stand in the order of their
- * tokens.  Rows behind the last group are zero.  Its gradient is moe_combine without weights. */
+ * tokens.  Rows behind the last group are zero.  Its gradient is moe_combine without weights.
+ *   Its scratchpad holds counts between its kernels.  With the library's scratchpad, executions of one primitive that overlap
+ *   on the GPU (other streams, other threads) leave undefined contents in their outputs: serialize them on one stream, or
+ *   create the primitive with the user scratchpad mode and give each stream a buffer of its own. */
 dnnl_status_t dnnl_cuda_interop_moe_dispatch_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
         dnnl_engine_t engine, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t indices_desc,
         const_dnnl_memory_desc_t dst_desc, const_dnnl_memory_desc_t positions_desc, const_dnnl_primitive_attr_t attr);

@@ -155,7 +155,7 @@ template <bool SELF> __global__ void __launch_bounds__(THREADS) dispatch_place_k
 
 // Zeros for the rows behind the last group, shared out over the grid.  E: an element.
 template <typename E> __device__ __forceinline__ void zero_behind(const DispatchArgs &a, int kept) {
-    char *begin = a.dst + (int64_t)kept * a.row_bytes, *end = a.dst + (int64_t)(a.tokens * a.choices) * a.row_bytes;
+    char *begin = a.dst + (int64_t)max(kept, 0) * a.row_bytes, *end = a.dst + (int64_t)(a.tokens * a.choices) * a.row_bytes;
     if (begin >= end) return;
     char *low = (char *)(((uintptr_t)begin + 15) & ~(uintptr_t)15), *high = (char *)((uintptr_t)end & ~(uintptr_t)15);
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -166,10 +166,14 @@ template <typename E> __device__ __forceinline__ void zero_behind(const Dispatch
     }
 }
 
+// Both copies take the places from memory that the kernel before has written, and store only inside dst: two executions at a
+// time on one scratchpad overwrite each other's counts, and the places made of them lie anywhere.
+//
 // Rows that start and end on 16-byte boundaries: a thread reads UNITS units of tokens' rows and stores each to its row's places.
 template <int UNITS> __global__ void __launch_bounds__(256) dispatch_copy_kernel(const __grid_constant__ DispatchArgs a) {
     ptx::grid_dependency_wait();
     const int64_t units = a.row_bytes / 16, total = a.tokens * units, first = (int64_t)blockIdx.x * (256 * UNITS) + threadIdx.x;
+    const uint32_t slots = (uint32_t)a.tokens * a.choices;
     uint4 v[UNITS];
     int64_t t[UNITS];
     char *dst[UNITS];
@@ -193,7 +197,7 @@ template <int UNITS> __global__ void __launch_bounds__(256) dispatch_copy_kernel
         for (int q = 0; q < UNITS; ++q)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (to[q][j] >= 0) *(uint4 *)(dst[q] + (int64_t)to[q][j] * a.row_bytes) = v[q];
+                if ((uint32_t)to[q][j] < slots) *(uint4 *)(dst[q] + (int64_t)to[q][j] * a.row_bytes) = v[q];
     }
     zero_behind<uint32_t>(a, ptx::ld_dependent(a.offsets + a.experts - 1));
 }
@@ -214,7 +218,8 @@ template <typename E> __global__ void __launch_bounds__(256) dispatch_shift_kern
         const int low = -(int)min(t * a.src_pitch, (int64_t)bytes);
         const int high = bytes + (int)min((a.tokens - 1 - t) * a.src_pitch, (int64_t)bytes);
         const uint32_t row_at = (uint32_t)(uintptr_t)row, dst_at = (uint32_t)(uintptr_t)a.dst; // for their last four bits
-        const int mine = lane < a.choices ? ptx::ld_dependent(a.positions + t * a.positions_ld + lane) : -1;
+        int mine = lane < a.choices ? ptx::ld_dependent(a.positions + t * a.positions_ld + lane) : -1;
+        if ((uint32_t)mine >= (uint32_t)a.tokens * a.choices) mine = -1;
         for (int j = 0; j < a.choices; ++j) {
             const int to = __shfl_sync(0xffffffffu, mine, j);
             if (to < 0) continue;

@@ -173,3 +173,57 @@ def test_no_slot_names_a_row(gpu):
     rows, offsets, _, pos = base.make_rows(r, 700, 6, 2, 264, "bf16", 0)
     pos[:] = -1
     check_both_ways(gpu[0], r, rows, offsets, pos, 0.0)
+
+
+# ---------------------------------------------------------------------------------------------- dispatch
+
+
+def guarded(shape, dtype, value):
+    """a tensor in the middle of a buffer, and a check that nothing around it changed"""
+    import torch
+    n, pad = int(np.prod(shape)), 4096
+    buf = torch.full((n + 2 * pad,), value, dtype=dtype, device="cuda:0")
+
+    def untouched():
+        return bool((buf[:pad] == value).all() and (buf[pad + n:] == value).all())
+    return buf[pad:pad + n].view(shape), untouched
+
+
+@pytest.mark.parametrize("H", [64, 65])  # both copies
+def test_one_dispatch_on_two_streams_with_scratchpads_of_their_own(gpu, H):
+    """one primitive in flight twice, above the number of slots from which counts go through the scratchpad; nothing is
+    written around the outputs and the scratchpads"""
+    import torch
+    from onednn_b200 import api as a
+    eng, T, E, k = gpu[0], 6000, 48, 3
+    attr = a.primitive_attr()
+    attr.set_scratchpad_mode(a.SCRATCHPAD_MODE_USER)
+    prim, calls = None, []
+    for n in range(2):
+        r = rng(H, n)
+        x, idx = device_matrix(r.standard_normal((T, H)), "bf16"), base.choices(r, T, E, k, 0.1)
+        c = base.Call(eng, torch.cuda.Stream().cuda_stream)
+        rows, rows_ok = guarded((T * k, H), torch.bfloat16, 7)
+        offsets, offsets_ok = guarded((E,), torch.int32, 7)
+        pos, pos_ok = guarded((T, k), torch.int32, 7)
+        mds = [c.bind(a.ARG_SRC, x), c.bind(a.ARG_SRC_1, torch.from_numpy(idx).cuda()), c.grouped(a.ARG_DST, rows, offsets),
+               c.bind(a.ARG_DST_1, pos)]
+        if prim is None:
+            pd = a.moe_dispatch.primitive_desc(eng, *mds, attr=attr)
+            prim = a.moe_dispatch(pd)
+        md = pd.query_md(136)
+        assert md.get_size() > 0
+        scratch, scratch_ok = guarded((md.get_size(),), torch.uint8, 255)
+        c.args[a.ARG_SCRATCHPAD] = a.memory(md, eng, scratch.data_ptr())
+        calls.append((c, x, idx, rows, offsets, pos, scratch, (rows_ok, offsets_ok, pos_ok, scratch_ok)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for call in calls:
+            prim.execute(call[0].strm, call[0].args)
+    torch.cuda.synchronize()
+    for c, x, idx, rows, offsets, pos, scratch, checks in calls:
+        ends, want_pos, order = R.sort_slots(idx, E)
+        want = np.zeros((T * k, H))
+        want[:order.size] = host(x)[order // k]
+        assert np.array_equal(host(offsets), ends) and np.array_equal(host(pos), want_pos) and np.array_equal(host(rows), want)
+        assert all(ok() for ok in checks) and not (scratch == 255).all()
