@@ -637,12 +637,15 @@ typedef enum {
     dnnl_cuda_interop_scoring_sigmoid = 1 /* 1 / (1 + exp(-l)) */
 } dnnl_cuda_interop_scoring_t;
 
+/* dnnl_types.h: the same numbers, whichever header says them */
 #ifndef DNNL_ARG_DST_1
 #define DNNL_ARG_DST_1 18
 #define DNNL_ARG_DIFF_SRC 129
 #define DNNL_ARG_DIFF_DST 145
 #define DNNL_ARG_DIFF_WEIGHTS 161
-#define DNNL_ARG_ATTR_DROPOUT_SEED 510
+#endif
+#ifndef DNNL_ARG_ATTR_DROPOUT_SEED
+#define DNNL_ARG_ATTR_DROPOUT_SEED 511
 #endif
 
 /* Router.  SRC logits [T, E] (f32, bf16, f16) -> DST weights [T, K] (f32), DST_1 indices [T, K] (s32), by falling logit,

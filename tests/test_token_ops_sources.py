@@ -1,8 +1,15 @@
-"""The operators around an expert layer's products, and dropout: what cannot be seen from results on a device without a
-misuse or a fault there, read from the sources instead."""
+"""The operators around an expert layer's products, and dropout: what the sources and the header say - what cannot be seen
+from results on a device without a misuse there, and what a C or C++ program meets."""
+import os
 import re
+import shutil
+import subprocess
+
+import pytest
 
 from test_dependent_launch import _functions, _source
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_places_out_of_memory_are_bounded_before_a_store():
@@ -15,3 +22,39 @@ def test_places_out_of_memory_are_bounded_before_a_store():
     assert re.search(r"if \(\(uint32_t\)mine >= \(uint32_t\)a\.tokens \* a\.choices\) mine = -1;", shift)
     assert re.search(r"to = __shfl_sync\(0xffffffffu, mine, j\);\s*if \(to < 0\) continue;", shift)
     assert "max(kept, 0)" in functions["zero_behind"]
+
+
+NAMES = ["SRC", "SRC_1", "SRC_2", "DST", "DST_1", "WEIGHTS", "DIFF_SRC", "DIFF_DST", "DIFF_WEIGHTS", "ATTR_DROPOUT_SEED"]
+# as oneDNN's dnnl_types.h documents them
+NUMBERS = [1, 2, 3, 17, 18, 33, 129, 145, 161, 511]
+
+
+def argument_ids(tmp_path, first=None, include=()):
+    """the ids a C++ program sees that includes `first` and then this library's header"""
+    source = "".join('#include "%s"\n' % h for h in ([first] if first else []) + ["dnnl_b200.h"])
+    source += "#include <stdio.h>\nint main() {" + "".join('printf("%%d ", DNNL_ARG_%s);' % n for n in NAMES) + " return 0; }\n"
+    (tmp_path / "ids.cpp").write_text(source)
+    exe = str(tmp_path / "ids")
+    r = subprocess.run([shutil.which("g++") or "/usr/bin/g++", "-std=c++17", str(tmp_path / "ids.cpp"), "-I" + os.path.join(ROOT, "include"), "-o", exe]
+                       + ["-I" + i for i in include], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return [int(v) for v in subprocess.run([exe], capture_output=True, text=True, timeout=60).stdout.split()]
+
+
+def test_argument_ids_are_those_of_the_reference(tmp_path, host_engine):
+    """a program that includes oneDNN's own header first gets its numbers for these arguments, and the library has to know
+    a tensor by them"""
+    from onednn_b200 import api
+    assert [getattr(api, "ARG_" + n) for n in NAMES] == NUMBERS
+    assert argument_ids(tmp_path) == NUMBERS
+    m = api.memory.desc((5, 4), 3, (4, 1))
+    pd = api.dropout.primitive_desc(host_engine, m, m, 0.5)
+    assert pd.query_md(255, 511) == api.memory.desc((2,), 16, (1,)) and pd.query_md(255, 510).get_ndims() == 0
+
+
+def test_argument_ids_behind_the_reference_header(tmp_path):
+    import torch
+    include = os.path.join(os.path.dirname(torch.__file__), "include")
+    if not os.path.exists(os.path.join(include, "oneapi", "dnnl", "dnnl.h")):
+        pytest.skip("no oneDNN header on this machine")
+    assert argument_ids(tmp_path, "oneapi/dnnl/dnnl.h", [include]) == NUMBERS
