@@ -939,7 +939,7 @@ dnnl_status_t dnnl_primitive_desc_query(const_dnnl_primitive_desc_t pd, dnnl_que
     switch ((int)what) {
         case dnnl_query_engine:
         case dnnl_query_scratchpad_engine: *(dnnl_engine_t *)result = pd->engine; break;
-        case dnnl_query_primitive_kind: *(dnnl_primitive_kind_t *)result = pd->kind; break;
+        case dnnl_query_primitive_kind: memcpy(result, &pd->kind, sizeof(int)); break; // (the caller's may be either enum)
         case dnnl_query_num_of_inputs_s32:
             *(int *)result = pd->kind == dnnl_reorder ? 1 : 2 + (pd->bias.ndims != 0) + n_binary;
             break;

@@ -190,7 +190,7 @@ std::string pd_info_string(const dnnl_primitive_desc &pd) {
         }
         std::ostringstream aux;
         if (pd.token_op.p != 0.f) aux << "p:" << pd.token_op.p;
-        else if (pd.kind == (int)dnnl_cuda_interop_moe_route || pd.kind == (int)dnnl_cuda_interop_moe_route_backward)
+        else if (pd.kind == dnnl_cuda_interop_moe_route || pd.kind == dnnl_cuda_interop_moe_route_backward)
             aux << "scoring:" << (pd.token_op.scoring ? "sigmoid" : "softmax") << " normalize:" << pd.token_op.normalize
                 << " scale:" << pd.token_op.scale;
         const dnnl_memory_desc *x = pd.token_op.find(DNNL_ARG_DIFF_DST) ? pd.token_op.find(DNNL_ARG_DIFF_DST) : pd.token_op.find(DNNL_ARG_SRC);
@@ -340,7 +340,8 @@ const char *dnnl_prim_kind2str(dnnl_primitive_kind_t v) {
     static const char *const names[] = {"undef", "reorder", "shuffle", "concat", "sum", "convolution", "deconvolution",
             "eltwise", "lrn", "batch_normalization", "inner_product", "rnn", "gemm", "binary", "matmul", "resampling",
             "pooling", "reduction", "prelu", "softmax", "layer_normalization", "group_normalization"};
-    const int i = (int)v;
+    int i; // what the caller passed, in or outside the enum
+    memcpy(&i, &v, sizeof(i));
     if (is_token_op(i)) return token_op_name(i);
     return i >= 0 && i < (int)(sizeof(names) / sizeof(*names)) ? names[i] : "unknown prim_kind";
 }

@@ -167,7 +167,7 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
         op.args[DNNL_ARG_ATTR_DROPOUT_SEED] = seed;
     }
     std::unique_ptr<dnnl_primitive_desc> pd(new dnnl_primitive_desc);
-    pd->kind = (dnnl_primitive_kind_t)kind;
+    pd->kind = kind;
     pd->engine = engine;
     if (attr) pd->attr = *attr;
     pd->impl_name = std::string("cuda:simt:") + token_op_name(kind);
@@ -324,7 +324,7 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
                 if (!agree(want.dims[d], got.dims[d])) return dnnl_invalid_arguments;
             want = got;
         }
-        const dnnl_status_t st = check((int)pd.kind, settled);
+        const dnnl_status_t st = check(pd.kind, settled);
         if (st != dnnl_success) return st;
         op = &settled;
     }
@@ -361,7 +361,7 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
         cudaEventRecord(ev0, stream->stream);
     }
     profiling_begin(stream);
-    const int rc = launch(primitive, (int)pd.kind, *op, bound, scratch, stream->stream);
+    const int rc = launch(primitive, pd.kind, *op, bound, scratch, stream->stream);
     profiling_end(stream);
     if (verbose) {
         cudaEventRecord(ev1, stream->stream);

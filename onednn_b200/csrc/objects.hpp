@@ -158,8 +158,9 @@ struct token_op_t {
 };
 
 struct dnnl_primitive_desc {
-    // dnnl_reorder: only src, dst and attr are used; the kinds of dnnl_cuda_interop_primitive_kind_t: attr and token_op
-    dnnl_primitive_kind_t kind = dnnl_matmul;
+    // dnnl_reorder: only src, dst and attr are used; the kinds of dnnl_cuda_interop_primitive_kind_t: attr and token_op.  Their
+    // values lie outside dnnl_primitive_kind_t, so the kind is a number here.
+    int kind = dnnl_matmul;
     token_op_t token_op;
     dnnl_engine_t engine = nullptr;
     dnnl_memory_desc src, wei, bias, dst, scratchpad;

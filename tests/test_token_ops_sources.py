@@ -58,3 +58,21 @@ def test_argument_ids_behind_the_reference_header(tmp_path):
     if not os.path.exists(os.path.join(include, "oneapi", "dnnl", "dnnl.h")):
         pytest.skip("no oneDNN header on this machine")
     assert argument_ids(tmp_path, "oneapi/dnnl/dnnl.h", [include]) == NUMBERS
+
+
+def test_kinds_outside_the_reference_enum_are_numbers(host_engine):
+    """dnnl_primitive_kind_t ends at 0x7fff; a C++ enum object may not hold the kinds of this library's own primitives"""
+    import ctypes as C
+
+    from onednn_b200 import api
+    sources = os.path.join(ROOT, "onednn_b200", "csrc")
+    for f in sorted(os.listdir(sources)):
+        if f.endswith((".cu", ".hpp", ".h", ".cuh")):
+            assert not re.search(r"\(dnnl_primitive_kind_t\s*\*?\)", open(os.path.join(sources, f)).read()), f
+    assert re.search(r"struct dnnl_primitive_desc \{[^}]*\n    int kind = dnnl_matmul;", _source("objects.hpp"))
+    lib, m, kind = api.lib(), api.memory.desc((5, 4), 3, (4, 1)), C.c_int()
+    pd = api.dropout.primitive_desc(host_engine, m, m, 0.5)
+    assert lib.dnnl_primitive_desc_query(pd._h, 2, 0, C.byref(kind)) == 0 and kind.value == 0x10006
+    lib.dnnl_prim_kind2str.restype = C.c_char_p
+    assert [lib.dnnl_prim_kind2str(k) for k in (0x10006, 0x10001, 0x10007, 14, 1)] == [
+        b"dropout", b"moe_route", b"unknown prim_kind", b"matmul", b"reorder"]
