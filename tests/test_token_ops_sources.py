@@ -76,3 +76,16 @@ def test_kinds_outside_the_reference_enum_are_numbers(host_engine):
     lib.dnnl_prim_kind2str.restype = C.c_char_p
     assert [lib.dnnl_prim_kind2str(k) for k in (0x10006, 0x10001, 0x10007, 14, 1)] == [
         b"dropout", b"moe_route", b"unknown prim_kind", b"matmul", b"reorder"]
+
+
+def test_the_example_compares_every_gradient_that_it_makes():
+    """examples/moe_layer.py: what the steps of its way back write is what run() compares with plain torch"""
+    text = open(os.path.join(ROOT, "examples", "moe_layer.py")).read()
+    steps = re.search(r"def backward\(self\):\s*for step in \(([^)]*)\)", text).group(1)
+    written = set()
+    for step in re.findall(r"self\.(\w+)", steps):
+        body = re.search(r"s = self\.%s = Step\(self\)(.*?)\n\n" % step, text, re.S).group(1)
+        written |= set(re.findall(r"api\.ARG_(?:DST|DIFF_SRC|DIFF_WEIGHTS), self\.(\w+)\)", body))
+    compared = re.search(r"results = \{(.*?)\}\n", text).group(1)
+    assert written == {"drows", "dw", "dlogits"}
+    assert all("layer." + name in compared for name in written)
