@@ -89,3 +89,18 @@ def test_the_example_compares_every_gradient_that_it_makes():
     compared = re.search(r"results = \{(.*?)\}\n", text).group(1)
     assert written == {"drows", "dw", "dlogits"}
     assert all("layer." + name in compared for name in written)
+
+
+def test_an_empty_matrix_may_have_any_strides(host_engine):
+    """tensor libraries give matrices without elements strides of zero"""
+    from onednn_b200 import api
+    md, O = api.memory.desc, api.RUNTIME_DIM_VAL
+    f, i = md((0, 2), 3, (0, 0)), md((0, 2), 4, (0, 0))
+    rows = md.grouped((0, 4), 3, 0, 8)
+    api.moe_route.primitive_desc(host_engine, md((0, 8), 3, (0, 0)), f, i)
+    api.moe_dispatch.primitive_desc(host_engine, md((0, 4), 3, (0, 0)), i, rows, i)
+    api.moe_combine.primitive_desc(host_engine, rows, i, md((0, 4), 3, (0, 0)), weights_md=f)
+    api.dropout.primitive_desc(host_engine, md((5, 0), 3, (0, 0)), md((5, 0), 3, (0, 0)), 0.5)
+    with pytest.raises(api.error) as e:  # but a known pitch of outputs with rows still counts
+        api.dropout.primitive_desc(host_engine, md((5, 4), 3, (4, 1)), md((5, 4), 3, (0, 1)), 0.5)
+    assert e.value.status == api.unimplemented
