@@ -227,3 +227,38 @@ def test_one_dispatch_on_two_streams_with_scratchpads_of_their_own(gpu, H):
         want[:order.size] = host(x)[order // k]
         assert np.array_equal(host(offsets), ends) and np.array_equal(host(pos), want_pos) and np.array_equal(host(rows), want)
         assert all(ok() for ok in checks) and not (scratch == 255).all()
+
+
+@pytest.mark.parametrize("T,E,k,H,dtype,pitch", [(128, 8, 2, 4096, "bf16", 0), (100, 5, 2, 1001, "f16", 1004), (60, 7, 4, 5003, "s8", 0)])
+def test_few_slots_of_wide_rows(gpu, T, E, k, H, dtype, pitch):
+    """the form of one launch, rows wide enough that its grid goes round"""
+    r = rng(T, H)
+    x = device_matrix(r.integers(-100, 100, (T, H)).astype(np.float64), dtype, pitch)
+    idx = base.choices(r, T, E, k, 0.1)
+    rows, offsets, pos = base.run_dispatch(gpu[0], x, idx, E)
+    ends, want_pos, order = R.sort_slots(idx, E)
+    want = np.zeros((T * k, H))
+    want[:order.size] = host(x)[order // k]
+    assert np.array_equal(host(offsets), ends) and np.array_equal(host(pos), want_pos) and np.array_equal(host(rows), want)
+
+
+# ----------------------------------------------------------------------------------------------- dropout
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,N,p,res,pitch", [
+    (1, 3 * 148 * 4 * 4096 + 4101, 0.1, True, 0), (1, 2 * 148 * 4 * 4096 + 3, 0.5, False, 0), (2600, 2048, 0.2, True, 2056),
+    (1700, 3076, 0.3, False, 3080), (4099, 1367, 0.25, True, 1371), (9001, 255, 0.1, False, 0), (1200, 2001, 1.0, True, 2003),
+    (1500, 1024, 1.0, False, 0)])
+def test_dropout_of_tensors_that_outnumber_the_grid(gpu, M, N, p, res, pitch, dtype):
+    """every form whose grid stays goes round at least once: one long row, aligned rows, rows that start anywhere, p = 1"""
+    r = rng(M, N)
+    x = device_matrix(r.standard_normal((M, N), dtype=np.float32), dtype, pitch)
+    residual = device_matrix(r.standard_normal((M, N), dtype=np.float32), dtype) if res else None
+    seed = (int(r.integers(0, 2 ** 62)), int(r.integers(0, 2 ** 62)))
+    got = base.run_dropout(gpu[0], x, p, seed, residual, pitch=pitch)
+    want = R.dropout(host(x), p, *seed)
+    size = np.abs(want)
+    if res:
+        want, size = want + host(residual), size + np.abs(host(residual))
+    base.check(got, want, size * 3 * EPS + out_slack(want, dtype))
