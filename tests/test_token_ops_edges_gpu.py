@@ -242,6 +242,45 @@ def test_few_slots_of_wide_rows(gpu, T, E, k, H, dtype, pitch):
     assert np.array_equal(host(offsets), ends) and np.array_equal(host(pos), want_pos) and np.array_equal(host(rows), want)
 
 
+@pytest.mark.parametrize("mode", ["library", "user"])
+def test_scratchpad_of_many_slots(gpu, mode):
+    """above the number of slots from which counts go through the scratchpad; a user's holds other values before every call"""
+    import torch
+    from onednn_b200 import api as a
+    r = rng(12)
+    T, E, k, H = 4000, 24, 3, 16
+    attr = a.primitive_attr()
+    attr.set_scratchpad_mode(a.SCRATCHPAD_MODE_USER if mode == "user" else a.SCRATCHPAD_MODE_LIBRARY)
+    x, idx = device_matrix(r.standard_normal((T, H)), "f32"), base.choices(r, T, E, k, 0.1)
+    c = base.Call(gpu[0])
+    rows, offsets = torch.empty((T * k, H), device="cuda:0"), torch.empty((E,), device="cuda:0", dtype=torch.int32)
+    pos, didx = torch.empty((T, k), device="cuda:0", dtype=torch.int32), torch.from_numpy(idx).cuda()
+    pd = a.moe_dispatch.primitive_desc(gpu[0], c.bind(a.ARG_SRC, x), c.bind(a.ARG_SRC_1, didx), c.grouped(a.ARG_DST, rows, offsets),
+                                       c.bind(a.ARG_DST_1, pos), attr=attr)
+    prim, md, untouched = a.moe_dispatch(pd), pd.query_md(136), lambda: True
+    assert (md.get_ndims() > 0) == (mode == "user")
+    if mode == "user":
+        with pytest.raises(a.error) as e:
+            prim.execute(c.strm, c.args)
+        assert e.value.status == a.invalid_arguments
+        scratch, untouched = guarded((md.get_size(),), torch.uint8, 255)
+        c.args[a.ARG_SCRATCHPAD] = a.memory(md, gpu[0], scratch.data_ptr())
+    for n in range(3):
+        if n:
+            idx = base.choices(r, T, E, k, 0.3)
+            didx.copy_(torch.from_numpy(idx))
+            if mode == "user":
+                scratch.fill_(255 if n == 1 else 1)
+        torch.cuda.synchronize()
+        prim.execute(c.strm, c.args)
+        c.strm.wait()
+        ends, want_pos, order = R.sort_slots(idx, E)
+        assert np.array_equal(host(offsets), ends) and np.array_equal(host(pos), want_pos)
+        assert np.array_equal(host(rows)[:order.size], host(x)[order // k]) and untouched()
+    if mode == "user":
+        assert not (scratch == 1).all()
+
+
 # ----------------------------------------------------------------------------------------------- dropout
 
 
