@@ -301,3 +301,90 @@ def test_dropout_of_tensors_that_outnumber_the_grid(gpu, M, N, p, res, pitch, dt
     if res:
         want, size = want + host(residual), size + np.abs(host(residual))
     base.check(got, want, size * 3 * EPS + out_slack(want, dtype))
+
+
+# ------------------------------------------------------------------------------------- how they are called
+
+
+def test_one_dispatch_of_open_dims_for_batches_on_both_sides_of_its_forms(gpu):
+    """few slots, slots that every CTA counts, and slots counted through the scratchpad, in turn"""
+    import torch
+    from onednn_b200 import api as a
+    eng, E, k, H, O = gpu[0], 30, 4, 24, a.RUNTIME_DIM_VAL
+    md, prim = a.memory.desc, None
+    for T in (5000, 17, 9000, 1500, 2100, 0, 30001):
+        r = rng(T)
+        x, idx = device_matrix(r.integers(-100, 100, (T, H)).astype(np.float64), "f32"), base.choices(r, T, E, k, 0.1)
+        c = base.Call(eng)
+        rows, offsets = torch.full((T * k, H), 7.0, device="cuda:0"), torch.full((E,), 7, device="cuda:0", dtype=torch.int32)
+        pos = torch.full((T, k), 7, device="cuda:0", dtype=torch.int32)
+        mds = [c.bind(a.ARG_SRC, x, (0,)), c.bind(a.ARG_SRC_1, torch.from_numpy(idx).cuda(), (0,)),
+               c.grouped(a.ARG_DST, rows, offsets, open_rows=True), c.bind(a.ARG_DST_1, pos, (0,))]
+        if prim is None:
+            prim = a.moe_dispatch(a.moe_dispatch.primitive_desc(eng, *mds))
+        prim.execute(c.strm, c.args)
+        c.strm.wait()
+        ends, want_pos, order = R.sort_slots(idx, E)
+        assert np.array_equal(host(offsets), ends) and np.array_equal(host(pos), want_pos)
+        assert np.array_equal(host(rows)[:order.size], host(x)[order // k]) and not host(rows)[order.size:].any()
+
+
+def test_gradients_and_dropout_of_open_dims(gpu):
+    """one primitive of each for batches of any size; memory that contradicts the rest is refused"""
+    import torch
+    from onednn_b200 import api as a
+    eng, E, k, H, p, seed = gpu[0], 12, 3, 40, 0.3, (77, 5)
+    prims = {}
+    dseed = torch.tensor(seed, dtype=torch.int64, device="cuda:0")
+    for T in (50, 1, 1200, 0, 7):
+        r = rng(T, 9)
+        # the router's gradient
+        logits, g = device_matrix(r.standard_normal((T, E)), "f32"), r.standard_normal((T, k)).astype(np.float32)
+        idx, d = R.choose(host(logits), k), torch.full((T, E), 7.0, device="cuda:0")
+        c = base.Call(eng)
+        mds = [c.bind(arg, t, (0,)) for arg, t in ((a.ARG_SRC, logits), (a.ARG_SRC_1, torch.from_numpy(idx).cuda()),
+                                                  (a.ARG_DIFF_DST, torch.from_numpy(g).cuda()), (a.ARG_DIFF_SRC, d))]
+        if "route" not in prims:
+            prims["route"] = a.moe_route_backward(a.moe_route_backward.primitive_desc(eng, *mds))
+        prims["route"].execute(c.strm, c.args)
+        c.strm.wait()
+        want, size = R.route_backward(host(logits), idx, g.astype(np.float64), "softmax", True, 1.0)
+        spread = np.ptp(host(logits)) if T else 0
+        base.check(host(d), want, size * EPS * (4 * (2 + spread) + 64 + k) + out_slack(want, "f32") + 2.0 ** -140)
+        # combine's
+        rows, offsets, dpos, pos = base.make_rows(r, T, E, k, H, "bf16", 0.1)
+        w, dy = r.standard_normal((T, k)).astype(np.float32), device_matrix(r.standard_normal((T, H)), "bf16")
+        drows, dw = torch.full_like(rows, 7.0), torch.full((T, k), 7.0, device="cuda:0")
+        c = base.Call(eng)
+        c.bind(a.ARG_ATTR_DROPOUT_SEED, dseed)
+        mds = [c.bind(a.ARG_DIFF_DST, dy, (0, 1)), c.grouped(a.ARG_SRC, rows, offsets, open_rows=True), c.bind(a.ARG_SRC_1, dpos, (0,)),
+               c.bind(a.ARG_WEIGHTS, torch.from_numpy(w).cuda(), (0,)), c.grouped(a.ARG_DIFF_SRC, drows, offsets, open_rows=True),
+               c.bind(a.ARG_DIFF_WEIGHTS, dw, (0, 1))]
+        if "combine" not in prims:
+            prims["combine"] = a.moe_combine_backward(a.moe_combine_backward.primitive_desc(eng, *mds, dropout_p=p))
+        prims["combine"].execute(c.strm, c.args)
+        c.strm.wait()
+        gy, x, named = R.dropout(host(dy), p, *seed), host(rows), pos >= 0
+        want, want_dw, size = np.zeros_like(x), np.zeros((T, k)), np.zeros((T, k))
+        slots, where = np.argwhere(named), pos[named]
+        want[where] = w[named].astype(np.float64)[:, None] * gy[slots[:, 0]]
+        want_dw[named], size[named] = (gy[slots[:, 0]] * x[where]).sum(1), np.abs(gy[slots[:, 0]] * x[where]).sum(1)
+        base.check(host(drows), want, np.abs(want) * 3 * EPS + out_slack(want, "bf16"))
+        base.check(host(dw), want_dw, size * EPS * (H + 16) + 2.0 ** -140)
+        # dropout, with an open width too
+        x = device_matrix(r.standard_normal((T, 33 + T % 5)), "f16")
+        y = torch.full_like(x, 7.0)
+        c = base.Call(eng)
+        c.bind(a.ARG_ATTR_DROPOUT_SEED, dseed)
+        mds = [c.bind(a.ARG_SRC, x, (0, 1)), c.bind(a.ARG_DST, y, (0, 1)), c.bind(a.ARG_SRC_2, x, (0, 1))]
+        if "dropout" not in prims:
+            prims["dropout"] = a.dropout(a.dropout.primitive_desc(eng, mds[0], mds[1], p, residual_md=mds[2]))
+        prims["dropout"].execute(c.strm, c.args)
+        c.strm.wait()
+        kept = R.dropout(host(x), p, *seed)
+        base.check(host(y), kept + host(x), (np.abs(kept) + np.abs(host(x))) * 3 * EPS + out_slack(kept + host(x), "f16"))
+        if T == 50:
+            c.bind(a.ARG_DST, y[:49])
+            with pytest.raises(a.error) as e:
+                prims["dropout"].execute(c.strm, c.args)
+            assert e.value.status == a.invalid_arguments
