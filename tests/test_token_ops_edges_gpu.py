@@ -1,5 +1,7 @@
 """The operators around an expert layer's products, and dropout: contents, sizes and uses at their edges, against plain 64-bit
 forms.  Every input is made from fixed numbers.  Tolerances as in test_token_ops_gpu.py."""
+import zlib
+
 import numpy as np
 import pytest
 
@@ -388,3 +390,29 @@ def test_gradients_and_dropout_of_open_dims(gpu):
             with pytest.raises(a.error) as e:
                 prims["dropout"].execute(c.strm, c.args)
             assert e.value.status == a.invalid_arguments
+
+
+# ------------------------------------------------------------- tests of test_token_ops_gpu.py with inputs that stay
+
+
+@pytest.fixture
+def fixed(monkeypatch):
+    """(the module draws its inputs from hash() of a string, which every process salts anew)"""
+    monkeypatch.setattr(base, "rng", lambda *key: rng(*(zlib.crc32(k.encode()) if isinstance(k, str) else k for k in key)))
+
+
+@pytest.mark.parametrize("scoring,normalize", base.MODES)
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T,E,k", base.SHAPES)
+def test_route_with_fixed_inputs(gpu, fixed, T, E, k, dtype, scoring, normalize):
+    base.test_route(gpu, T, E, k, dtype, scoring, normalize)
+    base.test_route_backward(gpu, T, E, k, dtype, scoring, normalize)
+
+
+DROPOUTS = next(m.args[1] for m in base.test_dropout.pytestmark if m.args[0].startswith("M,N"))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,N,p,res,pitch,out_pitch,offset", DROPOUTS)
+def test_dropout_with_fixed_inputs(gpu, fixed, M, N, p, res, pitch, out_pitch, offset, dtype):
+    base.test_dropout(gpu, M, N, p, res, pitch, out_pitch, offset, dtype)
