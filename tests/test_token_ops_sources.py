@@ -104,3 +104,10 @@ def test_an_empty_matrix_may_have_any_strides(host_engine):
     with pytest.raises(api.error) as e:  # but a known pitch of outputs with rows still counts
         api.dropout.primitive_desc(host_engine, md((5, 4), 3, (4, 1)), md((5, 4), 3, (0, 1)), 0.5)
     assert e.value.status == api.unimplemented
+
+
+@pytest.mark.parametrize("file", ["sm100_ptx.cuh", "token_rows.cuh", "moe_route.cu", "moe_dispatch.cu", "moe_combine.cu", "dropout.cu"])
+def test_every_function_is_called(file):
+    sources = os.path.join(ROOT, "onednn_b200", "csrc")
+    text = "".join(_source(f) for f in os.listdir(sources) if f.endswith((".cu", ".cuh", ".h", ".hpp")))
+    assert not [n for n in _functions(_source(file)) if len(re.findall(r"\b%s\b" % n, text)) < 2]
