@@ -24,7 +24,13 @@ constexpr int THREADS = 1024, WARPS = THREADS / 32;
 constexpr int TILE = 1024; // slots ranked at a time
 // Up to here every CTA that sorts counts all slots itself, which saves a launch (4096 slots 13.3 -> 11.4 us; 16384 32.6 -> 34.5).
 constexpr int SELF_SLOTS = 8192;
-constexpr int FEW_SLOTS = 256; // up to here one launch does everything
+// Up to here one launch does everything.  Ranking every slot against all takes as long as there are slots, and one thread after
+// the other copies with a unit in flight, so it ends where the other form's two launches are as fast.  us on the device, one
+// launch / two, bf16: 1 x 8 x 4096 2.5 / 5.2, 37 x 2 3.2 / 6.1, 16 x 8 4.3 / 5.5, 24 x 8 5.3 / 5.6, 32 x 8 6.3 / 5.6, 256 x 1 7.1 /
+// 5.9; 128 x 1 x 8192 (131072 units) 5.2 / 5.8, x 16384 6.4 / 5.9; rows that start anywhere, units of an element: 64 x 2 x 2047
+// 5.3 / 5.6, 128 x 2047 6.4 / 5.2.
+constexpr int FEW_SLOTS = 192, FEW_UNITS = 1 << 17;
+constexpr int FEW_THREADS = 256;
 
 struct Plan {
     DispatchArgs a;
@@ -252,14 +258,14 @@ template <typename E> __global__ void __launch_bounds__(256) dispatch_shift_kern
 }
 
 // Few slots: every CTA ranks all of them, each slot against all, and moves its share of the rows.
-template <typename U, typename E> __global__ void __launch_bounds__(FEW_SLOTS) dispatch_few_kernel(const __grid_constant__ DispatchArgs a) {
-    __shared__ __align__(16) int expert[FEW_SLOTS];
-    __shared__ int place[FEW_SLOTS];
+template <typename U, typename E> __global__ void __launch_bounds__(FEW_THREADS) dispatch_few_kernel(const __grid_constant__ DispatchArgs a) {
+    __shared__ __align__(16) int expert[FEW_THREADS];
+    __shared__ int place[FEW_THREADS];
     __shared__ int kept;
     ptx::grid_dependency_wait();
     const int n = a.tokens * a.choices, s = threadIdx.x;
-    const int64_t units = a.row_bytes / sizeof(U), work = a.tokens * units, stride = (int64_t)gridDim.x * FEW_SLOTS;
-    int64_t i = (int64_t)blockIdx.x * FEW_SLOTS + s;
+    const int64_t units = a.row_bytes / sizeof(U), work = a.tokens * units, stride = (int64_t)gridDim.x * FEW_THREADS;
+    int64_t i = (int64_t)blockIdx.x * FEW_THREADS + s;
     const int mine = s < n ? slot_expert(a, s) : -1;
     U v;
     if (i < work) v = *((const U *)(a.src + i / units * a.src_pitch) + i % units); // on its way while the slots are ranked
@@ -277,7 +283,7 @@ template <typename U, typename E> __global__ void __launch_bounds__(FEW_SLOTS) d
     if (s == 0) kept = there;
     if (blockIdx.x == 0) {
         if (s < n) a.positions[(int64_t)(s / a.choices) * a.positions_ld + s % a.choices] = place[s];
-        for (int e = s; e < a.experts; e += FEW_SLOTS) {
+        for (int e = s; e < a.experts; e += FEW_THREADS) {
             int ends = 0;
             for (int q = 0; q < n; q += 4) {
                 const int4 x = *reinterpret_cast<const int4 *>(expert + q);
@@ -307,8 +313,9 @@ int launched(int rc) {
 
 template <typename E> int launch_copy(const DispatchArgs &a, bool aligned, cudaStream_t st) {
     if (aligned) {
-        // with few places a row, more of it a thread, so that as many bytes are on their way
-        const int units = a.choices <= 2 ? 4 : 1;
+        // with one place a row, more of it a thread, so that as many bytes are on their way (8192 x 4096 bf16: one choice 31.4 us
+        // with one unit / 29.1 with four, two 39.2 / 39.2, four 60.6 / 61.4)
+        const int units = a.choices == 1 ? 4 : 1;
         const int64_t grid = (a.tokens * (a.row_bytes / 16) + 256 * units - 1) / (256 * units);
         return grid > INT_MAX ? 3 : launched(launch_dependent(units == 4 ? dispatch_copy_kernel<4> : dispatch_copy_kernel<1>, a, (unsigned)grid, 256, 0, st));
     }
@@ -319,7 +326,7 @@ template <typename E> int launch_copy(const DispatchArgs &a, bool aligned, cudaS
 template <typename U, typename E> int launch_few(const DispatchArgs &a, int sm_count, cudaStream_t st) {
     const int64_t work = a.tokens * (a.row_bytes / (int64_t)sizeof(U));
     const unsigned grid = (unsigned)std::min<int64_t>(sm_count, std::max<int64_t>(1, (work + 127) / 128));
-    return launched(launch_dependent(dispatch_few_kernel<U, E>, a, grid, FEW_SLOTS, 0, st));
+    return launched(launch_dependent(dispatch_few_kernel<U, E>, a, grid, FEW_THREADS, 0, st));
 }
 
 } // namespace
@@ -335,7 +342,7 @@ int launch_dispatch(const DispatchArgs &a, int *scratch, int sm_count, cudaStrea
     const bool aligned = places % 16 == 0;
     if (!aligned && a.row_bytes > INT_MAX / 2) return 3;
     const int64_t slots = (int64_t)a.tokens * a.choices;
-    if (slots <= FEW_SLOTS)
+    if (slots <= FEW_SLOTS && a.tokens * (a.row_bytes / (aligned ? 16 : a.element)) <= FEW_UNITS)
         return aligned           ? launch_few<uint4, uint32_t>(a, sm_count, st)
                 : a.element == 4 ? launch_few<uint32_t, uint32_t>(a, sm_count, st)
                 : a.element == 2 ? launch_few<uint16_t, uint16_t>(a, sm_count, st)

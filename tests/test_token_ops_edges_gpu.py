@@ -231,7 +231,8 @@ def test_one_dispatch_on_two_streams_with_scratchpads_of_their_own(gpu, H):
         assert all(ok() for ok in checks) and not (scratch == 255).all()
 
 
-@pytest.mark.parametrize("T,E,k,H,dtype,pitch", [(128, 8, 2, 4096, "bf16", 0), (100, 5, 2, 1001, "f16", 1004), (60, 7, 4, 5003, "s8", 0)])
+@pytest.mark.parametrize("T,E,k,H,dtype,pitch", [(128, 8, 2, 4096, "bf16", 0), (100, 5, 2, 1001, "f16", 1004), (60, 7, 4, 5003, "s8", 0),
+                                                     (96, 8, 2, 8192, "bf16", 0), (60, 5, 2, 2001, "f16", 2004), (24, 9, 8, 5003, "s8", 0)])
 def test_few_slots_of_wide_rows(gpu, T, E, k, H, dtype, pitch):
     """the form of one launch, rows wide enough that its grid goes round"""
     r = rng(T, H)
