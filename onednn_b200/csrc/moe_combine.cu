@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(BULK_THREADS, 1) combine_bulk_kernel(const __g
                             for (int n = 0; n < 8; n += 2) fma2(acc[h][n], acc[h][n + 1], wj, v[n], v[n + 1]);
                         }
                 };
-                const uint32_t every = a.choices == 32 ? 0xffffffffu : (1u << a.choices) - 1;
+                const uint32_t every = (1u << a.choices) - 1;
                 if ((there & every) == every) {
                     int j = 0;
                     for (; j + 4 <= a.choices; j += 4) {
@@ -500,12 +500,22 @@ template <typename S, typename D, bool DROP> int launch_bulk(const CombineArgs &
 template <typename S, typename D, bool DROP> int launch_forward(const CombineArgs &a, bool vec, int sm_count, cudaStream_t st) {
     const int64_t total = a.tokens * (vec ? row_units<true>(a.cols, DROP) : row_units<false>(a.cols, DROP));
     const int64_t grid = (total + 255) / 256;
-    // Below 2 KB a row or 2^21 sums the ring's start and the copies' number cost more than they give.  us a call, thread by
-    // thread / bulk, bf16, k = 8: 600 x 4096 7.9 / 7.5, 400 x 4096 5.8 / 6.0, 4096 x 512 7.4 / 9.0; k = 1: 4096 x 1024 8.3 / 6.7.
-    if (vec && a.cols * (int64_t)sizeof(S) >= 2048 && a.tokens * a.cols >= (1 << 21)
+    // The ring's start and the number of its copies cost more than they give where a row is below 2 KB, where there are few
+    // sums, with one or two rows a token (few bytes of a copy's wait are shared) and, with many, where a stage leaves the ring few
+    // others.  us a call, thread by thread / ring, inputs not in L2: bf16, 8 rows: 512 x 4096 11.5 / 11.1, 8192 x 4096 124 / 102,
+    // 1024 x 1024 7.6 / 7.8, 4096 x 512 7.4 / 9.0; 4 rows: 8192 x 4096 99 / 68; 1 row: 4096 x 1024 7.9 / 8.2, 8192 x 1024 13.0 /
+    // 12.1, 4096 x 4096 23.2 / 18.8; 2 rows: 8192 x 1024 14.5 / 15.7, x 4096 49.2 / 49.2; 12 rows: 2730 x 4096 61.8 / 52.8; 16: 4096 x 2048 54.2 / 61.4; 24:
+    // 1365 x 4096 51.6 / 57.0; 32: 1024 x 4096 49.8 / 68.0.  f32: 8 rows: 8192 x 2048 101.5 / 103, 512 x 2048 9.9 / 10.8, with
+    // dropout 106.6 / 106.5; 4 rows: 4096 x 512 12.4 / 11.8; 8192 x 4096 147 / 125; 12 rows: 2730 x 4096 97.9 / 97.8; 16: 2048 x 4096
+    // 90.3 / 93.4; 1 row: 8192 x 1024 19.4 / 19.7, x 4096 69.6 / 68.0; 2 rows: 42.0 / 45.0 for 8192 x 2048.
+    const int64_t sums = a.tokens * a.cols;
+    const bool many = a.choices >= 3 && a.choices <= 12 ? sums >= 1 << 21 : a.choices == 1 && sums >= 1 << 23;
+    if (vec && a.cols * (int64_t)sizeof(S) >= 2048 && many
             && a.tokens * ((a.cols + WARP_COLS - 1) / WARP_COLS) < (1 << 30) && !a.drop.drop_all)
         return launch_bulk<S, D, DROP>(a, sm_count, st);
     if (grid > 0x7fffffff) return 3;
+    // (3000 x 2 x 2047 bf16 with groups of eight rows 23.5 us / of two 14.4; four rows in groups of eight / of four: 400 x 4096 bf16
+    // with dropout 6.8 / 6.2, 3000 x 2047 bf16 25.5 / 25.8, f32 33.1 / 30.0: not worth their kernels)
     void (*kernel)(CombineArgs) = a.choices <= 2 ? (vec ? combine_kernel<S, D, true, DROP, 2> : combine_kernel<S, D, false, DROP, 2>)
                                                  : (vec ? combine_kernel<S, D, true, DROP, 8> : combine_kernel<S, D, false, DROP, 8>);
     return launch_dependent(kernel, a, (unsigned)grid, 256, 0, st);

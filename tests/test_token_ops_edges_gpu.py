@@ -177,6 +177,17 @@ def test_no_slot_names_a_row(gpu):
     check_both_ways(gpu[0], r, rows, offsets, pos, 0.0)
 
 
+# (the ring of bulk copies at its limits: one row a token, as few and as many as it takes, several tokens an item, ragged ones)
+RING = [(4100, 8, 1, 4104, "bf16", "bf16", 0.2), (2049, 8, 1, 8200, "f32", "f16", 0.0), (2100, 16, 3, 1000, "f32", "f32", 0.3),
+        (2051, 16, 12, 1032, "bf16", "f32", 0.1), (701, 16, 12, 3080, "f32", "f32", 0.0), (2063, 16, 7, 1040, "f16", "f16", 0.0),
+        (1500, 40, 13, 1544, "bf16", "bf16", 0.1), (1400, 40, 32, 1544, "f32", "bf16", 0.0), (4099, 8, 2, 2056, "bf16", "bf16", 0.3)]
+
+
+@pytest.mark.parametrize("T,E,k,H,dtype,out,p", RING)
+def test_combine_on_both_sides_of_the_ring(gpu, T, E, k, H, dtype, out, p):
+    base.test_combine(gpu, T, E, k, H, dtype, out, True, k % 2 == 1, p, 0, 0.05)
+
+
 # ---------------------------------------------------------------------------------------------- dispatch
 
 
