@@ -384,12 +384,17 @@ template <typename S, bool VEC> __device__ __forceinline__ void zero_unnamed(con
     }
 }
 
-// CTAs per SM that the gradient's registers are cut to (0: the compiler's choice).  4096 tokens, the same inputs every call: bf16,
-// eight rows of 4096 89 us three / 101 four (with positions and weights in every thread's registers 100 uncut / 103 two / 95
-// three), four rows of 4096 with dropout 51.5 uncut / 47.7 five, without 52.0 / 50.3; f32 220 uncut / 170 two / 238 three; rows
-// that start anywhere 102 two / 154 three, two rows of 2047 bf16 without dropout 21.9 four / 20.7 five.
+// CTAs per SM that the gradient's registers are cut to (0: the compiler's choice).  us a call, 4096 tokens, the same inputs every
+// call, uncut / cut: bf16 with dropout, eight rows of 4096 106.4 / 88.5 (three; 97.9 four), four rows of 4096 51.5 / 47.7 (five); rows that start anywhere, two of 2047 without dropout 21.9 / 20.7 (five); f32, eight rows of 512 with dropout 27.0 /
+// 25.4 (two), of 255 without 12.9 / 11.4.  Elsewhere a cut gains nothing or costs: rows that start anywhere, with dropout, bf16,
+// eight of 2047 81.2 / 82.4 (three), 101.6 (two), four of 2047 48.7 / 71.3 (two); f32, two of 4096 with dropout 53.0 / 67.5 (two).
 template <typename S, typename D, bool VEC, bool DROP, int GROUP, int THREADS>
-constexpr int GRADIENT_CTAS = !VEC && !DROP && GROUP == 2 ? 5 : !VEC || sizeof(S) == 4 ? 2 : THREADS == 32 || GROUP == 2 ? 0 : GROUP == 8 ? 3 : sizeof(D) == 2 ? 5 : 0;
+constexpr int GRADIENT_CTAS = !VEC && !DROP && GROUP == 2 ? 5
+        : sizeof(S) == 4 && GROUP == 8 && THREADS == 32   ? 2
+        : !VEC || sizeof(S) == 4 || THREADS == 32         ? 0
+        : GROUP == 8                                      ? 3
+        : GROUP == 4 && sizeof(D) == 2                    ? 5
+                                                          : 0;
 
 // THREADS of the 256 of a CTA work on a token: all of them, or a warp where rows are short.
 template <typename S, typename D, bool VEC, bool DROP, int THREADS, int GROUP>
