@@ -21,8 +21,8 @@ __device__ __forceinline__ uint32_t rows_of_groups(const CombineArgs &a) {
 }
 
 // GROUP rows of a token are in flight at a time: their loads leave before the first is used.  As many as a token has, up to
-// eight: what eight take in registers costs a token of fewer rows its warps (gradient, 4096 x 4096, two rows 55 us with
-// eight / 34 with two, four rows 72 / 56).
+// eight: what eight take in registers costs a token of fewer rows its warps (when the gradient was given its groups, 4096 x 4096
+// bf16: two rows 55 us in groups of eight / 34 of two, four rows 72 in groups of eight / 56 of four).
 
 template <typename S, typename D, bool VEC, bool DROP, int GROUP>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineArgs a) {
@@ -385,9 +385,10 @@ template <typename S, bool VEC> __device__ __forceinline__ void zero_unnamed(con
 }
 
 // CTAs per SM that the gradient's registers are cut to (0: the compiler's choice).  us a call, 4096 tokens, the same inputs every
-// call, uncut / cut: bf16 with dropout, eight rows of 4096 106.4 / 88.5 (three; 97.9 four), four rows of 4096 51.5 / 47.7 (five); rows that start anywhere, two of 2047 without dropout 21.9 / 20.7 (five); f32, eight rows of 512 with dropout 27.0 /
-// 25.4 (two), of 255 without 12.9 / 11.4.  Elsewhere a cut gains nothing or costs: rows that start anywhere, with dropout, bf16,
-// eight of 2047 81.2 / 82.4 (three), 101.6 (two), four of 2047 48.7 / 71.3 (two); f32, two of 4096 with dropout 53.0 / 67.5 (two).
+// call, uncut / cut: bf16 with dropout, eight rows of 4096 106.4 / 88.5 (three; 97.9 four), four rows of 4096 51.5 / 47.7 (five);
+// rows that start anywhere, bf16, two of 2047 without dropout 21.9 / 20.7 (five); f32, eight rows of 512 with dropout 27.0 / 25.4
+// (two), of 255 without 12.9 / 11.4.  Elsewhere a cut gains nothing or costs: rows that start anywhere, bf16 with dropout, eight of
+// 2047 81.2 / 82.4 (three), 101.6 (two), four of 2047 48.7 / 71.3 (two); f32, two of 4096 with dropout 53.0 / 67.5 (two).
 template <typename S, typename D, bool VEC, bool DROP, int GROUP, int THREADS>
 constexpr int GRADIENT_CTAS = !VEC && !DROP && GROUP == 2 ? 5
         : sizeof(S) == 4 && GROUP == 8 && THREADS == 32   ? 2
@@ -506,13 +507,19 @@ template <typename S, typename D, bool DROP> int launch_forward(const CombineArg
     const int64_t total = a.tokens * (vec ? row_units<true>(a.cols, DROP) : row_units<false>(a.cols, DROP));
     const int64_t grid = (total + 255) / 256;
     // The ring's start and the number of its copies cost more than they give where a row is below 2 KB, where there are few
-    // sums, with one or two rows a token (few bytes of a copy's wait are shared) and, with many, where a stage leaves the ring few
-    // others.  us a call, thread by thread / ring, inputs not in L2: bf16, 8 rows: 512 x 4096 11.5 / 11.1, 8192 x 4096 124 / 102,
-    // 1024 x 1024 7.6 / 7.8, 4096 x 512 7.4 / 9.0; 4 rows: 8192 x 4096 99 / 68; 1 row: 4096 x 1024 7.9 / 8.2, 8192 x 1024 13.0 /
-    // 12.1, 4096 x 4096 23.2 / 18.8; 2 rows: 8192 x 1024 14.5 / 15.7, x 4096 49.2 / 49.2; 12 rows: 2730 x 4096 61.8 / 52.8; 16: 4096 x 2048 54.2 / 61.4; 24:
-    // 1365 x 4096 51.6 / 57.0; 32: 1024 x 4096 49.8 / 68.0.  f32: 8 rows: 8192 x 2048 101.5 / 103, 512 x 2048 9.9 / 10.8, with
-    // dropout 106.6 / 106.5; 4 rows: 4096 x 512 12.4 / 11.8; 8192 x 4096 147 / 125; 12 rows: 2730 x 4096 97.9 / 97.8; 16: 2048 x 4096
-    // 90.3 / 93.4; 1 row: 8192 x 1024 19.4 / 19.7, x 4096 69.6 / 68.0; 2 rows: 42.0 / 45.0 for 8192 x 2048.
+    // sums, with one or two rows a token and, with many rows, where a stage leaves the ring few others.
+    // us a call, residual, no dropout, thread by thread / ring (up to eight rows: inputs that are not in L2)
+    //   rows     bf16                                                       f32
+    //    1       4096 x 1024 7.9 / 8.2, 8192 x 1024 13.0 / 12.1,            8192 x 1024 19.4 / 19.7, 8192 x 4096 69.6 / 68.0
+    //            4096 x 4096 23.2 / 18.8
+    //    2       8192 x 1024 14.5 / 15.7, 8192 x 4096 49.2 / 49.2           8192 x 2048 42.0 / 45.0
+    //    4       1024 x 1024 6.3 / 6.0, 8192 x 4096 99.3 / 68.0             1024 x 1024 7.3 / 8.8, 4096 x 512 12.4 / 11.8,
+    //                                                                       8192 x 4096 147 / 125
+    //    8       1024 x 1024 7.6 / 7.8, 512 x 4096 11.5 / 11.1,             2048 x 512 10.0 / 10.8, 8192 x 2048 101.5 / 103.1
+    //            8192 x 4096 124.5 / 101.9, 4096 x 512 7.4 / 9.0            (with dropout 106.6 / 106.5)
+    //   12       2730 x 4096 61.8 / 52.8                                    2730 x 4096 97.9 / 97.8
+    //   16       4096 x 2048 54.2 / 61.4, 2048 x 4096 54.0 / 52.7           2048 x 4096 90.3 / 93.4
+    //   32       1024 x 4096 49.8 / 68.0                                    1024 x 4096 84.7 / 100.7
     const int64_t sums = a.tokens * a.cols;
     const bool many = a.choices >= 3 && a.choices <= 12 ? sums >= 1 << 21 : a.choices == 1 && sums >= 1 << 23;
     if (vec && a.cols * (int64_t)sizeof(S) >= 2048 && many
