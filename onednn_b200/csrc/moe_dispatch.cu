@@ -24,13 +24,16 @@ constexpr int THREADS = 1024, WARPS = THREADS / 32;
 constexpr int TILE = 1024; // slots ranked at a time
 // Up to here every CTA that sorts counts all slots itself, which saves a launch (4096 slots 13.3 -> 11.4 us; 16384 32.6 -> 34.5).
 constexpr int SELF_SLOTS = 8192;
-// Up to here one launch does everything.  Ranking every slot against all takes as long as there are slots, and one thread after
-// the other copies with a unit in flight, so it ends where the other form's two launches are as fast.  us on the device, one
-// launch / two, bf16: 1 x 8 x 4096 2.5 / 5.2, 37 x 2 3.2 / 6.1, 16 x 8 4.3 / 5.5, 24 x 8 5.3 / 5.6, 32 x 8 6.3 / 5.6, 256 x 1 7.1 /
-// 5.9; 128 x 1 x 8192 (131072 units) 5.2 / 5.8, x 16384 6.4 / 5.9; rows that start anywhere, units of an element: 64 x 2 x 2047
-// 5.3 / 5.6, 128 x 2047 6.4 / 5.2.
-constexpr int FEW_SLOTS = 192, FEW_UNITS = 1 << 17;
-constexpr int FEW_THREADS = 256;
+// Up to here one launch does everything.  It takes about 2 us, 0.0155 for every slot (each is ranked against all) and 0.001 for
+// every 100 units of the tokens' rows (a thread copies one after the other); the other form's two launches 5.6, or for rows that
+// start anywhere 5 and 0.3 for every choice.  us on the device, one launch / two, bf16: 1 x 8 x 4096 2.5 / 5.2, 37 x 2 3.2 / 6.1,
+// 16 x 8 4.3 / 5.5, 24 x 8 5.3 / 5.6, 32 x 8 6.3 / 5.6, 256 x 1 7.1 / 5.9; 128 x 1 x 8192 (units of 16 bytes) 5.2 / 5.8, x 16384 6.4 /
+// 5.9; rows that start anywhere (units of an element): 64 x 2 x 2047 5.3 / 5.6, 32 x 8 6.1 / 8.1 for 1001 and 7.6 / 7.8 for 4097,
+// 128 x 2 x 1001 7.3 / 5.9, 128 x 1 x 2047 6.4 / 5.2.
+constexpr int FEW_SLOTS = 256;
+inline bool few(int64_t slots, int64_t units, int choices, bool aligned) {
+    return slots <= FEW_SLOTS && slots + units / 1500 <= (aligned ? 240 : 200 + 20 * choices);
+}
 
 struct Plan {
     DispatchArgs a;
@@ -257,15 +260,15 @@ template <typename E> __global__ void __launch_bounds__(256) dispatch_shift_kern
     zero_behind<E>(a, ptx::ld_dependent(a.offsets + a.experts - 1));
 }
 
-// Few slots: every CTA ranks all of them, each slot against all, and moves its share of the rows.
-template <typename U, typename E> __global__ void __launch_bounds__(FEW_THREADS) dispatch_few_kernel(const __grid_constant__ DispatchArgs a) {
-    __shared__ __align__(16) int expert[FEW_THREADS];
-    __shared__ int place[FEW_THREADS];
+// Few slots, one a thread: every CTA ranks all of them, each slot against all, and moves its share of the rows.
+template <typename U, typename E> __global__ void __launch_bounds__(FEW_SLOTS) dispatch_few_kernel(const __grid_constant__ DispatchArgs a) {
+    __shared__ __align__(16) int expert[FEW_SLOTS];
+    __shared__ int place[FEW_SLOTS];
     __shared__ int kept;
     ptx::grid_dependency_wait();
     const int n = a.tokens * a.choices, s = threadIdx.x;
-    const int64_t units = a.row_bytes / sizeof(U), work = a.tokens * units, stride = (int64_t)gridDim.x * FEW_THREADS;
-    int64_t i = (int64_t)blockIdx.x * FEW_THREADS + s;
+    const int64_t units = a.row_bytes / sizeof(U), work = a.tokens * units, stride = (int64_t)gridDim.x * FEW_SLOTS;
+    int64_t i = (int64_t)blockIdx.x * FEW_SLOTS + s;
     const int mine = s < n ? slot_expert(a, s) : -1;
     U v;
     if (i < work) v = *((const U *)(a.src + i / units * a.src_pitch) + i % units); // on its way while the slots are ranked
@@ -283,7 +286,7 @@ template <typename U, typename E> __global__ void __launch_bounds__(FEW_THREADS)
     if (s == 0) kept = there;
     if (blockIdx.x == 0) {
         if (s < n) a.positions[(int64_t)(s / a.choices) * a.positions_ld + s % a.choices] = place[s];
-        for (int e = s; e < a.experts; e += FEW_THREADS) {
+        for (int e = s; e < a.experts; e += FEW_SLOTS) {
             int ends = 0;
             for (int q = 0; q < n; q += 4) {
                 const int4 x = *reinterpret_cast<const int4 *>(expert + q);
@@ -326,7 +329,7 @@ template <typename E> int launch_copy(const DispatchArgs &a, bool aligned, cudaS
 template <typename U, typename E> int launch_few(const DispatchArgs &a, int sm_count, cudaStream_t st) {
     const int64_t work = a.tokens * (a.row_bytes / (int64_t)sizeof(U));
     const unsigned grid = (unsigned)std::min<int64_t>(sm_count, std::max<int64_t>(1, (work + 127) / 128));
-    return launched(launch_dependent(dispatch_few_kernel<U, E>, a, grid, FEW_THREADS, 0, st));
+    return launched(launch_dependent(dispatch_few_kernel<U, E>, a, grid, FEW_SLOTS, 0, st));
 }
 
 } // namespace
@@ -342,7 +345,7 @@ int launch_dispatch(const DispatchArgs &a, int *scratch, int sm_count, cudaStrea
     const bool aligned = places % 16 == 0;
     if (!aligned && a.row_bytes > INT_MAX / 2) return 3;
     const int64_t slots = (int64_t)a.tokens * a.choices;
-    if (slots <= FEW_SLOTS && a.tokens * (a.row_bytes / (aligned ? 16 : a.element)) <= FEW_UNITS)
+    if (few(slots, a.tokens * (a.row_bytes / (aligned ? 16 : a.element)), a.choices, aligned))
         return aligned           ? launch_few<uint4, uint32_t>(a, sm_count, st)
                 : a.element == 4 ? launch_few<uint32_t, uint32_t>(a, sm_count, st)
                 : a.element == 2 ? launch_few<uint16_t, uint16_t>(a, sm_count, st)
