@@ -507,12 +507,14 @@ template <typename S, typename D, bool DROP> int launch_forward(const CombineArg
     const int64_t total = a.tokens * (vec ? row_units<true>(a.cols, DROP) : row_units<false>(a.cols, DROP));
     const int64_t grid = (total + 255) / 256;
     // The ring's start and the number of its copies cost more than they give where a row is below 2 KB, where there are few
-    // sums, with one or two rows a token and, with many rows, where a stage leaves the ring few others.
+    // sums, most of all with one or two rows a token, and, with many rows, where a stage leaves the ring few others.
     // us a call, residual, no dropout, thread by thread / ring (up to eight rows: inputs that are not in L2)
     //   rows     bf16                                                       f32
     //    1       4096 x 1024 7.9 / 8.2, 8192 x 1024 13.0 / 12.1,            8192 x 1024 19.4 / 19.7, 8192 x 4096 69.6 / 68.0
     //            4096 x 4096 23.2 / 18.8
     //    2       8192 x 1024 14.5 / 15.7, 8192 x 4096 49.2 / 49.2           8192 x 2048 42.0 / 45.0
+    //            (with dropout 73.1 / 71.2), 6997 x 7936 without residual
+    //            88.1 / 84.5
     //    4       1024 x 1024 6.3 / 6.0, 8192 x 4096 99.3 / 68.0             1024 x 1024 7.3 / 8.8, 4096 x 512 12.4 / 11.8,
     //                                                                       8192 x 4096 147 / 125
     //    8       1024 x 1024 7.6 / 7.8, 512 x 4096 11.5 / 11.1,             2048 x 512 10.0 / 10.8, 8192 x 2048 101.5 / 103.1
@@ -521,7 +523,7 @@ template <typename S, typename D, bool DROP> int launch_forward(const CombineArg
     //   16       4096 x 2048 54.2 / 61.4, 2048 x 4096 54.0 / 52.7           2048 x 4096 90.3 / 93.4
     //   32       1024 x 4096 49.8 / 68.0                                    1024 x 4096 84.7 / 100.7
     const int64_t sums = a.tokens * a.cols;
-    const bool many = a.choices >= 3 && a.choices <= 12 ? sums >= 1 << 21 : a.choices == 1 && sums >= 1 << 23;
+    const bool many = a.choices == 1 ? sums >= 1 << 23 : a.choices == 2 ? sizeof(S) == 2 && sums >= 1 << 25 : a.choices <= 12 && sums >= 1 << 21;
     if (vec && a.cols * (int64_t)sizeof(S) >= 2048 && many
             && a.tokens * ((a.cols + WARP_COLS - 1) / WARP_COLS) < (1 << 30) && !a.drop.drop_all)
         return launch_bulk<S, D, DROP>(a, sm_count, st);

@@ -180,7 +180,8 @@ def test_no_slot_names_a_row(gpu):
 # (the ring of bulk copies at its limits: one row a token, as few and as many as it takes, several tokens an item, ragged ones)
 RING = [(4100, 8, 1, 4104, "bf16", "bf16", 0.2), (2049, 8, 1, 8200, "f32", "f16", 0.0), (2100, 16, 3, 1000, "f32", "f32", 0.3),
         (2051, 16, 12, 1032, "bf16", "f32", 0.1), (701, 16, 12, 3080, "f32", "f32", 0.0), (2063, 16, 7, 1040, "f16", "f16", 0.0),
-        (1500, 40, 13, 1544, "bf16", "bf16", 0.1), (1400, 40, 32, 1544, "f32", "bf16", 0.0), (4099, 8, 2, 2056, "bf16", "bf16", 0.3)]
+        (1500, 40, 13, 1544, "bf16", "bf16", 0.1), (1400, 40, 32, 1544, "f32", "bf16", 0.0), (4099, 8, 2, 2056, "bf16", "bf16", 0.3),
+        (4100, 8, 2, 8200, "bf16", "bf16", 0.1)]
 
 
 @pytest.mark.parametrize("T,E,k,H,dtype,out,p", RING)
