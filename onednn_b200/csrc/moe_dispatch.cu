@@ -25,14 +25,15 @@ constexpr int TILE = 1024; // slots ranked at a time
 // Up to here every CTA that sorts counts all slots itself, which saves a launch (4096 slots 13.3 -> 11.4 us; 16384 32.6 -> 34.5).
 constexpr int SELF_SLOTS = 8192;
 // Up to here one launch does everything.  It takes about 2 us, 0.0155 for every slot (each is ranked against all) and 0.001 for
-// every 100 units of the tokens' rows (a thread copies one after the other); the other form's two launches 5.6, or for rows that
-// start anywhere 5 and 0.3 for every choice.  us on the device, one launch / two, bf16: 1 x 8 x 4096 2.5 / 5.2, 37 x 2 3.2 / 6.1,
-// 16 x 8 4.3 / 5.5, 24 x 8 5.3 / 5.6, 32 x 8 6.3 / 5.6, 256 x 1 7.1 / 5.9; 128 x 1 x 8192 (units of 16 bytes) 5.2 / 5.8, x 16384 6.4 /
-// 5.9; rows that start anywhere (units of an element): 64 x 2 x 2047 5.3 / 5.6, 32 x 8 6.1 / 8.1 for 1001 and 7.6 / 7.8 for 4097,
-// 128 x 2 x 1001 7.3 / 5.9, 128 x 1 x 2047 6.4 / 5.2.
+// every 100 units of the tokens' rows (a thread copies one after the other).  The other form's two launches take the device 5.6,
+// where rows start anywhere 5 and 0.3 for every choice, and the host, called one by one, 6 to 7: the limit is 6.5, and 6.2 and 0.3 a
+// choice.  us on the device, one launch / two, bf16: 1 x 8 x 4096 2.5 / 5.2, 37 x 2 3.2 / 6.1, 16 x 8 4.3 / 5.5, 24 x 8 5.3 / 5.6,
+// 32 x 8 6.3 / 5.6 (one by one 6.5 / 6.9), 256 x 1 7.1 / 5.9; 128 x 1 x 8192 (units of 16 bytes) 5.2 / 5.8, 256 x 8192 8.3 / 6.1;
+// rows that start anywhere (units of an element): 64 x 2 x 2047 5.3 / 5.6, 32 x 8 6.1 / 8.1 for 1001 and 7.6 / 7.8 for 4097,
+// 128 x 2 x 1001 7.3 / 5.9, x 4097 11.2 / 5.9.
 constexpr int FEW_SLOTS = 256;
 inline bool few(int64_t slots, int64_t units, int choices, bool aligned) {
-    return slots <= FEW_SLOTS && slots + units / 1500 <= (aligned ? 240 : 200 + 20 * choices);
+    return slots <= FEW_SLOTS && slots + units / 1500 <= (aligned ? 290 : 270 + 20 * choices);
 }
 
 struct Plan {
