@@ -629,7 +629,9 @@ typedef enum {
     dnnl_cuda_interop_moe_dispatch,
     dnnl_cuda_interop_moe_combine,
     dnnl_cuda_interop_moe_combine_backward,
-    dnnl_cuda_interop_dropout
+    dnnl_cuda_interop_dropout,
+    dnnl_cuda_interop_rms_norm = 0x10010,
+    dnnl_cuda_interop_rms_norm_backward
 } dnnl_cuda_interop_primitive_kind_t; /* what dnnl_query_primitive_kind answers for them */
 
 typedef enum {
@@ -697,6 +699,38 @@ dnnl_status_t dnnl_cuda_interop_moe_combine_backward_primitive_desc_create(dnnl_
 dnnl_status_t dnnl_cuda_interop_dropout_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
         const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t residual_desc, const_dnnl_memory_desc_t dst_desc,
         float p, const_dnnl_primitive_attr_t attr);
+
+/* ---- the norm in front of a quantized product (no counterpart in the reference) ----
+ * As the primitives above: matrices [T, H] with neighbouring columns beside one another and any row pitch, dims that may be
+ * open, T that may be zero; 1 <= H <= 16384. */
+
+/* Root-mean-square norm.  h = SRC [T, H] (f32, bf16, f16) + SRC_2 (the residual, of SRC's type; residual_desc may be NULL)
+ * -> DST [T, H] = h / sqrt(mean over the row of h^2 + epsilon) x WEIGHTS [H] (f32 or SRC's type; NULL: 1), and, where sum_desc
+ * is given, DST_1 = h, of SRC's type.  (DST is made from the sum before it is rounded.)  DST is f32, of SRC's type, s8 or
+ * f8_e4m3.  DST_1 may be the residual's or SRC's memory, DST SRC's where the types agree.  Squares are summed in 32 bits: a
+ * row whose sum of squares exceeds them comes out as zeros, one with an infinity or a NaN as NaN.
+ *   An 8-bit DST holds round(value / scale), to nearest even, saturated (a NaN is 0 in s8).  Its scales are set by
+ * dnnl_primitive_attr_set_scales_v3 for DNNL_ARG_DST, f32, in device memory; without them the scale is 1:
+ *   mask 0, static: one scale, an input;
+ *   mask 1, dnnl_quantization_mode_dynamic_fp: a scale per row, [T, 1], which this primitive writes: the largest |value| of the
+ *     row over 127 (s8) or 448 (f8_e4m3);
+ *   mask 3 with groups {1, g}, dynamic_fp: the same per g neighbouring columns, [T, H / g]; g a power of two from 16 to 256 that
+ *     divides H.
+ * They are what dnnl_matmul takes as scales of its src.  Where the largest |value| is below 1e-36 the scale is 0 and so are the
+ * values; where a value is NaN the scale is NaN. */
+dnnl_status_t dnnl_cuda_interop_rms_norm_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t residual_desc, const_dnnl_memory_desc_t weights_desc,
+        const_dnnl_memory_desc_t dst_desc, const_dnnl_memory_desc_t sum_desc, float epsilon, const_dnnl_primitive_attr_t attr);
+/* Its gradient.  DIFF_DST [T, H], SRC the sum h, SRC_2 the gradient that reaches h along the residual path (diff_sum_desc may be
+ * NULL), all of one type, WEIGHTS as forward -> DIFF_SRC [T, H], of the same type: the gradient of h, which is that of src and
+ * that of the residual alike; DIFF_WEIGHTS [H] (f32 or SRC's type; diff_weights_desc may be NULL), summed in the same order
+ * every time.  DIFF_SRC may be the memory of DIFF_DST, SRC_2 or SRC.  Quantization of the output counts as the identity.
+ *   With DIFF_WEIGHTS, H may not be open, and there is a scratchpad, which holds sums between its kernels: executions of one
+ * primitive that overlap on the GPU need the user scratchpad mode and a buffer each, as moe_dispatch has it. */
+dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t diff_dst_desc, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t weights_desc,
+        const_dnnl_memory_desc_t diff_sum_desc, const_dnnl_memory_desc_t diff_src_desc, const_dnnl_memory_desc_t diff_weights_desc,
+        float epsilon, const_dnnl_primitive_attr_t attr);
 
 #ifdef __cplusplus
 }

@@ -23,7 +23,7 @@ _STATUS_NAME = ["success", "out_of_memory", "invalid_arguments", "unimplemented"
 
 # exec-arg ids (dnnl_types.h:2542-2786)
 ARG_SRC, ARG_SRC_1, ARG_DST, ARG_WEIGHTS, ARG_BIAS, ARG_SCRATCHPAD = 1, 2, 17, 33, 41, 80
-ARG_FROM, ARG_TO = ARG_SRC, ARG_DST
+ARG_FROM, ARG_TO, ARG_WEIGHTS_1 = ARG_SRC, ARG_DST, 34
 ARG_SRC_2, ARG_DST_1, ARG_DIFF_SRC, ARG_DIFF_DST, ARG_DIFF_WEIGHTS, ARG_ATTR_DROPOUT_SEED = 3, 18, 129, 145, 161, 511
 SCRATCHPAD_MODE_LIBRARY, SCRATCHPAD_MODE_USER = 0, 1  # dnnl_scratchpad_mode_t
 ARG_ATTR_SCALES, ARG_ATTR_ZERO_POINTS, ARG_ATTR_PRECOMPUTED_REDUCTIONS = 4096, 8192, 512
@@ -96,6 +96,8 @@ def lib():
         L.dnnl_cuda_interop_moe_combine_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, f, v]
         L.dnnl_cuda_interop_moe_combine_backward_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, v, f, v]
         L.dnnl_cuda_interop_dropout_primitive_desc_create.argtypes = [v, v, v, v, v, f, v]
+        L.dnnl_cuda_interop_rms_norm_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, f, v]
+        L.dnnl_cuda_interop_rms_norm_backward_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, v, f, v]
         L.dnnl_engine_create.argtypes = [C.c_void_p, C.c_int, C.c_size_t]
         _lib = L
     return _lib
@@ -322,6 +324,10 @@ class fpmath_mode:
     strict, bf16, f16, any, tf32 = range(5)
 
 
+class quantization_mode:  # dnnl_quantization_mode_t
+    undef, static_sazp, dynamic_mx, dynamic_fp = range(4)
+
+
 class primitive_attr:
     def __init__(self):
         self._h = C.c_void_p()
@@ -540,6 +546,37 @@ class dropout(matmul):
             _check(lib().dnnl_cuda_interop_dropout_primitive_desc_create(
                 C.byref(self._h), eng._h, src_md._h, _handle(residual_md), dst_md._h, p, _handle(attr)),
                 "could not create a primitive descriptor for the dropout primitive")
+
+
+class rms_norm(matmul):
+    """Root-mean-square norm of src + residual, times weights, in 32, 16 or 8 bits: ``{ARG_SRC: [T, H], ARG_SRC_2: residual
+    (optional), ARG_WEIGHTS: [H] (optional), ARG_DST: [T, H], ARG_DST_1: the sum (optional)}``.  An s8 or e4m3 dst takes its
+    scales from ``attr.set_scales(ARG_DST, ...)`` at ``ARG_ATTR_SCALES | ARG_DST``: mask 0 one that is given; with
+    ``qmode=quantization_mode.dynamic_fp`` the primitive writes them: mask 1 per row [T, 1], mask 3 and groups (1, g) per g
+    columns [T, H / g]."""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, src_md, dst_md, epsilon, weights_md=None, residual_md=None, sum_md=None, attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_rms_norm_primitive_desc_create(
+                C.byref(self._h), eng._h, src_md._h, _handle(residual_md), _handle(weights_md), dst_md._h, _handle(sum_md),
+                epsilon, _handle(attr)), "could not create a primitive descriptor for the rms_norm primitive")
+
+
+class rms_norm_backward(matmul):
+    """Its gradient: ``{ARG_DIFF_DST: [T, H], ARG_SRC: the sum, ARG_WEIGHTS: weights (optional), ARG_SRC_2: gradient of the sum
+    along the residual path (optional), ARG_DIFF_SRC: gradient of the sum, ARG_DIFF_WEIGHTS: [H] (optional)}``"""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, diff_dst_md, src_md, diff_src_md, epsilon, weights_md=None, diff_weights_md=None,
+                     diff_sum_md=None, attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(
+                C.byref(self._h), eng._h, diff_dst_md._h, src_md._h, _handle(weights_md), _handle(diff_sum_md), diff_src_md._h,
+                _handle(diff_weights_md), epsilon, _handle(attr)),
+                "could not create a primitive descriptor for the rms_norm_backward primitive")
 
 
 def launch_count():

@@ -932,7 +932,7 @@ dnnl_status_t dnnl_primitive_desc_query(const_dnnl_primitive_desc_t pd, dnnl_que
     if (is_token_op(pd->kind) && (what == dnnl_query_num_of_inputs_s32 || what == dnnl_query_num_of_outputs_s32)) {
         int in = 0, out = 0;
         for (const auto &kv : pd->token_op.args)
-            ++(kv.first == DNNL_ARG_DST || kv.first == DNNL_ARG_DST_1 || kv.first == DNNL_ARG_DIFF_SRC || kv.first == DNNL_ARG_DIFF_WEIGHTS ? out : in);
+            ++(kv.first == DNNL_ARG_DST || kv.first == DNNL_ARG_DST_1 || (kv.first == (DNNL_ARG_ATTR_SCALES | DNNL_ARG_DST) && pd->token_op.scaling > 1) || kv.first == DNNL_ARG_DIFF_SRC || kv.first == DNNL_ARG_DIFF_WEIGHTS ? out : in);
         *(int *)result = what == dnnl_query_num_of_inputs_s32 ? in : out;
         return dnnl_success;
     }

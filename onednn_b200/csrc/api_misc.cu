@@ -106,6 +106,7 @@ const char *arg_name(int arg) {
         case DNNL_ARG_DIFF_DST: return "diff_dst";
         case DNNL_ARG_DIFF_WEIGHTS: return "diff_wei";
         case DNNL_ARG_ATTR_DROPOUT_SEED: return "seed";
+        case DNNL_ARG_ATTR_SCALES | DNNL_ARG_DST: return "dst_scales";
         default: return "arg";
     }
 }
@@ -193,6 +194,8 @@ std::string pd_info_string(const dnnl_primitive_desc &pd) {
         else if (pd.kind == dnnl_cuda_interop_moe_route || pd.kind == dnnl_cuda_interop_moe_route_backward)
             aux << "scoring:" << (pd.token_op.scoring ? "sigmoid" : "softmax") << " normalize:" << pd.token_op.normalize
                 << " scale:" << pd.token_op.scale;
+        else if (pd.kind == dnnl_cuda_interop_rms_norm || pd.kind == dnnl_cuda_interop_rms_norm_backward)
+            aux << "epsilon:" << pd.token_op.epsilon;
         const dnnl_memory_desc *x = pd.token_op.find(DNNL_ARG_DIFF_DST) ? pd.token_op.find(DNNL_ARG_DIFF_DST) : pd.token_op.find(DNNL_ARG_SRC);
         return s + "," + attr_str(pd.attr) + "," + aux.str() + "," + dims_str(x->dims, x->ndims);
     }

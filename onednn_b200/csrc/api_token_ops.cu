@@ -1,4 +1,4 @@
-// Descriptors and execution of the operators around an expert layer's products and of dropout (dnnl_b200.h).  One check
+// Descriptors and execution of the operators around an expert layer's products, of dropout and of the norm (dnnl_b200.h).  One check
 // serves creation and, where dims were left open, each execution: it skips what an open dim leaves unsaid.
 #include <initializer_list>
 #include <memory>
@@ -46,6 +46,16 @@ struct checker_t {
         built(md->data_type == dt);
         return true;
     }
+    // `n` neighbouring values
+    bool vector(const dnnl_memory_desc *md, dnnl_dim_t n) {
+        require(md && md->ndims == 1 && md->format_kind != dnnl_format_kind_undef);
+        if (!md || md->ndims != 1 || md->format_kind == dnnl_format_kind_undef) return false;
+        built(md->format_kind == dnnl_blocked);
+        if (md->format_kind != dnnl_blocked) return false;
+        require(agree(md->dims[0], n));
+        built(md->dims[0] == 0 || md->dims[0] == 1 || md->strides[0] == 1);
+        return true;
+    }
     bool grouped(const dnnl_memory_desc *md, dnnl_dim_t rows, dnnl_dim_t cols, dnnl_dim_t groups) {
         require(md && md->is_grouped());
         if (!md || !md->is_grouped()) return false;
@@ -64,6 +74,37 @@ struct checker_t {
 
 dnnl_dim_t known(dnnl_dim_t a, dnnl_dim_t b) { return a == OPEN ? b : a; }
 dnnl_dim_t times(dnnl_dim_t a, dnnl_dim_t b) { return a == OPEN || b == OPEN || a > MAX_SLOTS || b > MAX_SLOTS ? OPEN : a * b; }
+
+// src, weights and sizes of the norm and of its gradient
+void norm_common(checker_t &c, const token_op_t &op, const dnnl_memory_desc *src, dnnl_dim_t T, dnnl_dim_t H, const dnnl_memory_desc *wei) {
+    c.require(op.epsilon > 0.f && op.epsilon - op.epsilon == 0.f);
+    c.built(is_float(src->data_type));
+    if (wei && c.vector(wei, H)) c.built(wei->data_type == dnnl_f32 || wei->data_type == src->data_type);
+    if (H != OPEN) {
+        c.require(H >= 1);
+        c.built(H <= NORM_MAX_COLS);
+    }
+    if (T != OPEN) c.built(T <= MAX_SLOTS);
+}
+
+// the tensor whose scales an attribute may set
+int scaled_arg(int kind) { return kind == dnnl_cuda_interop_rms_norm ? DNNL_ARG_DST : 0; }
+
+// the tensor's dims that the mask names, divided by the groups, dense
+dnnl_memory_desc scales_md(const quant_entry_t &q, const dnnl_memory_desc &base) {
+    dnnl_memory_desc md;
+    md.ndims = base.ndims;
+    md.data_type = q.dt;
+    md.format_kind = dnnl_blocked;
+    dnnl_dim_t stride = 1;
+    for (int i = base.ndims - 1; i >= 0; --i) {
+        const dnnl_dim_t g = q.group_ndims && i >= base.ndims - 2 ? q.groups[i - (base.ndims - 2)] : 1;
+        md.dims[i] = !((q.mask >> i) & 1) ? 1 : base.dims[i] == OPEN ? OPEN : base.dims[i] / g;
+        md.strides[i] = stride;
+        stride = stride == OPEN || md.dims[i] == OPEN ? OPEN : stride * md.dims[i];
+    }
+    return md;
+}
 
 dnnl_status_t check(int kind, const token_op_t &op) {
     checker_t c;
@@ -135,9 +176,59 @@ dnnl_status_t check(int kind, const token_op_t &op) {
             c.built(is_float(src->data_type));
             break;
         }
+        case dnnl_cuda_interop_rms_norm: {
+            if (!c.matrix(src, false) || !c.matrix(dst, true)) break;
+            const dnnl_dim_t T = known(src->dims[0], dst->dims[0]), H = known(src->dims[1], dst->dims[1]);
+            c.matrix(src, false, T, H, src->data_type);
+            c.matrix(dst, true, T, H, dst->data_type);
+            norm_common(c, op, src, T, H, wei);
+            if (src2) c.matrix(src2, false, T, H, src->data_type);
+            if (dst1) c.matrix(dst1, true, T, H, src->data_type);
+            const bool small = dst->data_type == dnnl_s8 || dst->data_type == dnnl_f8_e4m3;
+            c.built(small || dst->data_type == dnnl_f32 || dst->data_type == src->data_type);
+            if (op.scaling != NORM_SCALE_NONE) c.built(small);
+            if (op.scaling == NORM_SCALE_GROUP && H != OPEN) c.require(H % op.group == 0);
+            break;
+        }
+        case dnnl_cuda_interop_rms_norm_backward: {
+            if (!c.matrix(ddst, false) || !c.matrix(src, false) || !c.matrix(dsrc, true)) break;
+            const dnnl_dim_t T = known(known(ddst->dims[0], src->dims[0]), dsrc->dims[0]);
+            const dnnl_dim_t H = known(known(ddst->dims[1], src->dims[1]), dsrc->dims[1]);
+            c.matrix(src, false, T, H, src->data_type);
+            c.matrix(ddst, false, T, H, src->data_type);
+            c.matrix(dsrc, true, T, H, src->data_type);
+            norm_common(c, op, src, T, H, wei);
+            if (src2) c.matrix(src2, false, T, H, src->data_type);
+            if (dwei && c.vector(dwei, H)) {
+                c.built(H != OPEN); // (its scratchpad is made before the first execution)
+                c.built(dwei->data_type == dnnl_f32 || dwei->data_type == src->data_type);
+            }
+            break;
+        }
         default: return dnnl_invalid_arguments;
     }
     return c.status;
+}
+
+// Scales that an attribute asks for: how they are made or given, and their descriptor among the tensors.
+dnnl_status_t add_scales(int kind, token_op_t &op, const dnnl_primitive_attr &attr) {
+    const int arg = scaled_arg(kind);
+    const quant_entry_t &q = attr.scale(arg);
+    if (!arg || !q.set) return dnnl_success;
+    if (q.dt != dnnl_f32 || q.on_host) return dnnl_unimplemented;
+    if (kind == dnnl_cuda_interop_rms_norm) {
+        const bool made = q.qmode == dnnl_quantization_mode_dynamic_fp;
+        if (q.mask == 0 && q.qmode == dnnl_quantization_mode_static_sazp) op.scaling = NORM_SCALE_GIVEN;
+        else if (q.mask == 1 && made && !q.group_ndims) op.scaling = NORM_SCALE_ROW;
+        else if (q.mask == 3 && made && q.group_ndims && q.groups[0] == 1) {
+            const dnnl_dim_t g = q.groups[1];
+            if (g < 16 || g > 256 || (g & (g - 1))) return dnnl_unimplemented;
+            op.scaling = NORM_SCALE_GROUP;
+            op.group = (int)g;
+        } else return dnnl_unimplemented;
+    }
+    op.args[DNNL_ARG_ATTR_SCALES | arg] = scales_md(q, *op.find(arg));
+    return dnnl_success;
 }
 
 // A null or zero descriptor leaves an optional tensor out, and is an error for the others.
@@ -156,7 +247,11 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
     if (attr) {
         dnnl_primitive_attr plain = *attr;
         plain.scratchpad_mode = dnnl_scratchpad_mode_library;
+        if (scaled_arg(kind)) plain.scales.erase(scaled_arg(kind));
         if (!plain.has_default_values()) return dnnl_unimplemented;
+        st = add_scales(kind, op, *attr);
+        if (st == dnnl_success && op.scaling != NORM_SCALE_NONE) st = check(kind, op);
+        if (st != dnnl_success) return st;
     }
     if (op.p > 0.f || kind == dnnl_cuda_interop_dropout) { // (seed, offset)
         dnnl_memory_desc seed;
@@ -174,6 +269,13 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
     pd->impl_name = std::string("cuda:simt:") + token_op_name(kind);
     if (kind == dnnl_cuda_interop_moe_dispatch)
         pd->scratch_bytes = dispatch_scratch_bytes((int)op.args[DNNL_ARG_DST].group_count, engine->sm_count > 0 ? engine->sm_count : 148);
+    if (kind == dnnl_cuda_interop_rms_norm_backward && op.find(DNNL_ARG_DIFF_WEIGHTS)) {
+        const dnnl_dim_t cols[] = {op.find(DNNL_ARG_DIFF_WEIGHTS)->dims[0], op.find(DNNL_ARG_SRC)->dims[1],
+                op.find(DNNL_ARG_DIFF_DST)->dims[1], op.find(DNNL_ARG_DIFF_SRC)->dims[1]};
+        dnnl_dim_t known_cols = OPEN;
+        for (dnnl_dim_t n : cols) known_cols = known(known_cols, n);
+        pd->scratch_bytes = norm_scratch_bytes(known_cols, engine->sm_count > 0 ? engine->sm_count : 148);
+    }
     if (pd->scratch_bytes && pd->attr.scratchpad_mode == dnnl_scratchpad_mode_user) {
         pd->scratchpad.ndims = 1;
         pd->scratchpad.dims[0] = (dnnl_dim_t)pd->scratch_bytes;
@@ -190,7 +292,7 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
 
 // where an execution's tensors are
 struct bound_t {
-    struct { int arg; char *values; const int *offsets; } t[8];
+    struct { int arg; char *values; const int *offsets; } t[10];
     int n = 0;
 };
 
@@ -270,6 +372,30 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             a.diff_weights = (float *)ptr(DNNL_ARG_DIFF_WEIGHTS); a.diff_weights_ld = ld(DNNL_ARG_DIFF_WEIGHTS);
             return backward ? launch_combine_backward(a, sms, stream) : launch_combine(a, sms, stream);
         }
+        case dnnl_cuda_interop_rms_norm:
+        case dnnl_cuda_interop_rms_norm_backward: {
+            const bool backward = kind == dnnl_cuda_interop_rms_norm_backward;
+            const auto *src = op.find(DNNL_ARG_SRC), *dst = op.find(DNNL_ARG_DST), *wei = op.find(DNNL_ARG_WEIGHTS);
+            const auto *dwei = op.find(DNNL_ARG_DIFF_WEIGHTS);
+            NormArgs a {};
+            a.rows = src->dims[0]; a.cols = src->dims[1]; a.dt = src->data_type;
+            a.src = ptr(DNNL_ARG_SRC); a.src_ld = ld(DNNL_ARG_SRC);
+            a.residual = ptr(DNNL_ARG_SRC_2); a.residual_ld = ld(DNNL_ARG_SRC_2);
+            a.epsilon = op.epsilon;
+            a.weights = ptr(DNNL_ARG_WEIGHTS); a.weights_dt = wei ? wei->data_type : dnnl_f32;
+            if (backward) {
+                a.diff_dst = ptr(DNNL_ARG_DIFF_DST); a.diff_dst_ld = ld(DNNL_ARG_DIFF_DST);
+                a.diff_src = ptr(DNNL_ARG_DIFF_SRC); a.diff_src_ld = ld(DNNL_ARG_DIFF_SRC);
+                a.diff_weights = ptr(DNNL_ARG_DIFF_WEIGHTS); a.weights_grad_dt = dwei ? dwei->data_type : dnnl_f32;
+                a.parts = a.diff_weights ? (float *)scratch : nullptr;
+                return launch_rms_norm_backward(a, sms, stream);
+            }
+            a.sum = ptr(DNNL_ARG_DST_1); a.sum_ld = ld(DNNL_ARG_DST_1);
+            a.dst = ptr(DNNL_ARG_DST); a.dst_ld = ld(DNNL_ARG_DST); a.dst_dt = dst->data_type;
+            a.scaling = op.scaling; a.group = op.group;
+            a.scales = (float *)ptr(DNNL_ARG_ATTR_SCALES | DNNL_ARG_DST);
+            return launch_rms_norm(a, stream);
+        }
         default: {
             const auto *src = op.find(DNNL_ARG_SRC);
             DropoutArgs a {};
@@ -287,11 +413,16 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
 
 namespace qmm {
 
-bool is_token_op(int kind) { return kind >= dnnl_cuda_interop_moe_route && kind <= dnnl_cuda_interop_dropout; }
+bool is_token_op(int kind) {
+    return (kind >= dnnl_cuda_interop_moe_route && kind <= dnnl_cuda_interop_dropout)
+            || (kind >= dnnl_cuda_interop_rms_norm && kind <= dnnl_cuda_interop_rms_norm_backward);
+}
 
 const char *token_op_name(int kind) {
     static const char *const names[] = {"moe_route", "moe_route_backward", "moe_dispatch", "moe_combine", "moe_combine_backward", "dropout"};
-    return is_token_op(kind) ? names[kind - dnnl_cuda_interop_moe_route] : "unknown";
+    static const char *const later[] = {"rms_norm", "rms_norm_backward"};
+    if (!is_token_op(kind)) return "unknown";
+    return kind >= dnnl_cuda_interop_rms_norm ? later[kind - dnnl_cuda_interop_rms_norm] : names[kind - dnnl_cuda_interop_moe_route];
 }
 
 dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t stream, int nargs, const dnnl_exec_arg_t *args) try {
@@ -315,7 +446,7 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
         settled = pd.token_op;
         for (auto &kv : settled.args) {
             dnnl_memory_desc &want = kv.second;
-            if (kv.first == DNNL_ARG_ATTR_DROPOUT_SEED) continue;
+            if (kv.first == DNNL_ARG_ATTR_DROPOUT_SEED || (kv.first & DNNL_ARG_ATTR_SCALES)) continue;
             const dnnl_memory_desc &got = find(kv.first)->md;
             if (got.ndims != want.ndims || got.has_runtime_dims() || got.data_type != want.data_type
                     || got.format_kind != want.format_kind || got.is_grouped() != want.is_grouped()
@@ -327,13 +458,21 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
         }
         const dnnl_status_t st = check(pd.kind, settled);
         if (st != dnnl_success) return st;
+        const int scaled = scaled_arg(pd.kind), scales = DNNL_ARG_ATTR_SCALES | scaled;
+        if (settled.find(scales)) { // made from the settled tensor; the memory object has to hold as many
+            settled.args[scales] = scales_md(pd.attr.scale(scaled), *settled.find(scaled));
+            const dnnl_memory_desc &got = find(scales)->md;
+            if (got.data_type != dnnl_f32 || got.format_kind != dnnl_blocked || got.has_runtime_dims()
+                    || got.nelems() < settled.find(scales)->nelems())
+                return dnnl_invalid_arguments;
+        }
         op = &settled;
     }
     bound_t bound;
     for (const auto &kv : op->args) {
         const dnnl_memory_t m = find(kv.first);
         if (m->is_host_scalar) return dnnl_invalid_arguments;
-        auto &b = bound.t[bound.n++]; // (no kind has more than seven tensors)
+        auto &b = bound.t[bound.n++]; // (no kind has more than eight tensors)
         b.arg = kv.first;
         b.values = (char *)m->handles[0];
         b.offsets = nullptr;
@@ -439,6 +578,26 @@ dnnl_status_t dnnl_cuda_interop_dropout_primitive_desc_create(dnnl_primitive_des
     op.p = p;
     return create(primitive_desc, engine, dnnl_cuda_interop_dropout, op,
             {{DNNL_ARG_SRC, src_desc}, {DNNL_ARG_DST, dst_desc}}, {{DNNL_ARG_SRC_2, residual_desc}}, attr);
+}
+
+dnnl_status_t dnnl_cuda_interop_rms_norm_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t residual_desc, const_dnnl_memory_desc_t weights_desc,
+        const_dnnl_memory_desc_t dst_desc, const_dnnl_memory_desc_t sum_desc, float epsilon, const_dnnl_primitive_attr_t attr) {
+    token_op_t op;
+    op.epsilon = epsilon;
+    return create(primitive_desc, engine, dnnl_cuda_interop_rms_norm, op, {{DNNL_ARG_SRC, src_desc}, {DNNL_ARG_DST, dst_desc}},
+            {{DNNL_ARG_SRC_2, residual_desc}, {DNNL_ARG_WEIGHTS, weights_desc}, {DNNL_ARG_DST_1, sum_desc}}, attr);
+}
+
+dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t diff_dst_desc, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t weights_desc,
+        const_dnnl_memory_desc_t diff_sum_desc, const_dnnl_memory_desc_t diff_src_desc, const_dnnl_memory_desc_t diff_weights_desc,
+        float epsilon, const_dnnl_primitive_attr_t attr) {
+    token_op_t op;
+    op.epsilon = epsilon;
+    return create(primitive_desc, engine, dnnl_cuda_interop_rms_norm_backward, op,
+            {{DNNL_ARG_DIFF_DST, diff_dst_desc}, {DNNL_ARG_SRC, src_desc}, {DNNL_ARG_DIFF_SRC, diff_src_desc}},
+            {{DNNL_ARG_WEIGHTS, weights_desc}, {DNNL_ARG_SRC_2, diff_sum_desc}, {DNNL_ARG_DIFF_WEIGHTS, diff_weights_desc}}, attr);
 }
 
 } // extern "C"

@@ -145,11 +145,13 @@ enum impl_id_t : int {
     IMPL_COUNT
 };
 
-// The operators around an expert layer's products, and dropout (api_token_ops.cu): every tensor by its argument id.
+// The operators of dnnl_cuda_interop_primitive_kind_t (api_token_ops.cu): every tensor by its argument id.
 struct token_op_t {
     int scoring = 0, normalize = 0; // router
     float scale = 1.f;
     float p = 0.f; // dropout probability
+    float epsilon = 1.f; // norm
+    int scaling = 0, group = 0; // norm with an 8-bit dst: NORM_SCALE_*, columns of a group
     std::map<int, dnnl_memory_desc> args;
     const dnnl_memory_desc *find(int arg) const {
         auto it = args.find(arg);

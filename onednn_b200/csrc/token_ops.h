@@ -1,5 +1,5 @@
 // Plain-data descriptions of one execution of the operators around an expert layer's products (router, sort into grouped
-// rows, way back, their gradients) and of dropout, and the entry points that launch their kernels.  Each returns a
+// rows, way back, their gradients), of dropout and of the norm in front of a product, and the entry points that launch their kernels.  Each returns a
 // dnnl_status_t value (0 = success, 5 = CUDA runtime error) and only enqueues work on the stream.
 #pragma once
 #include <cuda_runtime.h>
@@ -96,6 +96,43 @@ struct DropoutArgs {
     DropoutState drop;
 };
 int launch_dropout(const DropoutArgs &a, int sm_count, cudaStream_t st);
+
+constexpr int64_t NORM_MAX_COLS = 16384; // a row stays in the registers of a CTA
+
+enum : int { NORM_SCALE_NONE = 0, NORM_SCALE_GIVEN = 1, NORM_SCALE_ROW = 2, NORM_SCALE_GROUP = 3 };
+
+struct NormArgs {
+    int64_t rows, cols;
+    int dt; // of src, residual and sum; of every gradient but the weights'
+    const void *src;
+    int64_t src_ld;
+    const void *residual; // may be null; backward: the gradient that comes along the residual path
+    int64_t residual_ld;
+    float epsilon;
+    const void *weights; // may be null: 1
+    int weights_dt; // f32 or dt
+    // forward
+    void *sum; // may be null
+    int64_t sum_ld;
+    void *dst;
+    int64_t dst_ld;
+    int dst_dt;
+    int scaling, group;
+    float *scales; // of dst: an input (given) or an output
+    // backward
+    const void *diff_dst;
+    int64_t diff_dst_ld;
+    void *diff_src;
+    int64_t diff_src_ld;
+    void *diff_weights; // may be null
+    int weights_grad_dt;
+    float *parts; // [part_count][cols], of the weights' gradient
+    int part_count; // the launcher's
+};
+int launch_rms_norm(const NormArgs &a, cudaStream_t st);
+int launch_rms_norm_backward(const NormArgs &a, int sm_count, cudaStream_t st);
+int norm_gradient_ctas(int64_t cols);
+size_t norm_scratch_bytes(int64_t cols, int sm_count);
 
 // Launches `kernel` as a programmatic dependent of whatever precedes it on the stream; the kernel reads and writes global
 // memory behind griddepcontrol.wait only.

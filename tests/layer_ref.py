@@ -1,0 +1,80 @@
+"""Plain 64-bit forms of the norm in front of a quantized product, with the bounds of what 32-bit sums may be off, and the
+binding of 8-bit tensors that its tests use."""
+import numpy as np
+
+import token_ref as R
+
+EPS = R.EPS
+E4M3 = 10
+LIMIT = {"s8": 127.0, "e4m3": 448.0}
+
+
+class Call(R.Call):
+    """also binds e4m3 tensors (torch.float8_e4m3fn)"""
+
+    CODE = dict(R.Call.CODE, e4m3=E4M3)
+
+    def name(self, t):
+        return "e4m3" if t.dtype == self.torch.float8_e4m3fn else super().name(t)
+
+
+def torch_dtype(name):
+    import torch
+    return torch.float8_e4m3fn if name == "e4m3" else R.torch_dtype(name)
+
+
+def rounded(a, dtype):
+    """64-bit numbers as `dtype` holds them"""
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(a))
+    return t.to(torch_dtype(dtype)).double().numpy()
+
+
+def norm(x, epsilon, weights=None, residual=None):
+    """(y, the sum)"""
+    h = x if residual is None else x + residual
+    y = h / np.sqrt((h * h).mean(1, keepdims=True) + epsilon)
+    return (y if weights is None else y * weights), h
+
+
+# Relative error of y before it is rounded to its type, in units of 2^-24: the sum (1), squares added by a thread (at most 32
+# of them), a warp (5) and a CTA (4), each square off by that of the sum twice (2): 43; the division, epsilon and, at half of
+# all that, the root: 24; the quotient (1) and two products (2).
+NORM_UNITS = 28
+
+
+def norm_backward(h, dy, epsilon, weights=None, dsum=None):
+    """(gradient of the sum, of the weights), and for each the size of the terms that it is the difference of"""
+    z = dy if weights is None else dy * weights
+    r = 1 / np.sqrt((h * h).mean(1, keepdims=True) + epsilon)
+    dh = r * z - h * r ** 3 * (h * z).mean(1, keepdims=True)
+    size = r * np.abs(z) + np.abs(h) * r ** 3 * np.abs(h * z).mean(1, keepdims=True)
+    if dsum is not None:
+        dh, size = dh + dsum, size + np.abs(dsum)
+    return dh, (dy * h * r).sum(0), size, np.abs(dy * h * r).sum(0)
+
+
+# Error of the gradient of the sum over that size: r (25) three times, the sum of h z (43), and six roundings of the rest.
+NORM_GRAD_UNITS = 125
+
+
+def step_e4m3(v):
+    """distance of the e4m3 values around |v|"""
+    return 2.0 ** (np.floor(np.log2(np.maximum(np.abs(v), 2.0 ** -6))) - 3)
+
+
+def check_8bit(q, v, units, out):
+    """q (what the device stored) is `v` rounded to nearest and saturated, v off by `units` 2^-24 of itself before that"""
+    limit, least = LIMIT[out], -128.0 if out == "s8" else -448.0
+    off = units * EPS * np.abs(v)
+    v = np.clip(v, least, limit)
+    half = 0.5 if out == "s8" else step_e4m3(np.abs(v) + off) / 2
+    assert (np.abs(q - v) <= half * (1 + 1e-12) + off).all(), np.abs(q - v).max()
+
+
+def quantized(y, out, group):
+    """(y / scale, scale) with the scale made per row (group 0) or per group of columns"""
+    T, H = y.shape
+    parts = y.reshape(T, -1, group or H)
+    scale = np.abs(parts).max(2) / LIMIT[out]
+    return (parts / scale[:, :, None]).reshape(T, H), scale
