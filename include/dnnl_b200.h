@@ -657,6 +657,19 @@ typedef enum {
 dnnl_status_t dnnl_cuda_interop_moe_route_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
         const_dnnl_memory_desc_t logits_desc, const_dnnl_memory_desc_t weights_desc, const_dnnl_memory_desc_t indices_desc,
         dnnl_cuda_interop_scoring_t scoring, int normalize, float scale, const_dnnl_primitive_attr_t attr);
+/* Router that chooses by score + bias, within the best groups of experts.  As above, but the K choices are those of the largest
+ * c = s + BIAS[e], by falling c, where s is the score (its softmax over all experts, or its sigmoid) and bias_desc may be NULL
+ * (0; f32 [E], neighbouring values): the bias moves the choice, not the weights, which are made from the scores of the chosen
+ * as above.  The experts are `groups` (1 to 32, a divisor of E) runs of neighbours; only those of the groups_kept groups take part
+ * whose group_best (1 or 2) largest c have the largest sum (of those that are there, where a group has fewer); K <= E / groups x groups_kept.
+ * The choice is by the values of c and of their sums in 64 bits, ties to the lowest group and expert.  A masked logit is masked here
+ * too; an expert with a bias of -inf or NaN is never chosen; +inf counts as the largest finite value.  With no bias and one group
+ * this is the router above, which chooses by the logits (scores that 64 bits hold as the same number differ there).  Its gradient is
+ * moe_route_backward with the indices that this primitive chose; the bias has none. */
+dnnl_status_t dnnl_cuda_interop_moe_route_v2_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t logits_desc, const_dnnl_memory_desc_t bias_desc, const_dnnl_memory_desc_t weights_desc,
+        const_dnnl_memory_desc_t indices_desc, dnnl_cuda_interop_scoring_t scoring, int normalize, float scale, int groups,
+        int groups_kept, int group_best, const_dnnl_primitive_attr_t attr);
 /* Its gradient.  SRC logits, SRC_1 the indices that the router chose, DIFF_DST the weights' gradient [T, K] (f32) ->
  * DIFF_SRC [T, E], of the logits' type. */
 dnnl_status_t dnnl_cuda_interop_moe_route_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,

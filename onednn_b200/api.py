@@ -92,6 +92,7 @@ def lib():
         v, i, f = C.c_void_p, C.c_int, C.c_float
         L.dnnl_cuda_interop_moe_route_primitive_desc_create.argtypes = [v, v, v, v, v, i, i, f, v]
         L.dnnl_cuda_interop_moe_route_backward_primitive_desc_create.argtypes = [v, v, v, v, v, v, i, i, f, v]
+        L.dnnl_cuda_interop_moe_route_v2_primitive_desc_create.argtypes = [v, v, v, v, v, v, i, i, f, i, i, i, v]
         L.dnnl_cuda_interop_moe_dispatch_primitive_desc_create.argtypes = [v, v, v, v, v, v, v]
         L.dnnl_cuda_interop_moe_combine_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, f, v]
         L.dnnl_cuda_interop_moe_combine_backward_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, v, f, v]
@@ -463,13 +464,22 @@ def _handle(obj):
 
 class moe_route(matmul):
     """The router of a mixture-of-experts layer: the k experts of the largest logits of each token and their weights.
-    ``{ARG_SRC: logits [T, E], ARG_DST: weights [T, k] f32, ARG_DST_1: indices [T, k] s32}``"""
+    ``{ARG_SRC: logits [T, E], ARG_DST: weights [T, k] f32, ARG_DST_1: indices [T, k] s32}``
+
+    With ``bias_md`` (``ARG_BIAS``: [E] f32) the choice is by score + bias; with ``groups`` only the ``groups_kept`` groups of
+    neighbouring experts take part whose ``group_best`` (1 or 2) best experts have the largest sum."""
 
     class primitive_desc(matmul.primitive_desc):
         def __init__(self, eng, logits_md, weights_md, indices_md, scoring=scoring.softmax, normalize=True, scale=1.0,
-                     attr=None):
+                     attr=None, bias_md=None, groups=1, groups_kept=1, group_best=1):
             self._h = C.c_void_p()
             self._eng = eng
+            if bias_md is not None or (groups, groups_kept, group_best) != (1, 1, 1):
+                _check(lib().dnnl_cuda_interop_moe_route_v2_primitive_desc_create(
+                    C.byref(self._h), eng._h, logits_md._h, _handle(bias_md), weights_md._h, indices_md._h, scoring,
+                    int(normalize), scale, groups, groups_kept, group_best, _handle(attr)),
+                    "could not create a primitive descriptor for the moe_route primitive")
+                return
             _check(lib().dnnl_cuda_interop_moe_route_primitive_desc_create(
                 C.byref(self._h), eng._h, logits_md._h, weights_md._h, indices_md._h, scoring, int(normalize), scale,
                 _handle(attr)), "could not create a primitive descriptor for the moe_route primitive")

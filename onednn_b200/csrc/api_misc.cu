@@ -194,7 +194,8 @@ std::string pd_info_string(const dnnl_primitive_desc &pd) {
         else if (pd.kind == dnnl_cuda_interop_moe_route || pd.kind == dnnl_cuda_interop_moe_route_backward)
             aux << "scoring:" << (pd.token_op.scoring ? "sigmoid" : "softmax") << " normalize:" << pd.token_op.normalize
                 << " scale:" << pd.token_op.scale;
-        else if (pd.kind == dnnl_cuda_interop_rms_norm || pd.kind == dnnl_cuda_interop_rms_norm_backward)
+        if (pd.token_op.groups > 1) aux << " groups:" << pd.token_op.groups_kept << "/" << pd.token_op.groups << ":" << pd.token_op.group_best;
+        if (pd.kind == dnnl_cuda_interop_rms_norm || pd.kind == dnnl_cuda_interop_rms_norm_backward)
             aux << "epsilon:" << pd.token_op.epsilon;
         const dnnl_memory_desc *x = pd.token_op.find(DNNL_ARG_DIFF_DST) ? pd.token_op.find(DNNL_ARG_DIFF_DST) : pd.token_op.find(DNNL_ARG_SRC);
         return s + "," + attr_str(pd.attr) + "," + aux.str() + "," + dims_str(x->dims, x->ndims);

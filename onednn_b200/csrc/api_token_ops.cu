@@ -131,6 +131,14 @@ dnnl_status_t check(int kind, const token_op_t &op) {
                 c.built(E <= TOKEN_MAX_EXPERTS);
             }
             c.choices(T, K);
+            if (const auto *bias = op.find(DNNL_ARG_BIAS))
+                if (c.vector(bias, E)) c.built(bias->data_type == dnnl_f32);
+            c.require(op.groups >= 1 && op.groups_kept >= 1 && op.groups_kept <= op.groups && (op.group_best == 1 || op.group_best == 2));
+            c.built(op.groups <= TOKEN_MAX_GROUPS);
+            if (E != OPEN && op.groups >= 1) {
+                c.require(E % op.groups == 0);
+                if (K != OPEN) c.require(K <= E / op.groups * op.groups_kept);
+            }
             if (backward) c.matrix(dsrc, true, T, E, src->data_type);
             break;
         }
@@ -333,6 +341,8 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             a.logits = ptr(DNNL_ARG_SRC); a.logits_ld = ld(DNNL_ARG_SRC);
             a.weights = (float *)ptr(weights); a.weights_ld = ld(weights);
             a.indices = (int *)ptr(indices); a.indices_ld = ld(indices);
+            a.bias = (const float *)ptr(DNNL_ARG_BIAS);
+            a.groups = op.groups; a.groups_kept = op.groups_kept; a.group_best = op.group_best;
             a.diff_logits = ptr(DNNL_ARG_DIFF_SRC); a.diff_logits_ld = ld(DNNL_ARG_DIFF_SRC);
             return backward ? launch_route_backward(a, stream) : launch_route(a, stream);
         }
@@ -528,6 +538,17 @@ dnnl_status_t dnnl_cuda_interop_moe_route_primitive_desc_create(dnnl_primitive_d
     op.scoring = (int)scoring; op.normalize = normalize != 0; op.scale = scale;
     return create(primitive_desc, engine, dnnl_cuda_interop_moe_route, op,
             {{DNNL_ARG_SRC, logits_desc}, {DNNL_ARG_DST, weights_desc}, {DNNL_ARG_DST_1, indices_desc}}, {}, attr);
+}
+
+dnnl_status_t dnnl_cuda_interop_moe_route_v2_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t logits_desc, const_dnnl_memory_desc_t bias_desc, const_dnnl_memory_desc_t weights_desc,
+        const_dnnl_memory_desc_t indices_desc, dnnl_cuda_interop_scoring_t scoring, int normalize, float scale, int groups,
+        int groups_kept, int group_best, const_dnnl_primitive_attr_t attr) {
+    token_op_t op;
+    op.scoring = (int)scoring; op.normalize = normalize != 0; op.scale = scale;
+    op.groups = groups; op.groups_kept = groups_kept; op.group_best = group_best;
+    return create(primitive_desc, engine, dnnl_cuda_interop_moe_route, op,
+            {{DNNL_ARG_SRC, logits_desc}, {DNNL_ARG_DST, weights_desc}, {DNNL_ARG_DST_1, indices_desc}}, {{DNNL_ARG_BIAS, bias_desc}}, attr);
 }
 
 dnnl_status_t dnnl_cuda_interop_moe_route_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,

@@ -147,7 +147,7 @@ enum impl_id_t : int {
 
 // The operators of dnnl_cuda_interop_primitive_kind_t (api_token_ops.cu): every tensor by its argument id.
 struct token_op_t {
-    int scoring = 0, normalize = 0; // router
+    int scoring = 0, normalize = 0, groups = 1, groups_kept = 1, group_best = 1; // router
     float scale = 1.f;
     float p = 0.f; // dropout probability
     float epsilon = 1.f; // norm

@@ -1,5 +1,5 @@
 // Plain-data descriptions of one execution of the operators around an expert layer's products (router, sort into grouped
-// rows, way back, their gradients), of dropout and of the norm in front of a product, and the entry points that launch their kernels.  Each returns a
+// rows, way back, their gradients), of dropout, of the norm in front of a product and of the adapters beside it, and the entry points that launch their kernels.  Each returns a
 // dnnl_status_t value (0 = success, 5 = CUDA runtime error) and only enqueues work on the stream.
 #pragma once
 #include <cuda_runtime.h>
@@ -10,6 +10,7 @@ namespace qmm {
 
 constexpr int TOKEN_MAX_EXPERTS = 1024; // a logit row stays in the registers of a warp; a count per expert in shared memory
 constexpr int TOKEN_MAX_CHOICES = 32; // one lane per choice
+constexpr int TOKEN_MAX_GROUPS = 32; // one lane per group of experts
 
 enum : int { SCORING_SOFTMAX = 0, SCORING_SIGMOID = 1 };
 
@@ -29,7 +30,11 @@ struct RouteArgs {
     int64_t indices_ld;
     void *diff_logits;
     int64_t diff_logits_ld;
+    // forward: what the choice goes by besides the scores
+    const float *bias; // [experts], may be null
+    int groups, groups_kept, group_best;
 };
+int launch_route_groups(const RouteArgs &a, cudaStream_t st); // with a bias or groups
 int launch_route(const RouteArgs &a, cudaStream_t st);
 int launch_route_backward(const RouteArgs &a, cudaStream_t st);
 
@@ -96,6 +101,28 @@ struct DropoutArgs {
     DropoutState drop;
 };
 int launch_dropout(const DropoutArgs &a, int sm_count, cudaStream_t st);
+
+constexpr int LOW_RANK_MAX = 128; // ranks of an adapter
+constexpr int LOW_RANK_MAX_ADAPTERS = 1024; // a count per adapter in shared memory
+
+struct LowRankArgs {
+    int64_t rows, in, out;
+    int rank, adapters;
+    int dt, dst_dt; // of src and both weights; of base and dst
+    const void *src;
+    int64_t src_ld;
+    const int *indices;
+    const void *down, *up; // [adapters][in][rank], [adapters][rank][out] by these strides, in elements
+    int64_t down_adapter, down_in, down_rank;
+    int64_t up_adapter, up_rank, up_out;
+    const float *scales; // [adapters], may be null: 1
+    const void *base; // may be null: 0
+    int64_t base_ld;
+    void *dst;
+    int64_t dst_ld;
+    int *status; // the engine's status word
+};
+int launch_low_rank(const LowRankArgs &a, int sm_count, cudaStream_t st);
 
 constexpr int64_t NORM_MAX_COLS = 16384; // a row stays in the registers of a CTA
 

@@ -1,5 +1,5 @@
-"""Plain 64-bit forms of the norm in front of a quantized product, with the bounds of what 32-bit sums may be off, and the
-binding of 8-bit tensors that its tests use."""
+"""Plain 64-bit forms of the norm in front of a quantized product and of the router with a bias and groups, with the bounds of
+what 32-bit sums may be off, and the binding of 8-bit tensors that the tests use."""
 import numpy as np
 
 import token_ref as R
@@ -78,3 +78,25 @@ def quantized(y, out, group):
     parts = y.reshape(T, -1, group or H)
     scale = np.abs(parts).max(2) / LIMIT[out]
     return (parts / scale[:, :, None]).reshape(T, H), scale
+
+
+def choose(logits, bias, scoring, k, groups=1, kept=1, best=1):
+    """indices of the k largest of score + bias in the kept groups of each row, ties to the lowest index; -1 where nothing is left"""
+    T, E = logits.shape
+    l = np.where(np.isnan(logits), -np.inf, logits)
+    there = l > -np.inf
+    with np.errstate(all="ignore"):
+        if scoring == "sigmoid":
+            s = 1 / (1 + np.exp(-l))
+        else:
+            e = np.exp(l - l.max(1, keepdims=True))
+            s = e / e.sum(1, keepdims=True)
+    b = np.zeros(E) if bias is None else bias
+    c = np.where(there & (b > -np.inf), s + np.minimum(b, np.finfo(np.float32).max), -np.inf)
+    if kept < groups:
+        top = np.sort(c.reshape(T, groups, E // groups), axis=2)[:, :, ::-1][:, :, :best]
+        rank = np.where(top[:, :, 0] > -np.inf, np.where(top > -np.inf, top, 0).sum(2), -np.inf)
+        out = np.argsort(-rank, axis=1, kind="stable")[:, kept:]
+        c.reshape(T, groups, E // groups)[np.arange(T)[:, None], out] = -np.inf
+    idx = np.argsort(-c, axis=1, kind="stable")[:, :k]
+    return np.where(np.take_along_axis(c, idx, 1) > -np.inf, idx, -1).astype(np.int32)
