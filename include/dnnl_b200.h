@@ -631,7 +631,8 @@ typedef enum {
     dnnl_cuda_interop_moe_combine_backward,
     dnnl_cuda_interop_dropout,
     dnnl_cuda_interop_rms_norm = 0x10010,
-    dnnl_cuda_interop_rms_norm_backward
+    dnnl_cuda_interop_rms_norm_backward,
+    dnnl_cuda_interop_low_rank_adapter
 } dnnl_cuda_interop_primitive_kind_t; /* what dnnl_query_primitive_kind answers for them */
 
 typedef enum {
@@ -744,6 +745,23 @@ dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_pri
         const_dnnl_memory_desc_t diff_dst_desc, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t weights_desc,
         const_dnnl_memory_desc_t diff_sum_desc, const_dnnl_memory_desc_t diff_src_desc, const_dnnl_memory_desc_t diff_weights_desc,
         float epsilon, const_dnnl_primitive_attr_t attr);
+
+/* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference) ----
+ * Row t of SRC [T, K] (bf16, f16) has the adapter i = SRC_1[t] ([T] s32) of WEIGHTS [n, K, r] and WEIGHTS_1 [n, r, N], of SRC's type:
+ *   DST_t = base_t + scale_i (SRC_t WEIGHTS_i) WEIGHTS_1_i;
+ * a row whose index is outside [0, n) is base_t.  DST [T, N] is of SRC's type or f32; SRC_2 is the base, of DST's type (what the
+ * projection made; base_desc may be NULL: 0), and may be DST's memory: rows without an adapter are then not touched.  The scales are
+ * set by dnnl_primitive_attr_set_scales for DNNL_ARG_WEIGHTS with mask 1: f32 [n] in device memory; without them 1.
+ *   1 <= r <= 128, n <= 2^20; weights have any strides (neighbours along K, r or N on 16-byte boundaries are fastest), the matrices
+ * any row pitch; T, K and N may be zero, and any dim open.  Rows in any order; a batch of prompts and single tokens of many requests
+ * are the same call.  All sums are f32; the middle product is rounded to 17 bits (27 where DST is f32) before the second.  A row of
+ * SRC with an infinity or a NaN gives infinities or NaN.
+ *   The gradient of SRC is this primitive on the gradient of DST, with WEIGHTS_1 transposed as WEIGHTS and WEIGHTS as WEIGHTS_1 (their
+ * strides say so), and the projection's own gradient as base. */
+dnnl_status_t dnnl_cuda_interop_low_rank_adapter_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t indices_desc, const_dnnl_memory_desc_t down_desc,
+        const_dnnl_memory_desc_t up_desc, const_dnnl_memory_desc_t base_desc, const_dnnl_memory_desc_t dst_desc,
+        const_dnnl_primitive_attr_t attr);
 
 #ifdef __cplusplus
 }

@@ -99,6 +99,7 @@ def lib():
         L.dnnl_cuda_interop_dropout_primitive_desc_create.argtypes = [v, v, v, v, v, f, v]
         L.dnnl_cuda_interop_rms_norm_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, f, v]
         L.dnnl_cuda_interop_rms_norm_backward_primitive_desc_create.argtypes = [v, v, v, v, v, v, v, v, f, v]
+        L.dnnl_cuda_interop_low_rank_adapter_primitive_desc_create.argtypes = [v] * 9
         L.dnnl_engine_create.argtypes = [C.c_void_p, C.c_int, C.c_size_t]
         _lib = L
     return _lib
@@ -587,6 +588,22 @@ class rms_norm_backward(matmul):
                 C.byref(self._h), eng._h, diff_dst_md._h, src_md._h, _handle(weights_md), _handle(diff_sum_md), diff_src_md._h,
                 _handle(diff_weights_md), epsilon, _handle(attr)),
                 "could not create a primitive descriptor for the rms_norm_backward primitive")
+
+
+class low_rank_adapter(matmul):
+    """Low-rank adapters of many requests beside a shared projection, base + scale[i] (src down[i]) up[i] with i the index of
+    each row: ``{ARG_SRC: [T, K], ARG_SRC_1: indices [T] s32 (outside [0, n): no adapter), ARG_WEIGHTS: down [n, K, r],
+    ARG_WEIGHTS_1: up [n, r, N], ARG_SRC_2: base [T, N] (optional; may be dst), ARG_DST: [T, N]}``, and with
+    ``attr.set_scales(ARG_WEIGHTS, 1)`` ``ARG_ATTR_SCALES | ARG_WEIGHTS: [n] f32``.  Its gradient with respect to src is the same
+    primitive with ``up`` and ``down`` transposed and exchanged."""
+
+    class primitive_desc(matmul.primitive_desc):
+        def __init__(self, eng, src_md, indices_md, down_md, up_md, dst_md, base_md=None, attr=None):
+            self._h = C.c_void_p()
+            self._eng = eng
+            _check(lib().dnnl_cuda_interop_low_rank_adapter_primitive_desc_create(
+                C.byref(self._h), eng._h, src_md._h, indices_md._h, down_md._h, up_md._h, _handle(base_md), dst_md._h,
+                _handle(attr)), "could not create a primitive descriptor for the low_rank_adapter primitive")
 
 
 def launch_count():

@@ -889,7 +889,7 @@ const_dnnl_memory_desc_t dnnl_primitive_desc_query_md(const_dnnl_primitive_desc_
         };
         switch ((int)what) {
             case dnnl_query_src_md: return of(index == 0 ? DNNL_ARG_SRC : index == 1 ? DNNL_ARG_SRC_1 : index == 2 ? DNNL_ARG_SRC_2 : 0);
-            case dnnl_query_weights_md: return index == 0 ? of(DNNL_ARG_WEIGHTS) : nullptr;
+            case dnnl_query_weights_md: return of(index == 0 ? DNNL_ARG_WEIGHTS : index == 1 ? DNNL_ARG_WEIGHTS_1 : 0);
             case dnnl_query_dst_md: return of(index == 0 ? DNNL_ARG_DST : index == 1 ? DNNL_ARG_DST_1 : 0);
             case dnnl_query_diff_src_md: return index == 0 ? of(DNNL_ARG_DIFF_SRC) : nullptr;
             case dnnl_query_diff_weights_md: return index == 0 ? of(DNNL_ARG_DIFF_WEIGHTS) : nullptr;

@@ -106,7 +106,9 @@ const char *arg_name(int arg) {
         case DNNL_ARG_DIFF_DST: return "diff_dst";
         case DNNL_ARG_DIFF_WEIGHTS: return "diff_wei";
         case DNNL_ARG_ATTR_DROPOUT_SEED: return "seed";
+        case DNNL_ARG_WEIGHTS_1: return "wei1";
         case DNNL_ARG_ATTR_SCALES | DNNL_ARG_DST: return "dst_scales";
+        case DNNL_ARG_ATTR_SCALES | DNNL_ARG_WEIGHTS: return "wei_scales";
         default: return "arg";
     }
 }

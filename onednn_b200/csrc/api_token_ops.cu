@@ -1,4 +1,4 @@
-// Descriptors and execution of the operators around an expert layer's products, of dropout and of the norm (dnnl_b200.h).  One check
+// Descriptors and execution of the operators around an expert layer's products, of dropout, of the norm and of low-rank adapters (dnnl_b200.h).  One check
 // serves creation and, where dims were left open, each execution: it skips what an open dim leaves unsaid.
 #include <initializer_list>
 #include <memory>
@@ -56,6 +56,14 @@ struct checker_t {
         built(md->dims[0] == 0 || md->dims[0] == 1 || md->strides[0] == 1);
         return true;
     }
+    // [a, b, c], strided anyhow
+    bool cube(const dnnl_memory_desc *md, dnnl_dim_t a, dnnl_dim_t b, dnnl_dim_t c) {
+        require(md && md->ndims == 3 && md->format_kind != dnnl_format_kind_undef);
+        if (!md || md->ndims != 3 || md->format_kind == dnnl_format_kind_undef) return false;
+        built(md->format_kind == dnnl_blocked);
+        require(agree(md->dims[0], a) && agree(md->dims[1], b) && agree(md->dims[2], c));
+        return md->format_kind == dnnl_blocked;
+    }
     bool grouped(const dnnl_memory_desc *md, dnnl_dim_t rows, dnnl_dim_t cols, dnnl_dim_t groups) {
         require(md && md->is_grouped());
         if (!md || !md->is_grouped()) return false;
@@ -88,7 +96,9 @@ void norm_common(checker_t &c, const token_op_t &op, const dnnl_memory_desc *src
 }
 
 // the tensor whose scales an attribute may set
-int scaled_arg(int kind) { return kind == dnnl_cuda_interop_rms_norm ? DNNL_ARG_DST : 0; }
+int scaled_arg(int kind) {
+    return kind == dnnl_cuda_interop_rms_norm ? DNNL_ARG_DST : kind == dnnl_cuda_interop_low_rank_adapter ? DNNL_ARG_WEIGHTS : 0;
+}
 
 // the tensor's dims that the mask names, divided by the groups, dense
 dnnl_memory_desc scales_md(const quant_entry_t &q, const dnnl_memory_desc &base) {
@@ -213,6 +223,31 @@ dnnl_status_t check(int kind, const token_op_t &op) {
             }
             break;
         }
+        case dnnl_cuda_interop_low_rank_adapter: {
+            const auto *up = op.find(DNNL_ARG_WEIGHTS_1);
+            if (!c.matrix(src, false) || !c.matrix(dst, true) || !c.cube(wei, OPEN, OPEN, OPEN) || !c.cube(up, OPEN, OPEN, OPEN)) break;
+            if (!c.vector(src1, OPEN)) break;
+            const dnnl_dim_t T = known(known(src->dims[0], dst->dims[0]), src1->dims[0]), n = known(wei->dims[0], up->dims[0]);
+            const dnnl_dim_t r = known(wei->dims[2], up->dims[1]);
+            c.require(agree(src->dims[0], T) && agree(dst->dims[0], T) && agree(src1->dims[0], T));
+            c.cube(wei, n, src->dims[1], r);
+            c.cube(up, n, r, dst->dims[1]);
+            if (src2) c.matrix(src2, false, T, dst->dims[1], dst->data_type);
+            c.built(src1->data_type == dnnl_s32 && (src->data_type == dnnl_bf16 || src->data_type == dnnl_f16));
+            c.built(wei->data_type == src->data_type && up->data_type == src->data_type);
+            c.built(dst->data_type == src->data_type || dst->data_type == dnnl_f32);
+            if (n != OPEN) {
+                c.require(n >= 1);
+                c.built(n <= LOW_RANK_MAX_ADAPTERS);
+            }
+            if (r != OPEN) {
+                c.require(r >= 1);
+                c.built(r <= LOW_RANK_MAX);
+            }
+            for (dnnl_dim_t d : {T, src->dims[1], dst->dims[1]})
+                if (d != OPEN) c.built(d <= MAX_SLOTS);
+            break;
+        }
         default: return dnnl_invalid_arguments;
     }
     return c.status;
@@ -234,6 +269,8 @@ dnnl_status_t add_scales(int kind, token_op_t &op, const dnnl_primitive_attr &at
             op.scaling = NORM_SCALE_GROUP;
             op.group = (int)g;
         } else return dnnl_unimplemented;
+    } else if (q.mask != 1 || q.group_ndims || q.qmode != dnnl_quantization_mode_static_sazp) { // one per adapter
+        return dnnl_unimplemented;
     }
     op.args[DNNL_ARG_ATTR_SCALES | arg] = scales_md(q, *op.find(arg));
     return dnnl_success;
@@ -406,6 +443,21 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             a.scales = (float *)ptr(DNNL_ARG_ATTR_SCALES | DNNL_ARG_DST);
             return launch_rms_norm(a, stream);
         }
+        case dnnl_cuda_interop_low_rank_adapter: {
+            const auto *src = op.find(DNNL_ARG_SRC), *dst = op.find(DNNL_ARG_DST), *down = op.find(DNNL_ARG_WEIGHTS), *up = op.find(DNNL_ARG_WEIGHTS_1);
+            LowRankArgs a {};
+            a.rows = src->dims[0]; a.in = src->dims[1]; a.out = dst->dims[1];
+            a.adapters = (int)down->dims[0]; a.rank = (int)down->dims[2];
+            a.dt = src->data_type; a.dst_dt = dst->data_type;
+            a.src = ptr(DNNL_ARG_SRC); a.src_ld = ld(DNNL_ARG_SRC);
+            a.indices = (const int *)ptr(DNNL_ARG_SRC_1);
+            a.down = ptr(DNNL_ARG_WEIGHTS); a.down_adapter = down->strides[0]; a.down_in = down->strides[1]; a.down_rank = down->strides[2];
+            a.up = ptr(DNNL_ARG_WEIGHTS_1); a.up_adapter = up->strides[0]; a.up_rank = up->strides[1]; a.up_out = up->strides[2];
+            a.scales = (const float *)ptr(DNNL_ARG_ATTR_SCALES | DNNL_ARG_WEIGHTS);
+            a.base = ptr(DNNL_ARG_SRC_2); a.base_ld = ld(DNNL_ARG_SRC_2);
+            a.dst = ptr(DNNL_ARG_DST); a.dst_ld = ld(DNNL_ARG_DST);
+            return launch_low_rank(a, sms, stream);
+        }
         default: {
             const auto *src = op.find(DNNL_ARG_SRC);
             DropoutArgs a {};
@@ -425,12 +477,12 @@ namespace qmm {
 
 bool is_token_op(int kind) {
     return (kind >= dnnl_cuda_interop_moe_route && kind <= dnnl_cuda_interop_dropout)
-            || (kind >= dnnl_cuda_interop_rms_norm && kind <= dnnl_cuda_interop_rms_norm_backward);
+            || (kind >= dnnl_cuda_interop_rms_norm && kind <= dnnl_cuda_interop_low_rank_adapter);
 }
 
 const char *token_op_name(int kind) {
     static const char *const names[] = {"moe_route", "moe_route_backward", "moe_dispatch", "moe_combine", "moe_combine_backward", "dropout"};
-    static const char *const later[] = {"rms_norm", "rms_norm_backward"};
+    static const char *const later[] = {"rms_norm", "rms_norm_backward", "low_rank_adapter"};
     if (!is_token_op(kind)) return "unknown";
     return kind >= dnnl_cuda_interop_rms_norm ? later[kind - dnnl_cuda_interop_rms_norm] : names[kind - dnnl_cuda_interop_moe_route];
 }
@@ -619,6 +671,15 @@ dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_pri
     return create(primitive_desc, engine, dnnl_cuda_interop_rms_norm_backward, op,
             {{DNNL_ARG_DIFF_DST, diff_dst_desc}, {DNNL_ARG_SRC, src_desc}, {DNNL_ARG_DIFF_SRC, diff_src_desc}},
             {{DNNL_ARG_WEIGHTS, weights_desc}, {DNNL_ARG_SRC_2, diff_sum_desc}, {DNNL_ARG_DIFF_WEIGHTS, diff_weights_desc}}, attr);
+}
+
+dnnl_status_t dnnl_cuda_interop_low_rank_adapter_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
+        const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t indices_desc, const_dnnl_memory_desc_t down_desc,
+        const_dnnl_memory_desc_t up_desc, const_dnnl_memory_desc_t base_desc, const_dnnl_memory_desc_t dst_desc,
+        const_dnnl_primitive_attr_t attr) {
+    return create(primitive_desc, engine, dnnl_cuda_interop_low_rank_adapter, token_op_t(),
+            {{DNNL_ARG_SRC, src_desc}, {DNNL_ARG_SRC_1, indices_desc}, {DNNL_ARG_WEIGHTS, down_desc}, {DNNL_ARG_WEIGHTS_1, up_desc},
+                    {DNNL_ARG_DST, dst_desc}}, {{DNNL_ARG_SRC_2, base_desc}}, attr);
 }
 
 } // extern "C"

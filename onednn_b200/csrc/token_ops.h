@@ -103,7 +103,7 @@ struct DropoutArgs {
 int launch_dropout(const DropoutArgs &a, int sm_count, cudaStream_t st);
 
 constexpr int LOW_RANK_MAX = 128; // ranks of an adapter
-constexpr int LOW_RANK_MAX_ADAPTERS = 1024; // a count per adapter in shared memory
+constexpr int LOW_RANK_MAX_ADAPTERS = 1 << 20;
 
 struct LowRankArgs {
     int64_t rows, in, out;
@@ -120,7 +120,6 @@ struct LowRankArgs {
     int64_t base_ld;
     void *dst;
     int64_t dst_ld;
-    int *status; // the engine's status word
 };
 int launch_low_rank(const LowRankArgs &a, int sm_count, cudaStream_t st);
 

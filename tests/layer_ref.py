@@ -100,3 +100,30 @@ def choose(logits, bias, scoring, k, groups=1, kept=1, best=1):
         c.reshape(T, groups, E // groups)[np.arange(T)[:, None], out] = -np.inf
     idx = np.argsort(-c, axis=1, kind="stable")[:, :k]
     return np.where(np.take_along_axis(c, idx, 1) > -np.inf, idx, -1).astype(np.int32)
+
+
+def low_rank(x, index, down, up, scale=None, base=None):
+    """(base + scale[i] (x down[i]) up[i], terms of the second product, of both): the latter are sums of magnitudes"""
+    T, N = x.shape[0], up.shape[2]
+    y = np.zeros((T, N)) if base is None else base.copy()
+    second, both = np.zeros((T, N)), np.zeros((T, N))
+    for i in np.unique(index):
+        if not 0 <= i < down.shape[0]:
+            continue
+        on, s = index == i, 1.0 if scale is None else scale[i]
+        v = x[on] @ down[i]
+        y[on] += s * (v @ up[i])
+        second[on] = abs(s) * (np.abs(v) @ np.abs(up[i]))
+        both[on] = abs(s) * ((np.abs(x[on]) @ np.abs(down[i])) @ np.abs(up[i]))
+    return y, second, both
+
+
+def low_rank_bound(y, second, both, base, K, r, dtype, out):
+    """What the adapters' result may be off.  An MMA adds sixteen products to a sum; its sum may be cut instead of rounded: 2^-23
+    of its terms' magnitudes each.  First product: at most K / 16 MMAs a warp, sums over 8 warps and 8 CTAs (16 roundings), the
+    scale (2).  What 16-bit parts leave out: 2^-18 (two of bf16), 2^-27 (three), 2^-22 (two of f16, whose smallest parts are
+    further down).  Second product: r / 16 MMAs a part on top of the base.  Then the output's rounding."""
+    parts = 2.0 ** -22 if dtype == "f16" else 2.0 ** -27 if out == "f32" else 2.0 ** -18
+    mmas = 3 * (r / 16 + 1) + 1
+    b = 0 if base is None else np.abs(base)
+    return both * (K / 16 + 20) * 2 * EPS + second * parts * (1 + 2.0 ** -8) + mmas * 2 * EPS * (second * 1.01 + b) + R.out_slack(y, out)
