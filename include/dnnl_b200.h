@@ -752,7 +752,7 @@ dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_pri
  * a row whose index is outside [0, n) is base_t.  DST [T, N] is of SRC's type or f32; SRC_2 is the base, of DST's type (what the
  * projection made; base_desc may be NULL: 0), and may be DST's memory: rows without an adapter are then not touched.  The scales are
  * set by dnnl_primitive_attr_set_scales for DNNL_ARG_WEIGHTS with mask 1: f32 [n] in device memory; without them 1.
- *   1 <= r <= 128, n <= 2^20; weights have any strides (neighbours along K, r or N on 16-byte boundaries are fastest), the matrices
+ *   1 <= r <= 128, n <= 1024; weights have any strides (neighbours along K, r or N on 16-byte boundaries are fastest), the matrices
  * any row pitch; T, K and N may be zero, and any dim open.  Rows in any order; a batch of prompts and single tokens of many requests
  * are the same call.  All sums are f32; the middle product is rounded to 17 bits (27 where DST is f32) before the second.  A row of
  * SRC with an infinity or a NaN gives infinities or NaN.

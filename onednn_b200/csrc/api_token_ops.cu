@@ -321,6 +321,11 @@ dnnl_status_t create(dnnl_primitive_desc_t *out, dnnl_engine_t engine, int kind,
         for (dnnl_dim_t n : cols) known_cols = known(known_cols, n);
         pd->scratch_bytes = norm_scratch_bytes(known_cols, engine->sm_count > 0 ? engine->sm_count : 148);
     }
+    if (kind == dnnl_cuda_interop_low_rank_adapter) {
+        const dnnl_dim_t rows = known(known(op.find(DNNL_ARG_SRC)->dims[0], op.find(DNNL_ARG_DST)->dims[0]), op.find(DNNL_ARG_SRC_1)->dims[0]);
+        const dnnl_dim_t rank = known(op.find(DNNL_ARG_WEIGHTS)->dims[2], op.find(DNNL_ARG_WEIGHTS_1)->dims[1]);
+        pd->scratch_bytes = low_rank_scratch_bytes(rows, rank);
+    }
     if (pd->scratch_bytes && pd->attr.scratchpad_mode == dnnl_scratchpad_mode_user) {
         pd->scratchpad.ndims = 1;
         pd->scratchpad.dims[0] = (dnnl_dim_t)pd->scratch_bytes;
@@ -456,7 +461,7 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             a.scales = (const float *)ptr(DNNL_ARG_ATTR_SCALES | DNNL_ARG_WEIGHTS);
             a.base = ptr(DNNL_ARG_SRC_2); a.base_ld = ld(DNNL_ARG_SRC_2);
             a.dst = ptr(DNNL_ARG_DST); a.dst_ld = ld(DNNL_ARG_DST);
-            return launch_low_rank(a, sms, stream);
+            return launch_low_rank(a, scratch, sms, stream);
         }
         default: {
             const auto *src = op.find(DNNL_ARG_SRC);

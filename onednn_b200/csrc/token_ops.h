@@ -103,7 +103,7 @@ struct DropoutArgs {
 int launch_dropout(const DropoutArgs &a, int sm_count, cudaStream_t st);
 
 constexpr int LOW_RANK_MAX = 128; // ranks of an adapter
-constexpr int LOW_RANK_MAX_ADAPTERS = 1 << 20;
+constexpr int LOW_RANK_MAX_ADAPTERS = 1024; // sixteen counts for each in shared memory
 
 struct LowRankArgs {
     int64_t rows, in, out;
@@ -121,7 +121,11 @@ struct LowRankArgs {
     void *dst;
     int64_t dst_ld;
 };
-int launch_low_rank(const LowRankArgs &a, int sm_count, cudaStream_t st);
+constexpr int LOW_RANK_FEW = 64; // rows that one launch serves
+constexpr int LOW_RANK_CHUNK = 8192; // rows whose sums are in the scratchpad at a time
+constexpr int LOW_RANK_SPLITS = 4; // of the columns that these sums run over, at most
+int launch_low_rank(const LowRankArgs &a, void *scratch, int sm_count, cudaStream_t st);
+size_t low_rank_scratch_bytes(int64_t rows, int64_t rank); // (negative: open)
 
 constexpr int64_t NORM_MAX_COLS = 16384; // a row stays in the registers of a CTA
 

@@ -83,7 +83,7 @@ def test_descriptors_and_refusals(host_engine):
 
 def test_kernels_read_with_coherent_loads():
     kernels = _reachable("low_rank.cu")
-    assert set(kernels) == {"low_rank_kernel"}
+    assert set(kernels) == {"low_rank_few_kernel", "low_rank_down_kernel", "low_rank_up_kernel"}
     for name, text in kernels.items():
         assert not NON_COHERENT.findall(text), name
 
@@ -96,7 +96,7 @@ def test_every_function_is_called():
 
 def test_cluster_barriers_come_in_pairs():
     """each arrival at the cluster's barrier has its wait: one right behind it, one before the sums are overwritten or the CTA ends"""
-    body = _functions(_source("low_rank.cu"))["low_rank_kernel"]
+    body = _functions(_source("low_rank.cu"))["low_rank_few_kernel"]
     assert len(re.findall(r"cluster_arrive\(\)", body)) == 2
     assert re.search(r"if \(arrived\) cluster_wait\(\);.*cluster_arrive\(\);\s*cluster_wait\(\);.*cluster_arrive\(\);\s*arrived = true;", body, re.S)
     assert re.search(r"if \(arrived\) cluster_wait\(\);\s*\}?\s*$", body)
