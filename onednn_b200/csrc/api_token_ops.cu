@@ -446,7 +446,7 @@ int launch(const dnnl_primitive &primitive, int kind, const token_op_t &op, cons
             a.dst = ptr(DNNL_ARG_DST); a.dst_ld = ld(DNNL_ARG_DST); a.dst_dt = dst->data_type;
             a.scaling = op.scaling; a.group = op.group;
             a.scales = (float *)ptr(DNNL_ARG_ATTR_SCALES | DNNL_ARG_DST);
-            return launch_rms_norm(a, stream);
+            return launch_rms_norm(a, sms, stream);
         }
         case dnnl_cuda_interop_low_rank_adapter: {
             const auto *src = op.find(DNNL_ARG_SRC), *dst = op.find(DNNL_ARG_DST), *down = op.find(DNNL_ARG_WEIGHTS), *up = op.find(DNNL_ARG_WEIGHTS_1);

@@ -158,26 +158,85 @@ __device__ __forceinline__ float make_scale(uint32_t most, float limit, float &i
     return m < SMALLEST_MAX ? 0.f : m / limit;
 }
 
-template <typename T, bool VEC, int THREADS, int CHUNKS>
-__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rms_norm_kernel(const __grid_constant__ NormArgs a) {
-    __shared__ float sums[64];
-    __shared__ uint32_t largest[32];
-    ptx::grid_dependency_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t t = THREADS == 32 ? (int64_t)blockIdx.x * 8 + threadIdx.x / 32 : (int64_t)blockIdx.x;
-    if (t >= a.rows) return; // (whole warps, and whole CTAs where they work together)
-    const int thread = threadIdx.x % THREADS;
-    const T *src = (const T *)a.src + t * a.src_ld;
-    float h[CHUNKS][8];
-    {
-        Chunk<T, VEC> x[CHUNKS], r[CHUNKS];
+// v / scale of its group, and the scales.  Groups of 16 to 256 columns, a power of two: in a warp's 256 columns they are whole
+// lanes' (VEC), or one to eight times 32 columns of all lanes, or half of them.
+template <bool VEC> __device__ __forceinline__ void scale_groups(const NormArgs &a, int64_t t, int64_t col, float limit, float (&v)[8]) {
+    float *scales = a.scales + t * (a.cols / a.group);
+    float inverse;
+    if constexpr (VEC) {
+        uint32_t m = 0;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) x[c].load(src, chunk_column<VEC>(c * THREADS + thread), a.cols);
-        if (a.residual) {
-            const T *residual = (const T *)a.residual + t * a.residual_ld;
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        for (int s = 1; s < a.group / 8; s *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
+        const float s = make_scale(m, limit, inverse);
+        if (col < a.cols && (col & (a.group - 1)) == 0) scales[col / a.group] = s;
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) r[c].load(residual, chunk_column<VEC>(c * THREADS + thread), a.cols);
+        for (int i = 0; i < 8; ++i) v[i] *= inverse;
+    } else {
+        uint32_t m[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m[i] = __float_as_uint(v[i]) & 0x7fffffffu;
+            if (a.group == 16) {
+#pragma unroll
+                for (int s = 1; s < 16; s *= 2) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], s));
+            } else {
+                m[i] = __reduce_max_sync(0xffffffffu, m[i]);
+            }
         }
+#pragma unroll
+        for (int step = 1; step < 8; step *= 2) // (pairs, fours, all eight of the 32 columns)
+            if (a.group > 32 * step) {
+                uint32_t other[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) other[i] = m[i ^ step];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m[i] = max(m[i], other[i]);
+            }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float s = make_scale(m[i], limit, inverse);
+            if (col + 32 * i < a.cols && ((col + 32 * i) & (a.group - 1)) == 0) scales[(col + 32 * i) / a.group] = s;
+            v[i] *= inverse;
+        }
+    }
+}
+
+// A CTA's threads, the rows that they work on at the same time, and the CTAs of an SM that registers are cut to.
+template <int THREADS> constexpr int BLOCK = THREADS == 32 ? 256 : THREADS;
+template <int THREADS> constexpr int TEAMS = THREADS == 32 ? 8 : 1;
+template <typename T, bool VEC, int THREADS> constexpr int FORWARD_CTAS = THREADS > 256 ? 1 : (VEC && sizeof(T) == 2 ? 768 : 512) / BLOCK<THREADS>;
+template <int THREADS> constexpr int BACKWARD_CTAS = THREADS > 256 ? 1 : 512 / BLOCK<THREADS>;
+template <int CHUNKS> constexpr bool AHEAD = CHUNKS <= 2; // registers for a row that is on its way
+
+// CTAs that stay take rows in turn; the next row is on its way while one is worked on, and the weights stay in registers.
+template <typename T, bool VEC, int THREADS, int CHUNKS>
+__global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS>) rms_norm_kernel(const __grid_constant__ NormArgs a) {
+    __shared__ float sums[2][64];
+    __shared__ uint32_t largest[2][32];
+    ptx::grid_dependency_wait();
+    const int thread = threadIdx.x % THREADS;
+    const int64_t step = (int64_t)gridDim.x * TEAMS<THREADS>;
+    int64_t t = (int64_t)blockIdx.x * TEAMS<THREADS> + (THREADS == 32 ? threadIdx.x / 32 : 0);
+    Chunk<T, VEC> x[CHUNKS], r[CHUNKS];
+    auto load = [&](int64_t row) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int64_t col = chunk_column<VEC>(c * THREADS + thread);
+            x[c].load((const T *)a.src + row * a.src_ld, col, a.cols);
+            if (a.residual) r[c].load((const T *)a.residual + row * a.residual_ld, col, a.cols);
+        }
+    };
+    if (AHEAD<CHUNKS> && t < a.rows) load(t);
+    float w[CHUNKS][8];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) load_weights<T, VEC>(a, chunk_column<VEC>(c * THREADS + thread), w[c]);
+    const float given = a.scaling == NORM_SCALE_GIVEN ? ptx::ld_dependent(a.scales) : 1.f;
+    const float limit = a.dst_dt == DT_S8 ? 127.f : 448.f;
+    for (int turn = 0; t < a.rows; t += step, turn ^= 1) {
+        if (!AHEAD<CHUNKS>) load(t);
+        float h[CHUNKS][8];
+        float sum[1] = {0.f};
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             x[c].get(h[c]);
@@ -187,87 +246,44 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rms_norm_kernel
 #pragma unroll
                 for (int i = 0; i < 8; ++i) h[c][i] += v[i];
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[0] = fmaf(h[c][i], h[c][i], sum[0]);
         }
-    }
-    const float given = a.scaling == NORM_SCALE_GIVEN ? ptx::ld_dependent(a.scales) : 1.f;
-    float sum[1] = {0.f};
+        if (AHEAD<CHUNKS> && t + step < a.rows) load(t + step);
+        if (a.sum) {
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum[0] = fmaf(h[c][i], h[c][i], sum[0]);
-        if (a.sum) Chunk<T, VEC>::store((T *)a.sum + t * a.sum_ld, chunk_column<VEC>(c * THREADS + thread), a.cols, h[c]);
-    }
-    row_sum<THREADS>(sum, sums);
-    const float scale = 1.f / sqrtf(sum[0] / (float)a.cols + a.epsilon);
-    uint32_t most = 0;
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        float w[8];
-        load_weights<T, VEC>(a, chunk_column<VEC>(c * THREADS + thread), w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            h[c][i] = h[c][i] * scale * w[i];
-            most = max(most, __float_as_uint(h[c][i]) & 0x7fffffffu);
+            for (int c = 0; c < CHUNKS; ++c) Chunk<T, VEC>::store((T *)a.sum + t * a.sum_ld, chunk_column<VEC>(c * THREADS + thread), a.cols, h[c]);
         }
-    }
-    float inverse = 1.f / given;
-    const float limit = a.dst_dt == DT_S8 ? 127.f : 448.f;
-    if (a.scaling == NORM_SCALE_ROW) {
-        const float s = make_scale(row_max<THREADS>(most, largest), limit, inverse);
-        if (thread == 0) a.scales[t] = s;
-    }
+        row_sum<THREADS>(sum, sums[turn]);
+        const float scale = 1.f / sqrtf(sum[0] / (float)a.cols + a.epsilon);
+        uint32_t most = 0;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        const int64_t col = chunk_column<VEC>(c * THREADS + thread);
-        if (a.scaling == NORM_SCALE_GROUP) {
-            // groups of 16 to 256 columns, a power of two: in a warp's 256 columns, whole lanes' (VEC) or 32 columns of all lanes
-            float *scales = a.scales + t * (a.cols / a.group);
-            if constexpr (VEC) {
-                uint32_t m = 0;
+        for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(h[c][i]) & 0x7fffffffu);
-                for (int s = 1; s < a.group / 8; s *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
-                const float s = make_scale(m, limit, inverse);
-                if (col < a.cols && col % a.group == 0) scales[col / a.group] = s;
+            for (int i = 0; i < 8; ++i) {
+                h[c][i] = h[c][i] * scale * w[c][i];
+                most = max(most, __float_as_uint(h[c][i]) & 0x7fffffffu);
+            }
+        float inverse = 1.f / given;
+        if (a.scaling == NORM_SCALE_ROW) {
+            const float s = make_scale(row_max<THREADS>(most, largest[turn]), limit, inverse);
+            if (thread == 0) a.scales[t] = s;
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int64_t col = chunk_column<VEC>(c * THREADS + thread);
+            if (a.scaling == NORM_SCALE_GROUP) {
+                scale_groups<VEC>(a, t, col, limit, h[c]);
+            } else if (a.scaling != NORM_SCALE_NONE) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) h[c][i] *= inverse;
-            } else {
-                uint32_t m[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    m[i] = __float_as_uint(h[c][i]) & 0x7fffffffu;
-                    if (a.group == 16) { // half a warp
-#pragma unroll
-                        for (int s = 1; s < 16; s *= 2) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], s));
-                    } else {
-                        m[i] = __reduce_max_sync(0xffffffffu, m[i]);
-                    }
-                }
-#pragma unroll
-                for (int step = 1; step < 8; step *= 2) // (pairs, fours, all eight of the 32 columns)
-                    if (a.group > 32 * step) {
-                        uint32_t other[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) other[i] = m[i ^ step];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) m[i] = max(m[i], other[i]);
-                    }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float s = make_scale(m[i], limit, inverse);
-                    if (col + 32 * i < a.cols && (col + 32 * i) % a.group == 0) scales[(col + 32 * i) / a.group] = s;
-                    h[c][i] *= inverse;
-                }
             }
-        } else if (a.scaling != NORM_SCALE_NONE) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h[c][i] *= inverse;
-        }
-        switch (a.dst_dt) {
-            case DT_F32: Chunk<float, VEC>::store((float *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
-            case DT_BF16: Chunk<__nv_bfloat16, VEC>::store((__nv_bfloat16 *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
-            case DT_F16: Chunk<__half, VEC>::store((__half *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
-            default: store_8bit<VEC>(a, t, col, h[c]);
+            switch (a.dst_dt) {
+                case DT_F32: Chunk<float, VEC>::store((float *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
+                case DT_BF16: Chunk<__nv_bfloat16, VEC>::store((__nv_bfloat16 *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
+                case DT_F16: Chunk<__half, VEC>::store((__half *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
+                default: store_8bit<VEC>(a, t, col, h[c]);
+            }
         }
     }
 }
@@ -275,12 +291,24 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rms_norm_kernel
 // Gradient: CTAs that stay take rows in turn; the weights and this CTA's part of their gradient stay in registers, and the
 // parts of all CTAs meet in the scratchpad, which the kernel behind this one adds up, in the same order every time.
 template <typename T, bool VEC, int THREADS, int CHUNKS>
-__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rms_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_norm_backward_kernel(const __grid_constant__ NormArgs a) {
     extern __shared__ float gathered[]; // a warp a row: [8][columns]
     __shared__ float sums[2][64];
     ptx::grid_dependency_wait();
-    constexpr int TEAMS = THREADS == 32 ? 8 : 1;
     const int thread = threadIdx.x % THREADS, team = THREADS == 32 ? threadIdx.x / 32 : 0;
+    const int64_t step = (int64_t)gridDim.x * TEAMS<THREADS>;
+    int64_t t = (int64_t)blockIdx.x * TEAMS<THREADS> + team;
+    Chunk<T, VEC> next_h[CHUNKS], next_dy[CHUNKS], next_more[CHUNKS];
+    auto load = [&](int64_t row) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int64_t col = chunk_column<VEC>(c * THREADS + thread);
+            next_h[c].load((const T *)a.src + row * a.src_ld, col, a.cols);
+            next_dy[c].load((const T *)a.diff_dst + row * a.diff_dst_ld, col, a.cols);
+            if (a.residual) next_more[c].load((const T *)a.residual + row * a.residual_ld, col, a.cols);
+        }
+    };
+    if (AHEAD<CHUNKS> && t < a.rows) load(t);
     float w[CHUNKS][8], dw[CHUNKS][8];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
@@ -288,16 +316,16 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rms_norm_backwa
 #pragma unroll
         for (int i = 0; i < 8; ++i) dw[c][i] = 0.f;
     }
-    int turn = 0;
-    for (int64_t t = (int64_t)blockIdx.x * TEAMS + team; t < a.rows; t += (int64_t)gridDim.x * TEAMS, turn ^= 1) {
+    for (int turn = 0; t < a.rows; t += step, turn ^= 1) {
+        if (!AHEAD<CHUNKS>) load(t);
         Chunk<T, VEC> h[CHUNKS], dy[CHUNKS], more[CHUNKS];
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int64_t col = chunk_column<VEC>(c * THREADS + thread);
-            h[c].load((const T *)a.src + t * a.src_ld, col, a.cols);
-            dy[c].load((const T *)a.diff_dst + t * a.diff_dst_ld, col, a.cols);
-            if (a.residual) more[c].load((const T *)a.residual + t * a.residual_ld, col, a.cols);
+            h[c] = next_h[c];
+            dy[c] = next_dy[c];
+            if (a.residual) more[c] = next_more[c];
         }
+        if (AHEAD<CHUNKS> && t + step < a.rows) load(t + step);
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
@@ -331,6 +359,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rms_norm_backwa
             Chunk<T, VEC>::store((T *)a.diff_src + t * a.diff_src_ld, chunk_column<VEC>(c * THREADS + thread), a.cols, d);
         }
     }
+    asm volatile("griddepcontrol.launch_dependents;"); // nothing is read any more
     if (!a.parts) return;
     if constexpr (THREADS == 32) {
 #pragma unroll
@@ -371,18 +400,17 @@ __global__ void __launch_bounds__(1024) rms_norm_weights_kernel(const __grid_con
     }
 }
 
-// threads of a row and its chunks of eight columns each: two chunks keep enough loads in flight, more where a CTA has no more threads
 template <typename T, bool VEC, int THREADS, int CHUNKS> int launch_shape(NormArgs &a, bool backward, int sm_count, cudaStream_t st) {
-    constexpr int block = THREADS == 32 ? 256 : THREADS, teams = THREADS == 32 ? 8 : 1;
-    const int64_t ctas = (a.rows + teams - 1) / teams;
-    if (!backward) {
-        if (ctas > 0x7fffffff) return 3;
-        return launch_dependent(rms_norm_kernel<T, VEC, THREADS, CHUNKS>, a, (unsigned)ctas, block, 0, st);
-    }
-    a.part_count = (int)std::min<int64_t>(ctas, (int64_t)sm_count * norm_gradient_ctas(a.cols));
-    return launch_dependent(rms_norm_backward_kernel<T, VEC, THREADS, CHUNKS>, a, a.part_count, block,
+    const int64_t ctas = (a.rows + TEAMS<THREADS> - 1) / TEAMS<THREADS>;
+    if (!backward)
+        return launch_dependent(rms_norm_kernel<T, VEC, THREADS, CHUNKS>, a, (unsigned)std::min<int64_t>(ctas, sm_count * FORWARD_CTAS<T, VEC, THREADS>),
+                BLOCK<THREADS>, 0, st);
+    // a part of the weights' gradient for each CTA: four rows at least, unless the SMs are too many
+    a.part_count = (int)std::min<int64_t>(std::min<int64_t>(ctas, std::max<int64_t>(ctas / 4, sm_count)), sm_count * norm_gradient_ctas(a.cols));
+    return launch_dependent(rms_norm_backward_kernel<T, VEC, THREADS, CHUNKS>, a, a.part_count, BLOCK<THREADS>,
             THREADS == 32 ? 8 * a.cols * sizeof(float) : 0, st);
 }
+// Threads of a row and its chunks of eight columns each: two chunks keep enough loads in flight, more where a CTA has no more threads.
 template <typename T, bool VEC> int launch_form(NormArgs &a, bool backward, int sm_count, cudaStream_t st) {
     const int64_t chunks = VEC ? (a.cols + 7) / 8 : (a.cols + 255) / 256 * 32;
     if (chunks <= 32) return launch_shape<T, VEC, 32, 1>(a, backward, sm_count, st);
@@ -426,12 +454,12 @@ int launch_any(const NormArgs &a, bool backward, int sm_count, cudaStream_t st) 
 } // namespace
 
 // CTAs per SM of the gradient's kernel, each with a part of the weights' gradient
-int norm_gradient_ctas(int64_t cols) { return cols <= 2048 ? 8 : cols <= 4096 ? 4 : 2; }
+int norm_gradient_ctas(int64_t cols) { return cols <= 512 ? 2 : cols <= 1024 ? 8 : cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1; }
 size_t norm_scratch_bytes(int64_t cols, int sm_count) { return (size_t)sm_count * norm_gradient_ctas(cols) * cols * sizeof(float); }
 
-int launch_rms_norm(const NormArgs &a, cudaStream_t st) {
+int launch_rms_norm(const NormArgs &a, int sm_count, cudaStream_t st) {
     if (a.rows == 0 || a.cols == 0) return 0;
-    return launch_any(a, false, 0, st);
+    return launch_any(a, false, sm_count, st);
 }
 int launch_rms_norm_backward(const NormArgs &a, int sm_count, cudaStream_t st) {
     if (a.cols == 0) return 0;

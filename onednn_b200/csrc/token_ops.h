@@ -159,7 +159,7 @@ struct NormArgs {
     float *parts; // [part_count][cols], of the weights' gradient
     int part_count; // the launcher's
 };
-int launch_rms_norm(const NormArgs &a, cudaStream_t st);
+int launch_rms_norm(const NormArgs &a, int sm_count, cudaStream_t st);
 int launch_rms_norm_backward(const NormArgs &a, int sm_count, cudaStream_t st);
 int norm_gradient_ctas(int64_t cols);
 size_t norm_scratch_bytes(int64_t cols, int sm_count);
