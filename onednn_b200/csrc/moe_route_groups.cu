@@ -146,12 +146,14 @@ __global__ void __launch_bounds__(WARPS * 32) route_groups_kernel(const __grid_c
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) {
-        const uint32_t k = expert_of(i, lane) < a.experts ? order_key(to_f32(raw[i])) : 0u;
-        there |= k ? 1u << i : 0u;
-        value[i] = k ? fminf(to_f32(raw[i]), LARGEST<T>) : -INFINITY;
-        top = fmaxf(top, value[i]);
+        const float l = to_f32(raw[i]);
+        const bool on = expert_of(i, lane) < a.experts && l > -INFINITY; // (not a NaN either)
+        there |= on ? 1u << i : 0u;
+        value[i] = on ? fminf(l, LARGEST<T>) : -INFINITY;
     }
     if (a.scoring == SCORING_SOFTMAX) {
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i) top = fmaxf(top, value[i]);
         top = warp_max(top);
 #pragma unroll
         for (int i = 0; i < PER_LANE; ++i) {
@@ -164,60 +166,96 @@ __global__ void __launch_bounds__(WARPS * 32) route_groups_kernel(const __grid_c
         for (int i = 0; i < PER_LANE; ++i) value[i] *= inverse;
     } else {
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i) value[i] = sigmoid(value[i]);
+        for (int i = 0; i < PER_LANE; ++i) value[i] = __fdividef(1.f, 1.f + expf(-value[i]));
     }
     float most_bias = 0.f;
+    if (a.bias) {
+        float bias[PER_LANE];
+        if (a.aligned_bias) {
+            constexpr int B = V < 4 ? V : 4;
+            struct alignas(4 * B) Group { float v[B]; };
+#pragma unroll
+            for (int i = 0; i < PER_LANE; i += B)
+                if (expert_of(i, lane) < a.experts) {
+                    const Group g = *reinterpret_cast<const Group *>(a.bias + expert_of(i, lane));
+#pragma unroll
+                    for (int j = 0; j < B; ++j) bias[i + j] = g.v[j];
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i)
+                if (expert_of(i, lane) < a.experts) bias[i] = a.bias[expert_of(i, lane)];
+        }
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i) {
+            const bool on = expert_of(i, lane) < a.experts && bias[i] > -INFINITY;
+            if (!on) there &= ~(1u << i);
+            const float b = on ? fminf(bias[i], LARGEST<float>) : 0.f;
+            most_bias = fmaxf(most_bias, fabsf(b));
+            value[i] += b;
+        }
+        most_bias = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_bias)));
+    }
     uint32_t key[PER_LANE];
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) {
-        if (a.bias) {
-            const uint32_t b = there >> i & 1 ? order_key(a.bias[expert_of(i, lane)]) : 0u;
-            if (!b) there &= ~(1u << i);
-            const float v = key_value<float>(b ? b : 0x80000000u);
-            most_bias = fmaxf(most_bias, fabsf(v));
-            value[i] += v;
-        }
-        key[i] = there >> i & 1 ? order_key(value[i]) : 0u;
+        value[i] = there >> i & 1 ? value[i] : -INFINITY;
+        key[i] = order_key(value[i]);
     }
-    if (a.bias) most_bias = warp_max(most_bias);
     bool close = false; // 32 bits do not tell
     if (a.groups_kept < a.groups) {
-        float *values = (float *)own;
-        const uint32_t reciprocal = (1u << 20) / size + 1; // e / size for e < 1024: the error stays below 1 / size
-#pragma unroll
-        for (int i = 0; i < PER_LANE; ++i) {
-            const int e = expert_of(i, lane), g = (int)((e * reciprocal) >> 20);
-            if (e < a.experts) values[g * stride + (e - g * size)] = key[i] ? value[i] : -INFINITY;
-        }
-        __syncwarp();
+        // the two largest of group `lane`
         float first = -INFINITY, second = -INFINITY;
-        const int group = lane / lanes;
-        if (group < a.groups)
-            for (int i = lane % lanes; i < size; i += lanes) {
-                const float c = values[group * stride + i];
-                second = fmaxf(second, fminf(first, c));
-                first = fmaxf(first, c);
+        auto merge = [](float &f, float &s, float f2, float s2) {
+            s = fmaxf(fminf(f, f2), fmaxf(s, s2));
+            f = fmaxf(f, f2);
+        };
+        const uint32_t reciprocal = (1u << 20) / size + 1; // e / size for e < 1024: the error stays below 1 / size
+        const int span = size / V; // lanes of a group, where a lane's neighbours share one
+        if (size % V == 0 && (span & (span - 1)) == 0 && span <= 32) {
+            const int per_chunk = 32 / span;
+#pragma unroll
+            for (int c = 0; c < PER_LANE / V; ++c) {
+                float f = -INFINITY, s = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < V; ++i) merge(f, s, value[c * V + i], -INFINITY);
+                for (int d = 1; d < span; d *= 2) merge(f, s, __shfl_xor_sync(0xffffffffu, f, d), __shfl_xor_sync(0xffffffffu, s, d));
+                const int from = lane % per_chunk * span;
+                const float f2 = __shfl_sync(0xffffffffu, f, from), s2 = __shfl_sync(0xffffffffu, s, from);
+                if (lane / per_chunk == c) {
+                    first = f2;
+                    second = s2;
+                }
             }
-        for (int s = 1; s < lanes; s *= 2) {
-            const float f = __shfl_xor_sync(0xffffffffu, first, s), n = __shfl_xor_sync(0xffffffffu, second, s);
-            second = fmaxf(fminf(first, f), fmaxf(second, n));
-            first = fmaxf(first, f);
+        } else {
+            float *values = (float *)own;
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) {
+                const int e = expert_of(i, lane), g = (int)((e * reciprocal) >> 20);
+                if (e < a.experts) values[g * stride + (e - g * size)] = value[i];
+            }
+            __syncwarp();
+            const int group = lane / lanes;
+            float f = -INFINITY, s = -INFINITY;
+            if (group < a.groups)
+                for (int i = lane % lanes; i < size; i += lanes) merge(f, s, values[group * stride + i], -INFINITY);
+            for (int d = 1; d < lanes; d *= 2) merge(f, s, __shfl_xor_sync(0xffffffffu, f, d), __shfl_xor_sync(0xffffffffu, s, d));
+            first = __shfl_sync(0xffffffffu, f, lane * lanes);
+            second = __shfl_sync(0xffffffffu, s, lane * lanes);
         }
-        const float rank = a.group_best == 2 && second > -INFINITY ? first + second : first;
-        uint32_t k = lane % lanes == 0 && group < a.groups ? order_key(rank) : 0u, kept = 0;
-        float last = 0.f;
-        for (int j = 0; j <= a.groups_kept; ++j) {
-            const uint32_t most = __reduce_max_sync(0xffffffffu, k);
-            if (most == 0) break;
-            const float r = key_value<float>(most);
-            if (j == a.groups_kept) { // the first that is left out: two sums, each of scores up to rank + 2 biases
-                close = last - r <= 2.f * (score_error(a.scoring) + 0x1p-22f) * (fabsf(last) + 4.f * most_bias);
-                break;
-            }
-            last = r;
-            const int at = __ffs(__ballot_sync(0xffffffffu, k == most)) - 1;
-            kept |= 1u << (at / lanes);
-            if (lane == at) k = 0;
+        const bool real = lane < a.groups && first > -INFINITY;
+        const float rank = !real ? -INFINITY : a.group_best == 2 && second > -INFINITY ? first + second : first;
+        int better = 0;
+        for (int g = 0; g < a.groups; ++g) {
+            const float other = __shfl_sync(0xffffffffu, rank, g);
+            better += other > rank || (other == rank && g < lane);
+        }
+        const uint32_t kept = __ballot_sync(0xffffffffu, real && better < a.groups_kept);
+        // the last that is kept and the first that is not: two sums, each of scores up to rank + 2 biases
+        const uint32_t ends = __ballot_sync(0xffffffffu, real && better == a.groups_kept - 1), next = __ballot_sync(0xffffffffu, real && better == a.groups_kept);
+        if (next) {
+            const float l = __shfl_sync(0xffffffffu, rank, __ffs(ends) - 1), n = __shfl_sync(0xffffffffu, rank, __ffs(next) - 1);
+            close = !(l - n > 2.f * (score_error(a.scoring) + 0x1p-22f) * (fabsf(l) + 4.f * most_bias));
         }
 #pragma unroll
         for (int i = 0; i < PER_LANE; ++i) {
@@ -231,21 +269,29 @@ __global__ void __launch_bounds__(WARPS * 32) route_groups_kernel(const __grid_c
         key[i] = key[i] ? (key[i] & ~SLOT) | (SLOT - i) : 0u;
         best = max(best, key[i]);
     }
-    int index = -1; // of choice `lane`
-    float last = 0.f;
-    for (int j = 0; j <= a.choices && !close; ++j) {
+    uint32_t mine = 0, owner = 0, several = 0; // lane j: key and lane (as a bit) of choice j
+    for (int j = 0; j < a.choices && !close; ++j) {
         const uint32_t most = __reduce_max_sync(0xffffffffu, best);
         if (most == 0) break;
         const uint32_t owners = __ballot_sync(0xffffffffu, best == most);
-        const float c = key_value<float>(most & ~SLOT);
-        // what the slot's bits hide (2^-23 of the value each), the sum's rounding and the score's error, of both
-        if (j > 0) close = last - c <= 2.f * (score_error(a.scoring) + (PER_LANE + 1) * 0x1p-23f) * (fabsf(last) + most_bias);
-        if (j == a.choices) break;
-        close = close || (owners & (owners - 1));
-        last = c;
-        const int owner = __ffs(owners) - 1, slot = (int)(SLOT - (most & SLOT));
-        if (lane == j) index = expert_of(slot, owner);
-        if (lane == owner) best = next_below(key, most);
+        if (lane == j) {
+            mine = most;
+            owner = owners;
+        }
+        several |= owners & (owners - 1);
+        best = next_below(key, most);
+    }
+    const int slot = (int)(SLOT - (mine & SLOT));
+    int index = mine ? expert_of(slot, __ffs(owner) - 1) : -1; // of choice `lane`
+    {
+        // The next key, of the first that is left out behind the last choice.  Keys differ from c by what the slot's bits hide
+        // (2^-23 of the value each), the sum's rounding and the score's error.
+        const uint32_t left_out = __reduce_max_sync(0xffffffffu, best), down = __shfl_down_sync(0xffffffffu, mine, 1);
+        const uint32_t after = lane == a.choices - 1 ? left_out : down;
+        const float c = key_value<float>(mine & ~SLOT), n = key_value<float>(after & ~SLOT);
+        const bool near = lane < a.choices && mine && after
+                && !(c - n > 2.f * (score_error(a.scoring) + (PER_LANE + 1) * 0x1p-23f) * (fabsf(c) + most_bias));
+        close = close || several || __any_sync(0xffffffffu, near);
     }
     if (close) index = choose_in_64_bits(a, row, own);
     const bool chosen = index >= 0;
@@ -284,6 +330,8 @@ template <typename T> int launch_typed(RouteArgs a, cudaStream_t st) {
                                               : route_groups_kernel<T, 32>;
     const int grouped = a.groups_kept < a.groups ? a.groups * group_stride(a.experts / a.groups, group_lanes(a.groups)) : 0;
     const size_t smem = (size_t)WARPS * ((std::max(2 * a.experts, grouped) + 1) / 2) * sizeof(double); // at most 40 KB
+    const int four = std::min(values, 4);
+    a.aligned_bias = a.bias && (uintptr_t)a.bias % (4 * four) == 0 && a.experts % four == 0;
     const int rc = launch_dependent(kernel, a, (unsigned)grid, WARPS * 32, smem, st);
     if (rc == 0) count_launch();
     return rc;

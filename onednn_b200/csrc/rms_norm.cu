@@ -32,21 +32,54 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) { // saturate
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// two 32-bit floats in a register pair: one instruction works on both
+struct Pair { uint64_t bits; };
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ Pair both(float v) { return pair(v, v); }
+__device__ __forceinline__ void split(Pair p, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.bits)); }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) { // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // Eight columns of a row.  VEC: neighbours from `col` on, the row a multiple of eight and all its tensors aligned to 16 bytes
 // (8-bit ones to 8).  Otherwise col, col + 32, ...: a warp covers the same 256 columns in either form.
-template <bool VEC> __device__ __forceinline__ int64_t chunk_column(int64_t chunk) {
+template <bool VEC> __device__ __forceinline__ int chunk_column(int chunk) {
     return VEC ? chunk * 8 : chunk / 32 * 256 + chunk % 32;
 }
 template <typename T, bool VEC> struct Chunk {
     uint4 raw[VEC ? sizeof(T) / 2 : 1];
     T each[VEC ? 1 : 8];
-    __device__ __forceinline__ void load(const T *row, int64_t col, int64_t cols) {
+    __device__ __forceinline__ void load(const T *row, int col, int cols) {
         if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
                 raw[i] = make_uint4(0, 0, 0, 0);
                 if (col < cols) raw[i] = ptx::ld_dependent((const uint4 *)(row + col) + i);
             }
+        } else if (col + 224 < cols) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) each[i] = row[col + 32 * i];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) each[i] = col + 32 * i < cols ? row[col + 32 * i] : from_f32<T>(0.f);
@@ -71,9 +104,21 @@ template <typename T, bool VEC> struct Chunk {
             unpack2(raw[0].w, v[6], v[7], T());
         }
     }
-    static __device__ __forceinline__ void store(T *row, int64_t col, int64_t cols, const float (&v)[8]) {
+    __device__ __forceinline__ void get(Pair (&p)[4]) const {
+        float v[8];
+        get(v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
+    }
+    static __device__ __forceinline__ void store(T *row, int col, int cols, const Pair (&p)[4]) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split(p[i], v[2 * i], v[2 * i + 1]);
         if constexpr (VEC) {
             Cols<T, true>::store(row, col, cols, v);
+        } else if (col + 224 < cols) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row[col + 32 * i] = from_f32<T>(v[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -83,24 +128,28 @@ template <typename T, bool VEC> struct Chunk {
 };
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_weights(const NormArgs &a, int64_t col, float (&w)[8]) {
+__device__ __forceinline__ void load_weights(const NormArgs &a, int col, Pair (&w)[4]) {
     if (!a.weights) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = 1.f;
+        for (int i = 0; i < 4; ++i) w[i] = both(1.f);
     } else if (a.weights_dt == DT_F32) {
         Chunk<float, VEC> c;
-        c.load((const float *)a.weights, col, a.cols);
+        c.load((const float *)a.weights, col, (int)a.cols);
         c.get(w);
     } else {
         Chunk<T, VEC> c;
-        c.load((const T *)a.weights, col, a.cols);
+        c.load((const T *)a.weights, col, (int)a.cols);
         c.get(w);
     }
 }
 
-template <bool VEC> __device__ __forceinline__ void store_8bit(const NormArgs &a, int64_t t, int64_t col, const float (&v)[8]) {
+template <bool VEC> __device__ __forceinline__ void store_8bit(const NormArgs &a, int64_t t, int col, const Pair (&p)[4]) {
     uint8_t *row = (uint8_t *)a.dst + t * a.dst_ld;
-    if (col >= a.cols) return;
+    const int cols = (int)a.cols;
+    if (col >= cols) return;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split(p[i], v[2 * i], v[2 * i + 1]);
     uint32_t lo, hi; // bytes 0 to 3 and 4 to 7
     if (a.dst_dt == DT_S8) {
         lo = cvt_s8(v[0]) | cvt_s8(v[1]) << 8 | cvt_s8(v[2]) << 16 | cvt_s8(v[3]) << 24;
@@ -114,7 +163,7 @@ template <bool VEC> __device__ __forceinline__ void store_8bit(const NormArgs &a
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (col + 32 * i < a.cols) row[col + 32 * i] = (uint8_t)((i < 4 ? lo : hi) >> 8 * (i % 4));
+            if (col + 32 * i < cols) row[col + 32 * i] = (uint8_t)((i < 4 ? lo : hi) >> 8 * (i % 4));
     }
 }
 
@@ -151,32 +200,54 @@ template <int THREADS> __device__ __forceinline__ uint32_t row_max(uint32_t v, u
     return v;
 }
 
-// scale and its reciprocal from the bits of the largest |value| (the bits of a NaN are above all others)
-__device__ __forceinline__ float make_scale(uint32_t most, float limit, float &inverse) {
-    const float m = __uint_as_float(most);
-    inverse = m < SMALLEST_MAX ? 0.f : limit / m;
-    return m < SMALLEST_MAX ? 0.f : m / limit;
+// What brings h w to its 8-bit value, and the scale, of which h w `most` is the largest magnitude (in the bits of a float, those of
+// a NaN are above all others): limit / most, and most r / limit with r the row's norm.  reciprocal: of limit.
+__device__ __forceinline__ float make_scale(uint32_t most, float r, float limit, float reciprocal, float &factor) {
+    const float m = __uint_as_float(most), y = m * r, q = y * reciprocal;
+    float inverse; // off by one unit at most, subnormal results too
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(m));
+    factor = y < SMALLEST_MAX ? 0.f : y == y ? inverse * limit : y;
+    // the quotient, with what is left of the division put back; an infinity stays one
+    return y < SMALLEST_MAX ? 0.f : y < INFINITY ? fmaf(fmaf(-q, limit, y), reciprocal, q) : y;
+}
+// 1 / sqrt(v): one Newton step on the approximation
+__device__ __forceinline__ float inverse_root(float v) {
+    const float r = rsqrtf(v);
+    return v < INFINITY ? fmaf(r * 0.5f, fmaf(-v * r, r, 1.f), r) : r;
 }
 
-// v / scale of its group, and the scales.  Groups of 16 to 256 columns, a power of two: in a warp's 256 columns they are whole
-// lanes' (VEC), or one to eight times 32 columns of all lanes, or half of them.
-template <bool VEC> __device__ __forceinline__ void scale_groups(const NormArgs &a, int64_t t, int64_t col, float limit, float (&v)[8]) {
-    float *scales = a.scales + t * (a.cols / a.group);
-    float inverse;
+__device__ __forceinline__ float largest(const Pair (&v)[4]) { // magnitude, or NaN
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        split(v[i], lo, hi);
+        m = max_nan(max_nan(m, fabsf(lo)), fabsf(hi));
+    }
+    return m;
+}
+
+// h w to 8 bits by the scales of its groups, and the scales.  Groups of 16 to 256 columns, a power of two: in a warp's 256 columns
+// they are whole lanes' (VEC), or one to eight times 32 columns of all lanes, or half of them.
+template <bool VEC>
+__device__ __forceinline__ void scale_groups(const NormArgs &a, float *scales, int col, float r, float limit, float reciprocal, Pair (&v)[4]) {
+    const int shift = 31 - __clz(a.group), cols = (int)a.cols;
     if constexpr (VEC) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        uint32_t m = __float_as_uint(largest(v)) & 0x7fffffffu;
         for (int s = 1; s < a.group / 8; s *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
-        const float s = make_scale(m, limit, inverse);
-        if (col < a.cols && (col & (a.group - 1)) == 0) scales[col / a.group] = s;
+        float factor;
+        const float s = make_scale(m, r, limit, reciprocal, factor);
+        if (col < cols && (col & (a.group - 1)) == 0) scales[col >> shift] = s;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= inverse;
+        for (int i = 0; i < 4; ++i) v[i] = v[i] * both(factor);
     } else {
+        float each[8], factor[8];
         uint32_t m[8];
 #pragma unroll
+        for (int i = 0; i < 4; ++i) split(v[i], each[2 * i], each[2 * i + 1]);
+#pragma unroll
         for (int i = 0; i < 8; ++i) {
-            m[i] = __float_as_uint(v[i]) & 0x7fffffffu;
+            m[i] = __float_as_uint(each[i]) & 0x7fffffffu;
             if (a.group == 16) {
 #pragma unroll
                 for (int s = 1; s < 16; s *= 2) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], s));
@@ -195,93 +266,99 @@ template <bool VEC> __device__ __forceinline__ void scale_groups(const NormArgs 
             }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float s = make_scale(m[i], limit, inverse);
-            if (col + 32 * i < a.cols && ((col + 32 * i) & (a.group - 1)) == 0) scales[(col + 32 * i) / a.group] = s;
-            v[i] *= inverse;
+            const float s = make_scale(m[i], r, limit, reciprocal, factor[i]);
+            if (col + 32 * i < cols && ((col + 32 * i) & (a.group - 1)) == 0) scales[(col + 32 * i) >> shift] = s;
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = pair(each[2 * i] * factor[2 * i], each[2 * i + 1] * factor[2 * i + 1]);
     }
 }
 
 // A CTA's threads, the rows that they work on at the same time, and the CTAs of an SM that registers are cut to.
 template <int THREADS> constexpr int BLOCK = THREADS == 32 ? 256 : THREADS;
 template <int THREADS> constexpr int TEAMS = THREADS == 32 ? 8 : 1;
-template <typename T, bool VEC, int THREADS> constexpr int FORWARD_CTAS = THREADS > 256 ? 1 : (VEC && sizeof(T) == 2 ? 768 : 512) / BLOCK<THREADS>;
+template <typename T, bool VEC, int THREADS, int CHUNKS>
+constexpr int FORWARD_CTAS = THREADS > 256 ? 1 : (VEC && sizeof(T) == 2 && CHUNKS <= 2 ? 768 : 512) / BLOCK<THREADS>;
 template <int THREADS> constexpr int BACKWARD_CTAS = THREADS > 256 ? 1 : 512 / BLOCK<THREADS>;
-template <int CHUNKS> constexpr bool AHEAD = CHUNKS <= 2; // registers for a row that is on its way
+// whether registers hold a row that is on its way
+template <typename T, bool VEC, int THREADS, int CHUNKS> constexpr bool FORWARD_AHEAD = CHUNKS <= 2 || (VEC && sizeof(T) == 2 && THREADS <= 256);
+template <typename T, int CHUNKS> constexpr bool BACKWARD_AHEAD = CHUNKS * sizeof(T) <= 4;
 
 // CTAs that stay take rows in turn; the next row is on its way while one is worked on, and the weights stay in registers.
 template <typename T, bool VEC, int THREADS, int CHUNKS>
-__global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS>) rms_norm_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, CHUNKS>) rms_norm_kernel(const __grid_constant__ NormArgs a) {
     __shared__ float sums[2][64];
-    __shared__ uint32_t largest[2][32];
+    __shared__ uint32_t most[2][32];
     ptx::grid_dependency_wait();
-    const int thread = threadIdx.x % THREADS;
+    const int thread = threadIdx.x % THREADS, cols = (int)a.cols;
     const int64_t step = (int64_t)gridDim.x * TEAMS<THREADS>;
     int64_t t = (int64_t)blockIdx.x * TEAMS<THREADS> + (THREADS == 32 ? threadIdx.x / 32 : 0);
     Chunk<T, VEC> x[CHUNKS], r[CHUNKS];
     auto load = [&](int64_t row) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int64_t col = chunk_column<VEC>(c * THREADS + thread);
-            x[c].load((const T *)a.src + row * a.src_ld, col, a.cols);
-            if (a.residual) r[c].load((const T *)a.residual + row * a.residual_ld, col, a.cols);
+            const int col = chunk_column<VEC>(c * THREADS + thread);
+            x[c].load((const T *)a.src + row * a.src_ld, col, cols);
+            if (a.residual) r[c].load((const T *)a.residual + row * a.residual_ld, col, cols);
         }
     };
-    if (AHEAD<CHUNKS> && t < a.rows) load(t);
-    float w[CHUNKS][8];
+    if (FORWARD_AHEAD<T, VEC, THREADS, CHUNKS> && t < a.rows) load(t);
+    Pair w[CHUNKS][4];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) load_weights<T, VEC>(a, chunk_column<VEC>(c * THREADS + thread), w[c]);
-    const float given = a.scaling == NORM_SCALE_GIVEN ? ptx::ld_dependent(a.scales) : 1.f;
-    const float limit = a.dst_dt == DT_S8 ? 127.f : 448.f;
+    const float given = a.scaling == NORM_SCALE_GIVEN ? 1.f / ptx::ld_dependent(a.scales) : 1.f;
+    const float limit = a.dst_dt == DT_S8 ? 127.f : 448.f, reciprocal = a.dst_dt == DT_S8 ? 1.f / 127.f : 1.f / 448.f;
+    const float per_column = 1.f / (float)cols;
     for (int turn = 0; t < a.rows; t += step, turn ^= 1) {
-        if (!AHEAD<CHUNKS>) load(t);
-        float h[CHUNKS][8];
-        float sum[1] = {0.f};
+        if (!FORWARD_AHEAD<T, VEC, THREADS, CHUNKS>) load(t);
+        Pair h[CHUNKS][4], squares = both(0.f);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             x[c].get(h[c]);
             if (a.residual) {
-                float v[8];
+                Pair v[4];
                 r[c].get(v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[c][i] += v[i];
+                for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] + v[i];
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[0] = fmaf(h[c][i], h[c][i], sum[0]);
+            for (int i = 0; i < 4; ++i) squares = fma(h[c][i], h[c][i], squares);
         }
-        if (AHEAD<CHUNKS> && t + step < a.rows) load(t + step);
+        if (FORWARD_AHEAD<T, VEC, THREADS, CHUNKS> && t + step < a.rows) load(t + step);
         if (a.sum) {
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) Chunk<T, VEC>::store((T *)a.sum + t * a.sum_ld, chunk_column<VEC>(c * THREADS + thread), a.cols, h[c]);
+            for (int c = 0; c < CHUNKS; ++c) Chunk<T, VEC>::store((T *)a.sum + t * a.sum_ld, chunk_column<VEC>(c * THREADS + thread), cols, h[c]);
         }
-        row_sum<THREADS>(sum, sums[turn]);
-        const float scale = 1.f / sqrtf(sum[0] / (float)a.cols + a.epsilon);
-        uint32_t most = 0;
+        float sum[2];
+        split(squares, sum[0], sum[1]);
+        float total[1] = {sum[0] + sum[1]};
+        row_sum<THREADS>(total, sums[turn]);
+        const float root = inverse_root(fmaf(total[0], per_column, a.epsilon));
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                h[c][i] = h[c][i] * scale * w[c][i];
-                most = max(most, __float_as_uint(h[c][i]) & 0x7fffffffu);
-            }
-        float inverse = 1.f / given;
+            for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] * w[c][i];
+        float factor = root * given;
         if (a.scaling == NORM_SCALE_ROW) {
-            const float s = make_scale(row_max<THREADS>(most, largest[turn]), limit, inverse);
+            float m = 0.f;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) m = max_nan(m, largest(h[c]));
+            const float s = make_scale(row_max<THREADS>(__float_as_uint(m) & 0x7fffffffu, most[turn]), root, limit, reciprocal, factor);
             if (thread == 0) a.scales[t] = s;
         }
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int64_t col = chunk_column<VEC>(c * THREADS + thread);
+            const int col = chunk_column<VEC>(c * THREADS + thread);
             if (a.scaling == NORM_SCALE_GROUP) {
-                scale_groups<VEC>(a, t, col, limit, h[c]);
-            } else if (a.scaling != NORM_SCALE_NONE) {
+                scale_groups<VEC>(a, a.scales + t * (cols / a.group), col, root, limit, reciprocal, h[c]);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[c][i] *= inverse;
+                for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] * both(factor);
             }
             switch (a.dst_dt) {
-                case DT_F32: Chunk<float, VEC>::store((float *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
-                case DT_BF16: Chunk<__nv_bfloat16, VEC>::store((__nv_bfloat16 *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
-                case DT_F16: Chunk<__half, VEC>::store((__half *)a.dst + t * a.dst_ld, col, a.cols, h[c]); break;
+                case DT_F32: Chunk<float, VEC>::store((float *)a.dst + t * a.dst_ld, col, cols, h[c]); break;
+                case DT_BF16: Chunk<__nv_bfloat16, VEC>::store((__nv_bfloat16 *)a.dst + t * a.dst_ld, col, cols, h[c]); break;
+                case DT_F16: Chunk<__half, VEC>::store((__half *)a.dst + t * a.dst_ld, col, cols, h[c]); break;
                 default: store_8bit<VEC>(a, t, col, h[c]);
             }
         }
@@ -295,29 +372,31 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
     extern __shared__ float gathered[]; // a warp a row: [8][columns]
     __shared__ float sums[2][64];
     ptx::grid_dependency_wait();
-    const int thread = threadIdx.x % THREADS, team = THREADS == 32 ? threadIdx.x / 32 : 0;
+    const int thread = threadIdx.x % THREADS, team = THREADS == 32 ? threadIdx.x / 32 : 0, cols = (int)a.cols;
+    const float per_column = 1.f / (float)cols;
     const int64_t step = (int64_t)gridDim.x * TEAMS<THREADS>;
     int64_t t = (int64_t)blockIdx.x * TEAMS<THREADS> + team;
     Chunk<T, VEC> next_h[CHUNKS], next_dy[CHUNKS], next_more[CHUNKS];
     auto load = [&](int64_t row) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int64_t col = chunk_column<VEC>(c * THREADS + thread);
-            next_h[c].load((const T *)a.src + row * a.src_ld, col, a.cols);
-            next_dy[c].load((const T *)a.diff_dst + row * a.diff_dst_ld, col, a.cols);
-            if (a.residual) next_more[c].load((const T *)a.residual + row * a.residual_ld, col, a.cols);
+            const int col = chunk_column<VEC>(c * THREADS + thread);
+            next_h[c].load((const T *)a.src + row * a.src_ld, col, cols);
+            next_dy[c].load((const T *)a.diff_dst + row * a.diff_dst_ld, col, cols);
+            if (a.residual) next_more[c].load((const T *)a.residual + row * a.residual_ld, col, cols);
         }
     };
-    if (AHEAD<CHUNKS> && t < a.rows) load(t);
-    float w[CHUNKS][8], dw[CHUNKS][8];
+    if (BACKWARD_AHEAD<T, CHUNKS> && t < a.rows) load(t);
+    asm volatile("griddepcontrol.launch_dependents;"); // all CTAs are resident; what comes next waits for their end
+    Pair w[CHUNKS][4], dw[CHUNKS][4];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
         load_weights<T, VEC>(a, chunk_column<VEC>(c * THREADS + thread), w[c]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dw[c][i] = 0.f;
+        for (int i = 0; i < 4; ++i) dw[c][i] = both(0.f);
     }
     for (int turn = 0; t < a.rows; t += step, turn ^= 1) {
-        if (!AHEAD<CHUNKS>) load(t);
+        if (!BACKWARD_AHEAD<T, CHUNKS>) load(t);
         Chunk<T, VEC> h[CHUNKS], dy[CHUNKS], more[CHUNKS];
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
@@ -325,45 +404,49 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
             dy[c] = next_dy[c];
             if (a.residual) more[c] = next_more[c];
         }
-        if (AHEAD<CHUNKS> && t + step < a.rows) load(t + step);
-        float s[2] = {0.f, 0.f};
+        if (BACKWARD_AHEAD<T, CHUNKS> && t + step < a.rows) load(t + step);
+        Pair squares = both(0.f), products = both(0.f);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            float x[8], g[8];
+            Pair x[4], g[4];
             h[c].get(x);
             dy[c].get(g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s[0] = fmaf(x[i], x[i], s[0]);
-                s[1] = fmaf(x[i] * w[c][i], g[i], s[1]);
+            for (int i = 0; i < 4; ++i) {
+                squares = fma(x[i], x[i], squares);
+                products = fma(x[i] * w[c][i], g[i], products);
             }
         }
+        float s[2], odd[2];
+        split(squares, s[0], odd[0]);
+        split(products, s[1], odd[1]);
+        s[0] += odd[0];
+        s[1] += odd[1];
         row_sum<THREADS>(s, sums[turn]);
-        const float r = 1.f / sqrtf(s[0] / (float)a.cols + a.epsilon);
-        const float inner = s[1] / (float)a.cols * r * r; // dh = r (z - h inner)
+        const float r = inverse_root(fmaf(s[0], per_column, a.epsilon));
+        const Pair root = both(r), inner = both(-(s[1] * per_column * r * r)); // dh = r (z - h inner)
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            float x[8], g[8], d[8];
+            Pair x[4], g[4], d[4];
             h[c].get(x);
             dy[c].get(g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                d[i] = r * fmaf(g[i], w[c][i], -x[i] * inner);
-                dw[c][i] = fmaf(g[i], x[i] * r, dw[c][i]);
+            for (int i = 0; i < 4; ++i) {
+                d[i] = root * fma(g[i], w[c][i], x[i] * inner);
+                dw[c][i] = fma(g[i], x[i] * root, dw[c][i]);
             }
             if (a.residual) {
                 more[c].get(x);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] += x[i];
+                for (int i = 0; i < 4; ++i) d[i] = d[i] + x[i];
             }
-            Chunk<T, VEC>::store((T *)a.diff_src + t * a.diff_src_ld, chunk_column<VEC>(c * THREADS + thread), a.cols, d);
+            Chunk<T, VEC>::store((T *)a.diff_src + t * a.diff_src_ld, chunk_column<VEC>(c * THREADS + thread), cols, d);
         }
     }
-    asm volatile("griddepcontrol.launch_dependents;"); // nothing is read any more
     if (!a.parts) return;
     if constexpr (THREADS == 32) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) Chunk<float, VEC>::store(gathered + team * a.cols, chunk_column<VEC>(c * 32 + thread), a.cols, dw[c]);
+        for (int c = 0; c < CHUNKS; ++c) Chunk<float, VEC>::store(gathered + team * cols, chunk_column<VEC>(c * 32 + thread), cols, dw[c]);
         __syncthreads();
         for (int col = threadIdx.x; col < (int)a.cols; col += 256) {
             float sum = 0.f;
@@ -374,7 +457,7 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
     } else {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
-            Chunk<float, VEC>::store(a.parts + blockIdx.x * a.cols, chunk_column<VEC>(c * THREADS + thread), a.cols, dw[c]);
+            Chunk<float, VEC>::store(a.parts + blockIdx.x * a.cols, chunk_column<VEC>(c * THREADS + thread), cols, dw[c]);
     }
 }
 
@@ -400,26 +483,38 @@ __global__ void __launch_bounds__(1024) rms_norm_weights_kernel(const __grid_con
     }
 }
 
-template <typename T, bool VEC, int THREADS, int CHUNKS> int launch_shape(NormArgs &a, bool backward, int sm_count, cudaStream_t st) {
+template <typename T, bool VEC, int THREADS, int CHUNKS> int launch_forward(const NormArgs &a, int sm_count, cudaStream_t st) {
     const int64_t ctas = (a.rows + TEAMS<THREADS> - 1) / TEAMS<THREADS>;
-    if (!backward)
-        return launch_dependent(rms_norm_kernel<T, VEC, THREADS, CHUNKS>, a, (unsigned)std::min<int64_t>(ctas, sm_count * FORWARD_CTAS<T, VEC, THREADS>),
-                BLOCK<THREADS>, 0, st);
+    return launch_dependent(rms_norm_kernel<T, VEC, THREADS, CHUNKS>, a,
+            (unsigned)std::min<int64_t>(ctas, sm_count * FORWARD_CTAS<T, VEC, THREADS, CHUNKS>), BLOCK<THREADS>, 0, st);
+}
+template <typename T, bool VEC, int THREADS, int CHUNKS> int launch_backward(NormArgs &a, int sm_count, cudaStream_t st) {
+    const int64_t ctas = (a.rows + TEAMS<THREADS> - 1) / TEAMS<THREADS>;
     // a part of the weights' gradient for each CTA: four rows at least, unless the SMs are too many
     a.part_count = (int)std::min<int64_t>(std::min<int64_t>(ctas, std::max<int64_t>(ctas / 4, sm_count)), sm_count * norm_gradient_ctas(a.cols));
     return launch_dependent(rms_norm_backward_kernel<T, VEC, THREADS, CHUNKS>, a, a.part_count, BLOCK<THREADS>,
             THREADS == 32 ? 8 * a.cols * sizeof(float) : 0, st);
 }
-// Threads of a row and its chunks of eight columns each: two chunks keep enough loads in flight, more where a CTA has no more threads.
+// Threads of a row and its chunks of eight columns each: two chunks keep enough loads in flight; more where the row needs them
 template <typename T, bool VEC> int launch_form(NormArgs &a, bool backward, int sm_count, cudaStream_t st) {
     const int64_t chunks = VEC ? (a.cols + 7) / 8 : (a.cols + 255) / 256 * 32;
-    if (chunks <= 32) return launch_shape<T, VEC, 32, 1>(a, backward, sm_count, st);
-    if (chunks <= 64) return launch_shape<T, VEC, 32, 2>(a, backward, sm_count, st);
-    if (chunks <= 128) return launch_shape<T, VEC, 64, 2>(a, backward, sm_count, st);
-    if (chunks <= 256) return launch_shape<T, VEC, 128, 2>(a, backward, sm_count, st);
-    if (chunks <= 512) return launch_shape<T, VEC, 256, 2>(a, backward, sm_count, st);
-    if (chunks <= 1024) return launch_shape<T, VEC, 512, 2>(a, backward, sm_count, st);
-    return launch_shape<T, VEC, 512, 4>(a, backward, sm_count, st);
+    if (backward) {
+        if (chunks <= 32) return launch_backward<T, VEC, 32, 1>(a, sm_count, st);
+        if (chunks <= 64) return launch_backward<T, VEC, 32, 2>(a, sm_count, st);
+        if (chunks <= 128) return launch_backward<T, VEC, 64, 2>(a, sm_count, st);
+        if (chunks <= 256) return launch_backward<T, VEC, 128, 2>(a, sm_count, st);
+        if (chunks <= 512) return launch_backward<T, VEC, 256, 2>(a, sm_count, st);
+        if (chunks <= 1024) return launch_backward<T, VEC, 512, 2>(a, sm_count, st);
+        return launch_backward<T, VEC, 512, 4>(a, sm_count, st);
+    }
+    if (chunks <= 32) return launch_forward<T, VEC, 32, 1>(a, sm_count, st);
+    if (chunks <= 64) return launch_forward<T, VEC, 32, 2>(a, sm_count, st);
+    if (chunks <= 128) return launch_forward<T, VEC, 64, 2>(a, sm_count, st);
+    if (chunks <= 256) return launch_forward<T, VEC, 128, 2>(a, sm_count, st);
+    if (chunks <= 512) return launch_forward<T, VEC, 256, 2>(a, sm_count, st);
+    if (chunks <= 768) return launch_forward<T, VEC, 256, 3>(a, sm_count, st);
+    if (chunks <= 1024) return launch_forward<T, VEC, 256, 4>(a, sm_count, st);
+    return launch_forward<T, VEC, 512, 4>(a, sm_count, st);
 }
 
 template <typename T> int launch_typed(NormArgs a, bool backward, int sm_count, cudaStream_t st) {

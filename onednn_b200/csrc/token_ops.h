@@ -33,6 +33,7 @@ struct RouteArgs {
     // forward: what the choice goes by besides the scores
     const float *bias; // [experts], may be null
     int groups, groups_kept, group_best;
+    int aligned_bias; // the launcher's
 };
 int launch_route_groups(const RouteArgs &a, cudaStream_t st); // with a bias or groups
 int launch_route(const RouteArgs &a, cudaStream_t st);
