@@ -35,79 +35,140 @@ __host__ __device__ inline int group_lanes(int groups) {
 // 32 + 5 roundings, the exponential and the quotient are as above.
 __device__ __forceinline__ float score_error(int scoring) { return scoring == SCORING_SIGMOID ? 0x1p-21f : 0x1p-16f; }
 
+// exp(x), x <= 0, in 64 bits without a branch, so that several run at once: x = n log 2 + r with log 2 in two parts of which the
+// first has zeros enough that its product with n is exact (Cody and Waite: Software manual for the elementary functions; 1980),
+// the series of exp(r) up to r^13 / 13! (what follows is below 2^-57), and n into the exponent; 0 below the least normal number.
+__device__ __forceinline__ double exp_64(double x) {
+    const double n = rint(x * 1.4426950408889634);
+    const double r = fma(-n, 0x1.a39ef35793c76p-33, fma(-n, 0x1.62e42feep-1, x));
+    const double r2 = r * r, r4 = r2 * r2;
+    const double a = fma(r, 1. / 6, 1. / 2), b = fma(r, 1. / 120, 1. / 24), c = fma(r, 1. / 5040, 1. / 720), d = fma(r, 1. / 362880, 1. / 40320);
+    const double e = fma(r, 1. / 39916800, 1. / 3628800), f = fma(r, 1. / 6227020800, 1. / 479001600);
+    const double high = fma(r4, fma(r2, f, e), fma(r2, d, c)); // from r^6 on
+    const double sum = 1. + (r + r2 * fma(r4, high, fma(r2, b, a)));
+    const int k = n > -1023. ? (int)n : -1023;
+    return k > -1023 ? sum * __hiloint2double((k + 1023) << 20, 0) : 0.;
+}
+// 1 / d, 1 <= d <= 2: Newton's steps on the 32-bit reciprocal
+__device__ __forceinline__ double inverse_64(double d) {
+    double r = __frcp_rn((float)d);
+    r = fma(r, fma(-d, r, 1.), r);
+    return fma(r, fma(-d, r, 1.), r);
+}
+// bits in the order of the values, as order_key; 0 for -inf
+__device__ __forceinline__ uint64_t order_key_64(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.);
+    return v > -INFINITY ? u >> 63 ? ~u : u | 1ull << 63 : 0;
+}
+
 // The k choices of a row in 64 bits.  values: [experts] of this warp's own.  Lane j returns choice j, -1 without one.
 template <typename T>
 __device__ __noinline__ int choose_in_64_bits(const RouteArgs &a, const T *row, double *values) {
     const int lane = threadIdx.x & 31;
-    const double none = -__longlong_as_double(0x7ff0000000000000ll);
-    double top = none, sum = 0;
+    constexpr double none = -INFINITY;
+    float top = none;
+    double total = 0, inverse = 1;
+    auto logit = [&](int e, bool &there) {
+        const float l = e < a.experts ? to_f32(row[e]) : none;
+        there = l > none;
+        return there ? fminf(l, LARGEST<T>) : 0.f;
+    };
+    bool there[4];
+    float l[4];
     if (a.scoring == SCORING_SOFTMAX) {
         for (int e = lane; e < a.experts; e += 32) {
-            const uint32_t k = order_key(to_f32(row[e]));
-            if (k) top = fmax(top, (double)key_value<T>(k));
+            const float v = logit(e, there[0]);
+            if (there[0]) top = fmaxf(top, v);
+        }
+        top = warp_max(top);
+        for (int e0 = lane; e0 < a.experts; e0 += 128) {
+            double v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[i] = logit(e0 + 32 * i, there[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = exp_64(there[i] ? (double)l[i] - top : 0.);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total += there[i] ? v[i] : 0.;
         }
 #pragma unroll
-        for (int s = 16; s > 0; s /= 2) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, s));
-        for (int e = lane; e < a.experts; e += 32) {
-            const uint32_t k = order_key(to_f32(row[e]));
-            if (k) sum += exp((double)key_value<T>(k) - top);
-        }
-#pragma unroll
-        for (int s = 16; s > 0; s /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        for (int s = 16; s > 0; s /= 2) total += __shfl_xor_sync(0xffffffffu, total, s);
+        inverse = 1. / total; // (unused where every expert is masked)
     }
     __syncwarp(); // (the groups' 32-bit values lay here)
-    for (int e = lane; e < a.experts; e += 32) {
-        const uint32_t k = order_key(to_f32(row[e])), b = a.bias ? order_key(a.bias[e]) : 1u;
-        double c = none;
-        if (k && b) {
-            const double l = key_value<T>(k);
-            c = a.scoring == SCORING_SIGMOID ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / sum;
-            if (a.bias) c += (double)key_value<float>(b);
+    for (int e0 = lane; e0 < a.experts; e0 += 128) {
+        double v[4];
+        float b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            l[i] = logit(e0 + 32 * i, there[i]);
+            b[i] = a.bias && e0 + 32 * i < a.experts ? a.bias[e0 + 32 * i] : 0.f;
         }
-        values[e] = c;
+        if (a.scoring == SCORING_SIGMOID) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const double x = exp_64(-fabs((double)l[i])), r = inverse_64(1. + x);
+                v[i] = l[i] < 0.f ? x * r : r;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = exp_64(there[i] ? (double)l[i] - top : 0.) * inverse;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (e0 + 32 * i < a.experts)
+                values[e0 + 32 * i] = there[i] && b[i] > none ? v[i] + (double)fminf(b[i], LARGEST<float>) : none;
     }
     __syncwarp();
-    const int size = a.experts / a.groups;
+    const int size = a.experts / a.groups, lanes = group_lanes(a.groups);
     if (a.groups_kept < a.groups) {
-        double first = none, second = none; // of group `lane`
-        if (lane < a.groups)
-            for (int i = 0; i < size; ++i) {
-                const double c = values[lane * size + i];
+        double first = none, second = none;
+        const int group = lane / lanes;
+        if (group < a.groups)
+            for (int i = lane % lanes; i < size; i += lanes) {
+                const double c = values[group * size + i];
                 second = fmax(second, fmin(first, c));
                 first = fmax(first, c);
             }
+        for (int s = 1; s < lanes; s *= 2) {
+            const double f = __shfl_xor_sync(0xffffffffu, first, s), n = __shfl_xor_sync(0xffffffffu, second, s);
+            second = fmax(fmin(first, f), fmax(second, n));
+            first = fmax(first, f);
+        }
         const double rank = first == none ? none : a.group_best == 2 && second != none ? first + second : first;
         int better = 0;
         for (int g = 0; g < a.groups; ++g) {
-            const double other = __shfl_sync(0xffffffffu, rank, g);
-            better += other > rank || (other == rank && g < lane);
+            const double other = __shfl_sync(0xffffffffu, rank, g * lanes);
+            better += other > rank || (other == rank && g < group);
         }
-        if (lane < a.groups && better >= a.groups_kept)
-            for (int i = 0; i < size; ++i) values[lane * size + i] = none;
+        __syncwarp();
+        if (group < a.groups && better >= a.groups_kept)
+            for (int i = lane % lanes; i < size; i += lanes) values[group * size + i] = none;
         __syncwarp();
     }
-    int mine = -1;
-    for (int j = 0; j < a.choices; ++j) {
-        double best = none;
-        int at = a.experts;
-        for (int e = lane; e < a.experts; e += 32)
-            if (values[e] > best) {
-                best = values[e];
+    uint64_t best = 0; // the lane's, and its expert
+    int at = 0, mine = -1;
+    auto look = [&] {
+        best = 0;
+        for (int e = lane; e < a.experts; e += 32) {
+            const uint64_t k = order_key_64(values[e]);
+            if (k > best) {
+                best = k;
                 at = e;
             }
-#pragma unroll
-        for (int s = 16; s > 0; s /= 2) {
-            const double other = __shfl_xor_sync(0xffffffffu, best, s);
-            const int other_at = __shfl_xor_sync(0xffffffffu, at, s);
-            if (other > best || (other == best && other_at < at)) {
-                best = other;
-                at = other_at;
-            }
         }
-        if (best == none) break;
-        if (lane == j) mine = at;
-        if (at % 32 == lane) values[at] = none;
-        __syncwarp();
+    };
+    look();
+    for (int j = 0; j < a.choices; ++j) {
+        const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+        if (high == 0) break;
+        const bool leads = (uint32_t)(best >> 32) == high;
+        const uint32_t low = __reduce_max_sync(0xffffffffu, leads ? (uint32_t)best : 0u);
+        const int e = __reduce_min_sync(0xffffffffu, leads && (uint32_t)best == low ? at : a.experts);
+        if (lane == j) mine = e;
+        if (e % 32 == lane) {
+            values[e] = none;
+            look();
+        }
     }
     return mine;
 }

@@ -143,7 +143,7 @@ __device__ __forceinline__ void load_weights(const NormArgs &a, int col, Pair (&
     }
 }
 
-template <bool VEC> __device__ __forceinline__ void store_8bit(const NormArgs &a, int64_t t, int col, const Pair (&p)[4]) {
+template <bool VEC> __device__ __forceinline__ void store_8bit(const NormArgs &a, uint32_t t, int col, const Pair (&p)[4]) {
     uint8_t *row = (uint8_t *)a.dst + t * a.dst_ld;
     const int cols = (int)a.cols;
     if (col >= cols) return;
@@ -229,49 +229,69 @@ __device__ __forceinline__ float largest(const Pair (&v)[4]) { // magnitude, or 
 
 // h w to 8 bits by the scales of its groups, and the scales.  Groups of 16 to 256 columns, a power of two: in a warp's 256 columns
 // they are whole lanes' (VEC), or one to eight times 32 columns of all lanes, or half of them.
-template <bool VEC>
-__device__ __forceinline__ void scale_groups(const NormArgs &a, float *scales, int col, float r, float limit, float reciprocal, Pair (&v)[4]) {
+template <bool VEC, int THREADS, int CHUNKS>
+__device__ __forceinline__ void scale_groups(const NormArgs &a, float *scales, int thread, float r, float limit, float reciprocal, Pair (&v)[CHUNKS][4]) {
     const int shift = 31 - __clz(a.group), cols = (int)a.cols;
     if constexpr (VEC) {
-        uint32_t m = __float_as_uint(largest(v)) & 0x7fffffffu;
-        for (int s = 1; s < a.group / 8; s *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
-        float factor;
-        const float s = make_scale(m, r, limit, reciprocal, factor);
-        if (col < cols && (col & (a.group - 1)) == 0) scales[col >> shift] = s;
+        uint32_t m[CHUNKS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = v[i] * both(factor);
+        for (int c = 0; c < CHUNKS; ++c) m[c] = __float_as_uint(largest(v[c])) & 0x7fffffffu;
+#pragma unroll
+        for (int s = 1; s < 32; s *= 2)
+            if (8 * s < a.group)
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) m[c] = max(m[c], __shfl_xor_sync(0xffffffffu, m[c], s));
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int col = chunk_column<VEC>(c * THREADS + thread);
+            float factor;
+            const float s = make_scale(m[c], r, limit, reciprocal, factor);
+            if (col < cols && (col & (a.group - 1)) == 0) scales[col >> shift] = s;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] * both(factor);
+        }
     } else {
-        float each[8], factor[8];
-        uint32_t m[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split(v[i], each[2 * i], each[2 * i + 1]);
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int col = chunk_column<VEC>(c * THREADS + thread);
+            float each[8], factor[8];
+            uint32_t m[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m[i] = __float_as_uint(each[i]) & 0x7fffffffu;
-            if (a.group == 16) {
+            for (int i = 0; i < 4; ++i) split(v[c][i], each[2 * i], each[2 * i + 1]);
 #pragma unroll
-                for (int s = 1; s < 16; s *= 2) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], s));
-            } else {
-                m[i] = __reduce_max_sync(0xffffffffu, m[i]);
-            }
-        }
+            for (int i = 0; i < 8; ++i) {
+                m[i] = __float_as_uint(each[i]) & 0x7fffffffu;
+                if (a.group == 16) {
 #pragma unroll
-        for (int step = 1; step < 8; step *= 2) // (pairs, fours, all eight of the 32 columns)
-            if (a.group > 32 * step) {
-                uint32_t other[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) other[i] = m[i ^ step];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) m[i] = max(m[i], other[i]);
+                    for (int s = 1; s < 16; s *= 2) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], s));
+                } else {
+                    m[i] = __reduce_max_sync(0xffffffffu, m[i]);
+                }
             }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float s = make_scale(m[i], r, limit, reciprocal, factor[i]);
-            if (col + 32 * i < cols && ((col + 32 * i) & (a.group - 1)) == 0) scales[(col + 32 * i) >> shift] = s;
-        }
+            for (int step = 1; step < 8; step *= 2) // (pairs, fours, all eight of the 32 columns)
+                if (a.group > 32 * step) {
+                    uint32_t other[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = pair(each[2 * i] * factor[2 * i], each[2 * i + 1] * factor[2 * i + 1]);
+                    for (int i = 0; i < 8; ++i) other[i] = m[i ^ step];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) m[i] = max(m[i], other[i]);
+                }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float s = make_scale(m[i], r, limit, reciprocal, factor[i]);
+                if (col + 32 * i < cols && ((col + 32 * i) & (a.group - 1)) == 0) scales[(col + 32 * i) >> shift] = s;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[c][i] = pair(each[2 * i] * factor[2 * i], each[2 * i + 1] * factor[2 * i + 1]);
+        }
     }
+}
+
+template <typename D, bool VEC, int THREADS, int CHUNKS>
+__device__ __forceinline__ void store_row(D *row, int thread, int cols, const Pair (&v)[CHUNKS][4]) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) Chunk<D, VEC>::store(row, chunk_column<VEC>(c * THREADS + thread), cols, v[c]);
 }
 
 // A CTA's threads, the rows that they work on at the same time, and the CTAs of an SM that registers are cut to.
@@ -291,10 +311,10 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
     __shared__ uint32_t most[2][32];
     ptx::grid_dependency_wait();
     const int thread = threadIdx.x % THREADS, cols = (int)a.cols;
-    const int64_t step = (int64_t)gridDim.x * TEAMS<THREADS>;
-    int64_t t = (int64_t)blockIdx.x * TEAMS<THREADS> + (THREADS == 32 ? threadIdx.x / 32 : 0);
+    const uint32_t step = gridDim.x * TEAMS<THREADS>, rows = (uint32_t)a.rows; // (below 2^31)
+    uint32_t t = blockIdx.x * TEAMS<THREADS> + (THREADS == 32 ? threadIdx.x / 32 : 0);
     Chunk<T, VEC> x[CHUNKS], r[CHUNKS];
-    auto load = [&](int64_t row) {
+    auto load = [&](uint32_t row) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = chunk_column<VEC>(c * THREADS + thread);
@@ -302,14 +322,14 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
             if (a.residual) r[c].load((const T *)a.residual + row * a.residual_ld, col, cols);
         }
     };
-    if (FORWARD_AHEAD<T, VEC, THREADS, CHUNKS> && t < a.rows) load(t);
+    if (FORWARD_AHEAD<T, VEC, THREADS, CHUNKS> && t < rows) load(t);
     Pair w[CHUNKS][4];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) load_weights<T, VEC>(a, chunk_column<VEC>(c * THREADS + thread), w[c]);
     const float given = a.scaling == NORM_SCALE_GIVEN ? 1.f / ptx::ld_dependent(a.scales) : 1.f;
     const float limit = a.dst_dt == DT_S8 ? 127.f : 448.f, reciprocal = a.dst_dt == DT_S8 ? 1.f / 127.f : 1.f / 448.f;
     const float per_column = 1.f / (float)cols;
-    for (int turn = 0; t < a.rows; t += step, turn ^= 1) {
+    for (int turn = 0; t < rows; t += step, turn ^= 1) {
         if (!FORWARD_AHEAD<T, VEC, THREADS, CHUNKS>) load(t);
         Pair h[CHUNKS][4], squares = both(0.f);
 #pragma unroll
@@ -324,11 +344,8 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) squares = fma(h[c][i], h[c][i], squares);
         }
-        if (FORWARD_AHEAD<T, VEC, THREADS, CHUNKS> && t + step < a.rows) load(t + step);
-        if (a.sum) {
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) Chunk<T, VEC>::store((T *)a.sum + t * a.sum_ld, chunk_column<VEC>(c * THREADS + thread), cols, h[c]);
-        }
+        if (FORWARD_AHEAD<T, VEC, THREADS, CHUNKS> && t + step < rows) load(t + step);
+        if (a.sum) store_row<T, VEC, THREADS>((T *)a.sum + t * a.sum_ld, thread, cols, h);
         float sum[2];
         split(squares, sum[0], sum[1]);
         float total[1] = {sum[0] + sum[1]};
@@ -346,20 +363,21 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
             const float s = make_scale(row_max<THREADS>(__float_as_uint(m) & 0x7fffffffu, most[turn]), root, limit, reciprocal, factor);
             if (thread == 0) a.scales[t] = s;
         }
+        if (a.scaling == NORM_SCALE_GROUP) {
+            scale_groups<VEC, THREADS>(a, a.scales + (int64_t)t * (cols / a.group), thread, root, limit, reciprocal, h);
+        } else {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int col = chunk_column<VEC>(c * THREADS + thread);
-            if (a.scaling == NORM_SCALE_GROUP) {
-                scale_groups<VEC>(a, a.scales + t * (cols / a.group), col, root, limit, reciprocal, h[c]);
-            } else {
+            for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] * both(factor);
-            }
-            switch (a.dst_dt) {
-                case DT_F32: Chunk<float, VEC>::store((float *)a.dst + t * a.dst_ld, col, cols, h[c]); break;
-                case DT_BF16: Chunk<__nv_bfloat16, VEC>::store((__nv_bfloat16 *)a.dst + t * a.dst_ld, col, cols, h[c]); break;
-                case DT_F16: Chunk<__half, VEC>::store((__half *)a.dst + t * a.dst_ld, col, cols, h[c]); break;
-                default: store_8bit<VEC>(a, t, col, h[c]);
+        }
+        switch (a.dst_dt) {
+            case DT_F32: store_row<float, VEC, THREADS>((float *)a.dst + t * a.dst_ld, thread, cols, h); break;
+            case DT_BF16: store_row<__nv_bfloat16, VEC, THREADS>((__nv_bfloat16 *)a.dst + t * a.dst_ld, thread, cols, h); break;
+            case DT_F16: store_row<__half, VEC, THREADS>((__half *)a.dst + t * a.dst_ld, thread, cols, h); break;
+            default: {
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) store_8bit<VEC>(a, t, chunk_column<VEC>(c * THREADS + thread), h[c]);
             }
         }
     }
@@ -374,10 +392,10 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
     ptx::grid_dependency_wait();
     const int thread = threadIdx.x % THREADS, team = THREADS == 32 ? threadIdx.x / 32 : 0, cols = (int)a.cols;
     const float per_column = 1.f / (float)cols;
-    const int64_t step = (int64_t)gridDim.x * TEAMS<THREADS>;
-    int64_t t = (int64_t)blockIdx.x * TEAMS<THREADS> + team;
+    const uint32_t step = gridDim.x * TEAMS<THREADS>, rows = (uint32_t)a.rows; // (below 2^31)
+    uint32_t t = blockIdx.x * TEAMS<THREADS> + team;
     Chunk<T, VEC> next_h[CHUNKS], next_dy[CHUNKS], next_more[CHUNKS];
-    auto load = [&](int64_t row) {
+    auto load = [&](uint32_t row) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = chunk_column<VEC>(c * THREADS + thread);
@@ -386,7 +404,7 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
             if (a.residual) next_more[c].load((const T *)a.residual + row * a.residual_ld, col, cols);
         }
     };
-    if (BACKWARD_AHEAD<T, CHUNKS> && t < a.rows) load(t);
+    if (BACKWARD_AHEAD<T, CHUNKS> && t < rows) load(t);
     asm volatile("griddepcontrol.launch_dependents;"); // all CTAs are resident; what comes next waits for their end
     Pair w[CHUNKS][4], dw[CHUNKS][4];
 #pragma unroll
@@ -395,7 +413,7 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
 #pragma unroll
         for (int i = 0; i < 4; ++i) dw[c][i] = both(0.f);
     }
-    for (int turn = 0; t < a.rows; t += step, turn ^= 1) {
+    for (int turn = 0; t < rows; t += step, turn ^= 1) {
         if (!BACKWARD_AHEAD<T, CHUNKS>) load(t);
         Chunk<T, VEC> h[CHUNKS], dy[CHUNKS], more[CHUNKS];
 #pragma unroll
@@ -404,7 +422,7 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
             dy[c] = next_dy[c];
             if (a.residual) more[c] = next_more[c];
         }
-        if (BACKWARD_AHEAD<T, CHUNKS> && t + step < a.rows) load(t + step);
+        if (BACKWARD_AHEAD<T, CHUNKS> && t + step < rows) load(t + step);
         Pair squares = both(0.f), products = both(0.f);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
@@ -509,9 +527,15 @@ template <typename T, bool VEC> int launch_form(NormArgs &a, bool backward, int 
     }
     if (chunks <= 32) return launch_forward<T, VEC, 32, 1>(a, sm_count, st);
     if (chunks <= 64) return launch_forward<T, VEC, 32, 2>(a, sm_count, st);
-    if (chunks <= 128) return launch_forward<T, VEC, 64, 2>(a, sm_count, st);
-    if (chunks <= 256) return launch_forward<T, VEC, 128, 2>(a, sm_count, st);
-    if (chunks <= 512) return launch_forward<T, VEC, 256, 2>(a, sm_count, st);
+    if constexpr (VEC && sizeof(T) == 2) {
+        if (chunks <= 128) return launch_forward<T, VEC, 32, 4>(a, sm_count, st);
+        if (chunks <= 256) return launch_forward<T, VEC, 64, 4>(a, sm_count, st);
+        if (chunks <= 512) return launch_forward<T, VEC, 128, 4>(a, sm_count, st);
+    } else {
+        if (chunks <= 128) return launch_forward<T, VEC, 64, 2>(a, sm_count, st);
+        if (chunks <= 256) return launch_forward<T, VEC, 128, 2>(a, sm_count, st);
+        if (chunks <= 512) return launch_forward<T, VEC, 256, 2>(a, sm_count, st);
+    }
     if (chunks <= 768) return launch_forward<T, VEC, 256, 3>(a, sm_count, st);
     if (chunks <= 1024) return launch_forward<T, VEC, 256, 4>(a, sm_count, st);
     return launch_forward<T, VEC, 512, 4>(a, sm_count, st);
