@@ -7,7 +7,7 @@
 //            softmax's sum; +inf counts as the largest finite value of its type
 // The choice is by the values of c in 64 bits.  32 bits say the same wherever the values that the choice falls between differ by
 // more than what rounding can have moved them (8192 x 256: all but some 0.5 % of the rows); only the other rows are
-// computed again in 64 bits, out of line.  So a warp keeps a row's c as 32-bit keys in registers, as moe_route.cu does, with the
+// looked at in 64 bits, out of line: their first candidates, or all experts where the groups are in doubt.  So a warp keeps a row's c as 32-bit keys in registers, as moe_route.cu does, with the
 // number of the value in the lane in the lowest bits: keys of a lane differ, and a redux and a ballot say which expert it is.
 // Groups are looked at by 32 / groups lanes each, from shared memory.
 #include <algorithm>
@@ -61,63 +61,72 @@ __device__ __forceinline__ uint64_t order_key_64(double v) {
     return v > -INFINITY ? u >> 63 ? ~u : u | 1ull << 63 : 0;
 }
 
+// What the 64-bit values of a row are made with: a softmax's largest logit and the inverse of its sum.
+struct Row64 { float top; double inverse; };
+template <typename T> __device__ __forceinline__ float logit_of(const RouteArgs &a, const T *row, int e, bool &there) {
+    const float l = e < a.experts ? to_f32(row[e]) : -INFINITY;
+    there = l > -INFINITY;
+    return there ? fminf(l, LARGEST<T>) : 0.f;
+}
+template <typename T> __device__ __forceinline__ Row64 row_in_64_bits(const RouteArgs &a, const T *row) {
+    Row64 r {-INFINITY, 1.};
+    if (a.scoring == SCORING_SIGMOID) return r;
+    const int lane = threadIdx.x & 31;
+    bool there;
+    for (int e = lane; e < a.experts; e += 32) {
+        const float l = logit_of<T>(a, row, e, there);
+        if (there) r.top = fmaxf(r.top, l);
+    }
+    r.top = warp_max(r.top);
+    double total = 0;
+    for (int e = lane; e < a.experts; e += 32) {
+        const float l = logit_of<T>(a, row, e, there);
+        const double v = exp_64(there ? (double)l - r.top : 0.);
+        total += there ? v : 0.;
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) total += __shfl_xor_sync(0xffffffffu, total, s);
+    r.inverse = 1. / total; // (unused where every expert is masked)
+    return r;
+}
+// c of an expert, -inf where it cannot be chosen
+template <typename T> __device__ __forceinline__ double value_in_64_bits(const RouteArgs &a, const T *row, const Row64 &r, int e) {
+    bool there;
+    const float l = logit_of<T>(a, row, e, there), b = a.bias && e < a.experts ? a.bias[e] : 0.f;
+    const bool sigmoid = a.scoring == SCORING_SIGMOID;
+    const double x = exp_64(there ? sigmoid ? -fabs((double)l) : (double)l - r.top : 0.);
+    const double scale = sigmoid ? inverse_64(1. + x) : r.inverse;
+    const double s = sigmoid && l >= 0.f ? scale : x * scale;
+    return there && b > -INFINITY ? s + (double)fminf(b, LARGEST<float>) : -INFINITY;
+}
+
+// Lane j of the first `count` has candidate j; returns, in lane j, the one that is j-th by the values in 64 bits, ties to the lowest index.
+template <typename T>
+__device__ __noinline__ int order_in_64_bits(const RouteArgs &a, const T *row, int candidate, int count) {
+    const int lane = threadIdx.x & 31;
+    const double c = value_in_64_bits<T>(a, row, row_in_64_bits<T>(a, row), lane < count ? candidate : a.experts);
+    int place = 0;
+    for (int j = 0; j < count; ++j) {
+        const double other = __shfl_sync(0xffffffffu, c, j);
+        const int at = __shfl_sync(0xffffffffu, candidate, j);
+        place += other > c || (other == c && at < candidate);
+    }
+    int result = -1;
+    for (int j = 0; j < count; ++j) {
+        const int to = __shfl_sync(0xffffffffu, place, j), e = __shfl_sync(0xffffffffu, candidate, j);
+        if (to == lane) result = e;
+    }
+    return result;
+}
+
 // The k choices of a row in 64 bits.  values: [experts] of this warp's own.  Lane j returns choice j, -1 without one.
 template <typename T>
 __device__ __noinline__ int choose_in_64_bits(const RouteArgs &a, const T *row, double *values) {
     const int lane = threadIdx.x & 31;
     constexpr double none = -INFINITY;
-    float top = none;
-    double total = 0, inverse = 1;
-    auto logit = [&](int e, bool &there) {
-        const float l = e < a.experts ? to_f32(row[e]) : none;
-        there = l > none;
-        return there ? fminf(l, LARGEST<T>) : 0.f;
-    };
-    bool there[4];
-    float l[4];
-    if (a.scoring == SCORING_SOFTMAX) {
-        for (int e = lane; e < a.experts; e += 32) {
-            const float v = logit(e, there[0]);
-            if (there[0]) top = fmaxf(top, v);
-        }
-        top = warp_max(top);
-        for (int e0 = lane; e0 < a.experts; e0 += 128) {
-            double v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) l[i] = logit(e0 + 32 * i, there[i]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = exp_64(there[i] ? (double)l[i] - top : 0.);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) total += there[i] ? v[i] : 0.;
-        }
-#pragma unroll
-        for (int s = 16; s > 0; s /= 2) total += __shfl_xor_sync(0xffffffffu, total, s);
-        inverse = 1. / total; // (unused where every expert is masked)
-    }
+    const Row64 r = row_in_64_bits<T>(a, row);
     __syncwarp(); // (the groups' 32-bit values lay here)
-    for (int e0 = lane; e0 < a.experts; e0 += 128) {
-        double v[4];
-        float b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            l[i] = logit(e0 + 32 * i, there[i]);
-            b[i] = a.bias && e0 + 32 * i < a.experts ? a.bias[e0 + 32 * i] : 0.f;
-        }
-        if (a.scoring == SCORING_SIGMOID) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const double x = exp_64(-fabs((double)l[i])), r = inverse_64(1. + x);
-                v[i] = l[i] < 0.f ? x * r : r;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = exp_64(there[i] ? (double)l[i] - top : 0.) * inverse;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (e0 + 32 * i < a.experts)
-                values[e0 + 32 * i] = there[i] && b[i] > none ? v[i] + (double)fminf(b[i], LARGEST<float>) : none;
-    }
+    for (int e = lane; e < a.experts; e += 32) values[e] = value_in_64_bits<T>(a, row, r, e);
     __syncwarp();
     const int size = a.experts / a.groups, lanes = group_lanes(a.groups);
     if (a.groups_kept < a.groups) {
@@ -330,31 +339,49 @@ __global__ void __launch_bounds__(WARPS * 32) route_groups_kernel(const __grid_c
         key[i] = key[i] ? (key[i] & ~SLOT) | (SLOT - i) : 0u;
         best = max(best, key[i]);
     }
-    uint32_t mine = 0, owner = 0, several = 0; // lane j: key and lane (as a bit) of choice j
-    for (int j = 0; j < a.choices && !close; ++j) {
+    // Choice after choice; equal keys belong to the same slot of several lanes, and the lowest lane has the lowest expert.
+    uint32_t mine = 0; // lane j: key of choice j
+    int index = -1; // and its expert
+    auto choose = [&](int j) {
         const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-        if (most == 0) break;
-        const uint32_t owners = __ballot_sync(0xffffffffu, best == most);
+        if (most == 0) return false;
+        const int owner = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
         if (lane == j) {
             mine = most;
-            owner = owners;
+            index = owner;
         }
-        several |= owners & (owners - 1);
-        best = next_below(key, most);
-    }
-    const int slot = (int)(SLOT - (mine & SLOT));
-    int index = mine ? expert_of(slot, __ffs(owner) - 1) : -1; // of choice `lane`
-    {
-        // The next key, of the first that is left out behind the last choice.  Keys differ from c by what the slot's bits hide
-        // (2^-23 of the value each), the sum's rounding and the score's error.
-        const uint32_t left_out = __reduce_max_sync(0xffffffffu, best), down = __shfl_down_sync(0xffffffffu, mine, 1);
-        const uint32_t after = lane == a.choices - 1 ? left_out : down;
+        const uint32_t next = next_below(key, most);
+        if (lane == owner) best = next;
+        return true;
+    };
+    int found = 0;
+    for (; found < a.choices && !close; ++found)
+        if (!choose(found)) break;
+    // Whether the next key, of the first that is left out behind the last choice, is so near that 32 bits do not tell.  Keys differ
+    // from c by what the slot's bits hide (2^-23 of the value each), the sum's rounding and the score's error.
+    uint32_t left_out = __reduce_max_sync(0xffffffffu, best);
+    auto near = [&] {
+        const uint32_t down = __shfl_down_sync(0xffffffffu, mine, 1), after = lane == found - 1 ? left_out : down;
         const float c = key_value<float>(mine & ~SLOT), n = key_value<float>(after & ~SLOT);
-        const bool near = lane < a.choices && mine && after
-                && !(c - n > 2.f * (score_error(a.scoring) + (PER_LANE + 1) * 0x1p-23f) * (fabsf(c) + most_bias));
-        close = close || several || __any_sync(0xffffffffu, near);
+        return lane < found && after && !(c - n > 2.f * (score_error(a.scoring) + (PER_LANE + 1) * 0x1p-23f) * (fabsf(c) + most_bias));
+    };
+    const bool tight = near();
+    const bool some = !close && __any_sync(0xffffffffu, tight);
+    if (some) { // a few more candidates, up to a gap that 32 bits do tell; in 64 bits their order is found
+        while (found < min(a.choices + 4, 32) && choose(found)) ++found;
+        left_out = __reduce_max_sync(0xffffffffu, best);
     }
-    if (close) index = choose_in_64_bits(a, row, own);
+    auto expert_at = [&] { return mine ? expert_of((int)(SLOT - (mine & SLOT)), index) : -1; };
+    index = expert_at();
+    if (some) {
+        const bool gap = !near(); // (by the whole warp)
+        const uint32_t gaps = __ballot_sync(0xffffffffu, lane < found && lane >= a.choices - 1 && gap);
+        if (found < a.choices) index = order_in_64_bits<T>(a, row, index, found); // (all there are)
+        else if (gaps) index = order_in_64_bits<T>(a, row, index, __ffs(gaps));
+        else close = true;
+    }
+    if (close) index = choose_in_64_bits<T>(a, row, own);
+    if (lane >= a.choices) index = -1;
     const bool chosen = index >= 0;
     const float l = chosen ? key_value<T>(order_key(to_f32(row[index]))) : 0.f;
     float w;

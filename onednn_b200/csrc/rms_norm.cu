@@ -527,7 +527,7 @@ template <typename T, bool VEC> int launch_form(NormArgs &a, bool backward, int 
     }
     if (chunks <= 32) return launch_forward<T, VEC, 32, 1>(a, sm_count, st);
     if (chunks <= 64) return launch_forward<T, VEC, 32, 2>(a, sm_count, st);
-    if constexpr (VEC && sizeof(T) == 2) {
+    if (VEC && sizeof(T) == 2 && !a.residual) {
         if (chunks <= 128) return launch_forward<T, VEC, 32, 4>(a, sm_count, st);
         if (chunks <= 256) return launch_forward<T, VEC, 64, 4>(a, sm_count, st);
         if (chunks <= 512) return launch_forward<T, VEC, 128, 4>(a, sm_count, st);
