@@ -167,9 +167,13 @@ template <bool VEC> __device__ __forceinline__ void store_8bit(const NormArgs &a
     }
 }
 
-// Sum (of one or two numbers), or largest of unsigned bits, over the threads that share a row.  `buffer`: 64 words of shared
-// memory that nothing else uses until the next barrier but one.
-template <int THREADS, int N> __device__ __forceinline__ void row_sum(float (&v)[N], float *buffer) {
+// Sum (of one or two numbers), or largest of unsigned bits, over the threads that share a row: a CTA, or a part of one that has a
+// barrier of its own (TEAMS).  `buffer`: 64 words of shared memory that nothing else uses until the next barrier but one.
+template <int THREADS, int TEAMS> __device__ __forceinline__ void row_barrier() {
+    if constexpr (TEAMS == 1) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.x / THREADS + 1), "n"(THREADS) : "memory");
+}
+template <int THREADS, int TEAMS, int N> __device__ __forceinline__ void row_sum(float (&v)[N], float *buffer) {
 #pragma unroll
     for (int s = 16; s > 0; s /= 2)
 #pragma unroll
@@ -178,8 +182,8 @@ template <int THREADS, int N> __device__ __forceinline__ void row_sum(float (&v)
         const int lane = threadIdx.x & 31;
         if (lane == 0)
 #pragma unroll
-            for (int n = 0; n < N; ++n) buffer[n * 32 + threadIdx.x / 32] = v[n];
-        __syncthreads();
+            for (int n = 0; n < N; ++n) buffer[n * 32 + threadIdx.x % THREADS / 32] = v[n];
+        row_barrier<THREADS, TEAMS>();
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             v[n] = lane < THREADS / 32 ? buffer[n * 32 + lane] : 0.f;
@@ -294,12 +298,15 @@ __device__ __forceinline__ void store_row(D *row, int thread, int cols, const Pa
     for (int c = 0; c < CHUNKS; ++c) Chunk<D, VEC>::store(row, chunk_column<VEC>(c * THREADS + thread), cols, v[c]);
 }
 
-// A CTA's threads, the rows that they work on at the same time, and the CTAs of an SM that registers are cut to.
+// A CTA's threads, the rows that they work on at the same time, and the CTAs of an SM that registers are cut to.  (The gradient's
+// CTAs have at least 256 threads, so that there are few parts of the weights' gradient.)
 template <int THREADS> constexpr int BLOCK = THREADS == 32 ? 256 : THREADS;
 template <int THREADS> constexpr int TEAMS = THREADS == 32 ? 8 : 1;
+template <int THREADS> constexpr int BACKWARD_BLOCK = THREADS < 256 ? 256 : THREADS;
+template <int THREADS> constexpr int BACKWARD_TEAMS = BACKWARD_BLOCK<THREADS> / THREADS;
 template <typename T, bool VEC, int THREADS, int CHUNKS>
 constexpr int FORWARD_CTAS = THREADS > 256 ? 1 : (VEC && sizeof(T) == 2 && CHUNKS <= 2 ? 768 : 512) / BLOCK<THREADS>;
-template <int THREADS> constexpr int BACKWARD_CTAS = THREADS > 256 ? 1 : 512 / BLOCK<THREADS>;
+template <int THREADS> constexpr int BACKWARD_CTAS = 512 / BACKWARD_BLOCK<THREADS>;
 // whether registers hold a row that is on its way
 template <typename T, bool VEC, int THREADS, int CHUNKS> constexpr bool FORWARD_AHEAD = CHUNKS <= 2 || (VEC && sizeof(T) == 2 && THREADS <= 256);
 template <typename T, int CHUNKS> constexpr bool BACKWARD_AHEAD = CHUNKS * sizeof(T) <= 4;
@@ -349,7 +356,7 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
         float sum[2];
         split(squares, sum[0], sum[1]);
         float total[1] = {sum[0] + sum[1]};
-        row_sum<THREADS>(total, sums[turn]);
+        row_sum<THREADS, 1>(total, sums[turn]);
         const float root = inverse_root(fmaf(total[0], per_column, a.epsilon));
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
@@ -386,14 +393,15 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
 // Gradient: CTAs that stay take rows in turn; the weights and this CTA's part of their gradient stay in registers, and the
 // parts of all CTAs meet in the scratchpad, which the kernel behind this one adds up, in the same order every time.
 template <typename T, bool VEC, int THREADS, int CHUNKS>
-__global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_norm_backward_kernel(const __grid_constant__ NormArgs a) {
-    extern __shared__ float gathered[]; // a warp a row: [8][columns]
-    __shared__ float sums[2][64];
+__global__ void __launch_bounds__(BACKWARD_BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_norm_backward_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int ROWS = BACKWARD_TEAMS<THREADS>;
+    extern __shared__ float gathered[]; // several rows at a time: [ROWS][columns]
+    __shared__ float sums[2][ROWS][64];
     ptx::grid_dependency_wait();
-    const int thread = threadIdx.x % THREADS, team = THREADS == 32 ? threadIdx.x / 32 : 0, cols = (int)a.cols;
+    const int thread = threadIdx.x % THREADS, team = threadIdx.x / THREADS, cols = (int)a.cols;
     const float per_column = 1.f / (float)cols;
-    const uint32_t step = gridDim.x * TEAMS<THREADS>, rows = (uint32_t)a.rows; // (below 2^31)
-    uint32_t t = blockIdx.x * TEAMS<THREADS> + team;
+    const uint32_t step = gridDim.x * ROWS, rows = (uint32_t)a.rows; // (below 2^31)
+    uint32_t t = blockIdx.x * ROWS + team;
     Chunk<T, VEC> next_h[CHUNKS], next_dy[CHUNKS], next_more[CHUNKS];
     auto load = [&](uint32_t row) {
 #pragma unroll
@@ -440,7 +448,7 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
         split(products, s[1], odd[1]);
         s[0] += odd[0];
         s[1] += odd[1];
-        row_sum<THREADS>(s, sums[turn]);
+        row_sum<THREADS, ROWS>(s, sums[turn][team]);
         const float r = inverse_root(fmaf(s[0], per_column, a.epsilon));
         const Pair root = both(r), inner = both(-(s[1] * per_column * r * r)); // dh = r (z - h inner)
 #pragma unroll
@@ -462,14 +470,14 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_no
         }
     }
     if (!a.parts) return;
-    if constexpr (THREADS == 32) {
+    if constexpr (ROWS > 1) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) Chunk<float, VEC>::store(gathered + team * cols, chunk_column<VEC>(c * 32 + thread), cols, dw[c]);
+        for (int c = 0; c < CHUNKS; ++c) Chunk<float, VEC>::store(gathered + team * cols, chunk_column<VEC>(c * THREADS + thread), cols, dw[c]);
         __syncthreads();
-        for (int col = threadIdx.x; col < (int)a.cols; col += 256) {
+        for (int col = threadIdx.x; col < cols; col += 256) {
             float sum = 0.f;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) sum += gathered[q * a.cols + col];
+            for (int q = 0; q < ROWS; ++q) sum += gathered[q * cols + col];
             a.parts[blockIdx.x * a.cols + col] = sum;
         }
     } else {
@@ -487,7 +495,13 @@ __global__ void __launch_bounds__(1024) rms_norm_weights_kernel(const __grid_con
     const int64_t col = (int64_t)blockIdx.x * 32 + lane;
     float sum = 0.f;
     if (col < a.cols)
-        for (int p = warp; p < a.part_count; p += 32) sum += ptx::ld_dependent(a.parts + p * a.cols + col);
+        for (int p0 = warp; p0 < a.part_count; p0 += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = p0 + 32 * i < a.part_count ? ptx::ld_dependent(a.parts + (p0 + 32 * i) * a.cols + col) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += v[i];
+        }
     sums[warp][lane] = sum;
     __syncthreads();
     sum = sums[lane][warp];
@@ -507,11 +521,11 @@ template <typename T, bool VEC, int THREADS, int CHUNKS> int launch_forward(cons
             (unsigned)std::min<int64_t>(ctas, sm_count * FORWARD_CTAS<T, VEC, THREADS, CHUNKS>), BLOCK<THREADS>, 0, st);
 }
 template <typename T, bool VEC, int THREADS, int CHUNKS> int launch_backward(NormArgs &a, int sm_count, cudaStream_t st) {
-    const int64_t ctas = (a.rows + TEAMS<THREADS> - 1) / TEAMS<THREADS>;
+    const int64_t ctas = (a.rows + BACKWARD_TEAMS<THREADS> - 1) / BACKWARD_TEAMS<THREADS>;
     // a part of the weights' gradient for each CTA: four rows at least, unless the SMs are too many
-    a.part_count = (int)std::min<int64_t>(std::min<int64_t>(ctas, std::max<int64_t>(ctas / 4, sm_count)), sm_count * norm_gradient_ctas(a.cols));
-    return launch_dependent(rms_norm_backward_kernel<T, VEC, THREADS, CHUNKS>, a, a.part_count, BLOCK<THREADS>,
-            THREADS == 32 ? 8 * a.cols * sizeof(float) : 0, st);
+    a.part_count = (int)std::min<int64_t>(std::min<int64_t>(ctas, std::max<int64_t>(ctas / 4, sm_count)), sm_count * BACKWARD_CTAS<THREADS>);
+    return launch_dependent(rms_norm_backward_kernel<T, VEC, THREADS, CHUNKS>, a, a.part_count, BACKWARD_BLOCK<THREADS>,
+            BACKWARD_TEAMS<THREADS> > 1 ? BACKWARD_TEAMS<THREADS> * a.cols * sizeof(float) : 0, st);
 }
 // Threads of a row and its chunks of eight columns each: two chunks keep enough loads in flight; more where the row needs them
 template <typename T, bool VEC> int launch_form(NormArgs &a, bool backward, int sm_count, cudaStream_t st) {
@@ -572,9 +586,8 @@ int launch_any(const NormArgs &a, bool backward, int sm_count, cudaStream_t st) 
 
 } // namespace
 
-// CTAs per SM of the gradient's kernel, each with a part of the weights' gradient
-int norm_gradient_ctas(int64_t cols) { return cols <= 512 ? 2 : cols <= 1024 ? 8 : cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1; }
-size_t norm_scratch_bytes(int64_t cols, int sm_count) { return (size_t)sm_count * norm_gradient_ctas(cols) * cols * sizeof(float); }
+// a part of the weights' gradient for each CTA: two an SM at most
+size_t norm_scratch_bytes(int64_t cols, int sm_count) { return (size_t)sm_count * 2 * cols * sizeof(float); }
 
 int launch_rms_norm(const NormArgs &a, int sm_count, cudaStream_t st) {
     if (a.rows == 0 || a.cols == 0) return 0;

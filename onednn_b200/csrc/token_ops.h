@@ -162,7 +162,6 @@ struct NormArgs {
 };
 int launch_rms_norm(const NormArgs &a, int sm_count, cudaStream_t st);
 int launch_rms_norm_backward(const NormArgs &a, int sm_count, cudaStream_t st);
-int norm_gradient_ctas(int64_t cols);
 size_t norm_scratch_bytes(int64_t cols, int sm_count);
 
 // Launches `kernel` as a programmatic dependent of whatever precedes it on the stream; the kernel reads and writes global
