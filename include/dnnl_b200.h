@@ -740,7 +740,7 @@ dnnl_status_t dnnl_cuda_interop_rms_norm_primitive_desc_create(dnnl_primitive_de
  * that of the residual alike; DIFF_WEIGHTS [H] (f32 or SRC's type; diff_weights_desc may be NULL), summed in the same order
  * every time.  DIFF_SRC may be the memory of DIFF_DST, SRC_2 or SRC.  Quantization of the output counts as the identity.
  *   With DIFF_WEIGHTS, H may not be open, and there is a scratchpad, which holds sums between its kernels: executions of one
- * primitive that overlap on the GPU need the user scratchpad mode and a buffer each, as moe_dispatch has it. */
+ * primitive that overlap on the GPU need the user scratchpad mode and a buffer each (16-byte aligned), as moe_dispatch has it. */
 dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
         const_dnnl_memory_desc_t diff_dst_desc, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t weights_desc,
         const_dnnl_memory_desc_t diff_sum_desc, const_dnnl_memory_desc_t diff_src_desc, const_dnnl_memory_desc_t diff_weights_desc,
@@ -756,6 +756,8 @@ dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_pri
  * any row pitch; T, K and N may be zero, and any dim open.  Rows in any order; a batch of prompts and single tokens of many requests
  * are the same call.  All sums are f32; the middle product is rounded to 17 bits (27 where DST is f32) before the second.  A row of
  * SRC with an infinity or a NaN gives infinities or NaN.
+ *   Calls of more than 512 rows (or of open T) have a scratchpad, which holds the middle product: executions of one primitive that
+ * overlap on the GPU need the user scratchpad mode and a buffer each (16-byte aligned), as moe_dispatch has it.
  *   The gradient of SRC is this primitive on the gradient of DST, with WEIGHTS_1 transposed as WEIGHTS and WEIGHTS as WEIGHTS_1 (their
  * strides say so), and the projection's own gradient as base. */
 dnnl_status_t dnnl_cuda_interop_low_rank_adapter_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,

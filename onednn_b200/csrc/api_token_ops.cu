@@ -532,6 +532,9 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
             if (got.data_type != dnnl_f32 || got.format_kind != dnnl_blocked || got.has_runtime_dims()
                     || got.nelems() < settled.find(scales)->nelems())
                 return dnnl_invalid_arguments;
+            dnnl_dim_t dense = 1;
+            for (int d = got.ndims - 1; d >= 0; dense *= got.dims[d--])
+                if (got.dims[d] > 1 && got.strides[d] != dense) return dnnl_invalid_arguments;
         }
         op = &settled;
     }
@@ -559,6 +562,7 @@ dnnl_status_t execute_token_op(const dnnl_primitive &primitive, dnnl_stream_t st
         dnnl_memory_t sp = find(DNNL_ARG_SCRATCHPAD);
         if (!sp || !sp->handles[0]) return dnnl_invalid_arguments;
         scratch = sp->handles[0];
+        if (pd.kind >= dnnl_cuda_interop_rms_norm && (uintptr_t)scratch % 16) return dnnl_invalid_arguments; // (wide accesses)
     }
     cudaSetDevice(pd.engine->device);
     cudaEvent_t ev0 = nullptr, ev1 = nullptr;

@@ -4,11 +4,17 @@
 // time); with ranks up to 128 there are 2 to 60 operations a byte, which mma.sync keeps up with.
 //
 // Rows are looked at in windows of 512; the rows of a window that share an adapter make tiles, wherever they stand.
-//   Few rows: one launch.  A cluster of CTAs takes a tile of up to 16 rows: each CTA multiplies its share of the src's columns with
+//   Up to 1024 rows (512 from a rank of 33 on): one launch.  A cluster of CTAs takes a tile of up to 16 rows: each CTA multiplies its share of the src's columns with
 //     the first factor, the sums of [rows][rank] meet in the CTAs' shared memory, and each CTA multiplies them with its share of
 //     the second factor's columns.  So a single row's weights are streamed by a whole cluster.
-//   Many rows: two launches.  A CTA takes a tile of 32 rows through the first product, and the sums go to the scratchpad (4 r bytes
-//     a row, which stay in L2); then a CTA takes 64 rows and a run of dst's columns through the second.  No CTA waits for another.
+//   More: two launches.  A CTA takes a tile of 32 rows through the first product, and the sums go to the scratchpad (4 r bytes
+//     a row, which stay in L2); then a CTA takes 64 rows and a run of dst's columns through the second.  No CTA waits for another;
+//     the second kernel starts as the first one's CTAs end, and finds its rows and asks for its first base and weights meanwhile
+//     (777 rows of 37 adapters 20.1 us without, 17.4 with).
+// Measured: 8192 rows, 4096 x 11008, rank 32, 16 adapters 112.7 us (3.9 TB/s); 61 rows of 64 adapters, 4096 x 4096, rank 16 8.9 us.  The
+// second product's kernel takes the same time without its MMAs: latency of 16 warps an SM (128 registers) bounds it.  Deeper
+// prefetch through shared memory (cp.async, three blocks a warp), 64 columns a warp and 256 contiguous bytes a row were slower or the same
+// (119, 169, 130 us at a rank of 32; 108, 102, 118 for 106 at 16).
 // Operands go from global memory to the registers of an MMA without shared memory: a lane reads 8 or 16 bytes, and which of the
 // summed (or of the output's) columns these are is decided alike for both operands, so any order serves.
 // The middle is a 32-bit sum.  The second product takes it as a sum of 16-bit parts, most significant first: two (what is left
@@ -454,6 +460,9 @@ template <int RB, int M> struct Slabs {
 
 template <typename T, typename D> constexpr int PARTS = sizeof(D) == 4 && std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
 
+// (unit, 1 / unit) of a row
+__device__ __forceinline__ float2 with_inverse(float unit) { return make_float2(unit, 1.f / unit); }
+
 // The second product's left operand, for a row of which this thread (of four, t = threadIdx.x % 4) has the middle's columns
 // rank_column(mode, s, t, 0..3): operand[part][group of rows][s][lane].  f16: returns the power of two it was divided by.
 template <typename T, int RB, int P>
@@ -497,21 +506,24 @@ __device__ __forceinline__ float make_operand(uint4 *operand, int groups, float 
     return unit;
 }
 
-// Second product of M groups of 16 rows, from the operand in shared memory, over the warp's blocks of 32 columns.  A block's
-// base and weights are asked for one block ahead where registers allow it (the weights up to a rank of 32); start() does so for
-// the first block, and may be called long before.
-template <typename T, typename D, int RB, bool VEC, int M> struct SecondProduct {
+// Second product of the tile's GROUPS groups of 16 rows, from the operand in shared memory.  A warp has M of them and works on 32
+// columns of dst at a time, every `stride` of these blocks; its rows' base is asked for one block ahead, the weights too where
+// registers allow it (a rank of up to 32).  start() asks for the first block's, and may be called long before.
+template <typename T, typename D, int RB, bool VEC, int M, int GROUPS> struct SecondProduct {
+    static constexpr bool AHEAD = RB <= 2;
     const LowRankPlan &p;
     const uint16_t *up; // of the lane, in the block that is asked for next
     uint32_t bases, dsts; // shared memory, of the lane's first row
-    int count, lane, end;
+    int count, lane, group, end, stride;
     uint32_t raw[8 * RB];
     Eight<D, VEC> base[M][2];
 
-    __device__ __forceinline__ SecondProduct(const LowRankPlan &p, const uint16_t *up, const Window<16 * M> &rows, int count, int lane, int first, int end)
-        : p(p), count(count), lane(lane), end(end) {
-        bases = ptx::smem_u32(rows.base + (lane >> 2));
-        dsts = ptx::smem_u32(rows.dst + (lane >> 2));
+    // group: the warp's first; blocks first, first + stride, ... below end
+    __device__ __forceinline__ SecondProduct(const LowRankPlan &p, const uint16_t *up, const Window<16 * GROUPS> &rows, int count, int lane,
+            int group, int first, int end, int stride)
+        : p(p), count(count), lane(lane), group(group), end(end), stride(stride) {
+        bases = ptx::smem_u32(rows.base + 16 * group + (lane >> 2));
+        dsts = ptx::smem_u32(rows.dst + 16 * group + (lane >> 2));
         this->up = up + (32 * first + 4 * (lane >> 2)) * p.a.up_out + rank_column<RB>(p.up_mode, 0, lane & 3, 0) * p.a.up_rank;
     }
     __device__ __forceinline__ void load_base(int m, int h, int col) {
@@ -519,7 +531,7 @@ template <typename T, typename D, int RB, bool VEC, int M> struct SecondProduct 
     }
     __device__ __forceinline__ void load_weights(int b) {
         load_up<RB, VEC>(raw, p, up, (int)p.a.out - 32 * b - 4 * (lane >> 2), lane);
-        up += 32 * WARPS * p.a.up_out;
+        up += 32 * stride * p.a.up_out;
     }
     __device__ __forceinline__ void start(int first) {
         if (first >= end) return;
@@ -528,40 +540,40 @@ template <typename T, typename D, int RB, bool VEC, int M> struct SecondProduct 
             for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if (16 * m < count) load_base(m, h, 32 * first + 8 * (lane & 3));
+                    if (16 * (group + m) < count) load_base(m, h, 32 * first + 8 * (lane & 3));
         }
         load_weights(first);
     }
-    __device__ __forceinline__ void run(int first, const uint4 *operand, const float *units) {
-        for (int b = first; b < end; b += WARPS) {
+    __device__ __forceinline__ void run(int first, const uint4 *operand, const float2 *units) {
+        for (int b = first; b < end; b += stride) {
             const int col = 32 * b + 8 * (lane & 3);
-            const bool more = b + WARPS < end;
+            const bool more = b + stride < end;
             uint32_t w[4][RB][2];
             order_up<RB>(w, raw, p);
-            if (RB <= 2 && more) load_weights(b + WARPS);
+            if (AHEAD && more) load_weights(b + stride);
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                if (16 * m >= count) break;
-                float out[4][4], unit[2] = {1.f, 1.f};
+                if (16 * (group + m) >= count) break;
+                float out[4][4];
+                float2 unit[2]; // (f16)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if constexpr (std::is_same<T, __half>::value) unit[h] = units[16 * m + 8 * h + (lane >> 2)];
+                    if constexpr (std::is_same<T, __half>::value) unit[h] = units[16 * (group + m) + 8 * h + (lane >> 2)];
                     float v[8] = {};
                     if (p.a.base) {
                         base[m][h].get(v);
-                        if (more) load_base(m, h, col + 32 * WARPS);
+                        if (more) load_base(m, h, col + 32 * stride);
                     }
-                    const float inverse = 1.f / unit[h];
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) out[j][2 * h + i] = std::is_same<T, __half>::value ? v[4 * i + j] * inverse : v[4 * i + j];
+                        for (int i = 0; i < 2; ++i) out[j][2 * h + i] = std::is_same<T, __half>::value ? v[4 * i + j] * unit[h].y : v[4 * i + j];
                 }
 #pragma unroll
                 for (int q = PARTS<T, D> - 1; q >= 0; --q) // the smallest first
 #pragma unroll
                     for (int s = 0; s < RB; ++s) {
-                        const uint4 f = operand[((q * M + m) * RB + s) * 32 + lane];
+                        const uint4 f = operand[((q * GROUPS + group + m) * RB + s) * 32 + lane];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) mma_16816<T>(out[j], f.x, f.y, f.z, f.w, w[j][s][0], w[j][s][1]);
                     }
@@ -571,12 +583,12 @@ template <typename T, typename D, int RB, bool VEC, int M> struct SecondProduct 
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) v[4 * i + j] = std::is_same<T, __half>::value ? out[j][2 * h + i] * unit[h] : out[j][2 * h + i];
-                    if (16 * m + 8 * h + (lane >> 2) < count)
+                        for (int i = 0; i < 2; ++i) v[4 * i + j] = std::is_same<T, __half>::value ? out[j][2 * h + i] * unit[h].x : out[j][2 * h + i];
+                    if (16 * (group + m) + 8 * h + (lane >> 2) < count)
                         Eight<D, VEC>::store(ld_address<D>(dsts + 8 * (16 * m + 8 * h)) + col, (int)p.a.out - col, v);
                 }
             }
-            if (RB > 2 && more) load_weights(b + WARPS);
+            if (!AHEAD && more) load_weights(b + stride);
         }
     }
 };
@@ -590,7 +602,7 @@ template <typename T, typename D, int RB> struct FewShared {
         uint4 operand[PARTS<T, D> * RB * 32];
     };
     alignas(16) float part[16][16 * RB]; // this CTA's sums, which the whole cluster reads
-    float unit[16];
+    float2 unit[16];
     Window<16> window;
 };
 
@@ -618,7 +630,7 @@ __global__ void __launch_bounds__(THREADS) low_rank_few_kernel(const __grid_cons
         first_product<T, RB, VEC, 1, (!VEC || RB > 2) ? 1 : 4 / RB>(acc, p, (const uint16_t *)a.down + id * a.down_adapter, sh.window.rows,
                 window, count, lane, rank * WARPS + warp, p.cluster * WARPS);
         __syncthreads();
-        SecondProduct<T, D, RB, VEC, 1> second(p, (const uint16_t *)a.up + id * a.up_adapter, sh.window, count, lane, first, end);
+        SecondProduct<T, D, RB, VEC, 1, 1> second(p, (const uint16_t *)a.up + id * a.up_adapter, sh.window, count, lane, 0, first, end, WARPS);
         second.start(first); // on its way meanwhile
         sh.slabs.add(acc, p.down_mode);
         if (arrived) cluster_wait(); // (the last tile's `part` has been read everywhere)
@@ -640,7 +652,7 @@ __global__ void __launch_bounds__(THREADS) low_rank_few_kernel(const __grid_cons
                 v[s][0] = sum.x * scale; v[s][1] = sum.y * scale; v[s][2] = sum.z * scale; v[s][3] = sum.w * scale;
             }
             const float unit = make_operand<T, RB, PARTS<T, D>>(sh.operand, 1, v, p, row, true);
-            if (threadIdx.x % 4 == 0) sh.unit[row] = unit;
+            if (threadIdx.x % 4 == 0) sh.unit[row] = with_inverse(unit);
         }
         cluster_arrive();
         arrived = true;
@@ -663,6 +675,7 @@ __global__ void __launch_bounds__(THREADS, VEC && RB <= 2 ? 2 : 1) low_rank_down
     } sh;
     __shared__ Window<16 * M> rows;
     ptx::grid_dependency_wait();
+    asm volatile("griddepcontrol.launch_dependents;"); // (the second product's CTAs read the sums behind their own wait)
     const LowRankArgs &a = p.a;
     const int split = (int)blockIdx.x % p.splits, number = (int)blockIdx.x / p.splits;
     const int64_t window = p.first_row + (int64_t)(number / p.window_tiles) * WINDOW;
@@ -684,38 +697,51 @@ __global__ void __launch_bounds__(THREADS, VEC && RB <= 2 ? 2 : 1) low_rank_down
     }
 }
 
+template <typename D, int RB> constexpr int UP_GROUPS = sizeof(D) == 2 && RB <= 2 ? 4 : 2; // of 16 rows, of a warp
+template <int RB> constexpr int UP_CTAS = RB <= 4 ? 2 : 1; // of an SM
+
 template <typename T, typename D, int RB> struct UpShared {
     union {
         uint4 counts[LOW_RANK_MAX_ADAPTERS + 1];
         uint4 operand[PARTS<T, D> * 4 * RB * 32];
     };
-    float unit[64];
+    float2 unit[64];
     Window<64> window;
 };
 
 template <typename T, typename D, int RB, bool VEC>
-__global__ void __launch_bounds__(THREADS, VEC && RB <= 2 ? 2 : 1) low_rank_up_kernel(const __grid_constant__ LowRankPlan p) {
+__global__ void __launch_bounds__(THREADS, VEC ? UP_CTAS<RB> : 1) low_rank_up_kernel(const __grid_constant__ LowRankPlan p) {
     extern __shared__ __align__(16) unsigned char shared[];
     UpShared<T, D, RB> &sh = *reinterpret_cast<UpShared<T, D, RB> *>(shared);
-    ptx::grid_dependency_wait();
+    // What this kernel reads before it waits for the first product's end - indices, base, weights - the first product's kernel has
+    // waited for: all its CTAs had done so when this one could start.
     const LowRankArgs &a = p.a;
+    bool waited = false;
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const int chunk = (int)blockIdx.x % p.chunks, number = (int)blockIdx.x / p.chunks;
     const int64_t window = p.first_row + (int64_t)(number / p.window_tiles) * WINDOW;
     const int tiles = find_tiles(sh.window, sh.counts, a, window, (int)min((int64_t)WINDOW, p.end_row - window));
     const int64_t blocks = (a.out + 31) / 32;
-    const int first = (int)(blocks * chunk / p.chunks) + warp, end = (int)(blocks * (chunk + 1) / p.chunks);
+    const int begin = (int)(blocks * chunk / p.chunks), end = (int)(blocks * (chunk + 1) / p.chunks);
     for (int tile = number % p.window_tiles; tile < tiles; tile += p.window_tiles) {
         int count;
         const int id = find_rows(sh.window, tile, count);
         if (id == a.adapters) {
-            copy_rows<D, VEC>(a, sh.window.rows, window, count, first, end);
+            if (!waited) ptx::grid_dependency_wait(); // (whoever reads dst's memory before has ended)
+            waited = true;
+            copy_rows<D, VEC>(a, sh.window.rows, window, count, begin + warp, end);
             continue;
         }
         find_addresses<D>(sh.window, a, window, count);
         __syncthreads();
-        SecondProduct<T, D, RB, VEC, 4> second(p, (const uint16_t *)a.up + id * a.up_adapter, sh.window, count, lane, first, end);
+        // Where a warp's rows are fewer than the tile's, neighbouring warps share the columns.
+        constexpr int M = UP_GROUPS<D, RB>;
+        const int parts = 16 * M < count ? 4 / M : 1, first = begin + warp / parts;
+        SecondProduct<T, D, RB, VEC, M, 4> second(p, (const uint16_t *)a.up + id * a.up_adapter, sh.window, count, lane, warp % parts * M, first,
+                end, WARPS / parts);
         second.start(first);
+        if (!waited) ptx::grid_dependency_wait();
+        waited = true;
         const int row = threadIdx.x / 4;
         float v[RB][4] = {};
         if (row < count) {
@@ -728,10 +754,11 @@ __global__ void __launch_bounds__(THREADS, VEC && RB <= 2 ? 2 : 1) low_rank_up_k
                 }
         }
         const float unit = make_operand<T, RB, PARTS<T, D>>(sh.operand, 4, v, p, row, row < (count + 15) / 16 * 16);
-        if (threadIdx.x % 4 == 0) sh.unit[row] = unit;
+        if (threadIdx.x % 4 == 0) sh.unit[row] = with_inverse(unit);
         __syncthreads();
         second.run(first, sh.operand, sh.unit);
     }
+    if (!waited) ptx::grid_dependency_wait(); // (the next kernel on the stream relies on this one's wait)
 }
 
 template <typename Kernel> int launch_cluster(Kernel kernel, const LowRankPlan &p, unsigned grid, cudaStream_t st) {
@@ -778,8 +805,8 @@ template <typename T, typename D, int RB, bool VEC> int launch_form(LowRankPlan 
         if (rc != 0) return rc;
         count_launch();
         // Three rounds of CTAs, of at least three blocks of columns a warp (us a call, four / six / eight chunks: the first of those
-        // calls 23.2 / 20.8 / 22.4, the second 115.0 / 114.1 / 116.3).
-        p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((a.out + 31) / 32 / (3 * WARPS + 4), 6 * sm_count / (ends + rows / 64)));
+        // calls 21.0 / 17.5 / 18.7, the second 113.2 / 112.7 / 114.8).
+        p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((a.out + 31) / 32 / (3 * WARPS + 4), 6 * sm_count / (windows + rows / 64)));
         p.window_tiles = (int)std::min<int64_t>(most, std::max<int64_t>(WINDOW / 64 + 2, 4 * sm_count / (windows * p.chunks)));
         if (windows * p.window_tiles * p.chunks > 0x7fffffff) return 3;
         rc = launch_dependent(low_rank_up_kernel<T, D, RB, VEC>, p, (unsigned)(windows * p.window_tiles * p.chunks), THREADS, sizeof(UpShared<T, D, RB>), st);
@@ -815,9 +842,13 @@ template <typename T, typename D> int launch_typed(LowRankPlan &p, int sm_count,
 
 } // namespace
 
-// What a call of `rows` rows needs (0: not known yet) - none for few rows, which one launch serves.
+// What one launch serves: above, tiles of 16 rows read the weights too often (us a call, one launch / two: 64 adapters 4096 x 4096, rank
+// 16, 100 rows 9.1 / 9.9, 400 10.6 / 15.9, 1024 20.9 / 29.0, 2048 38.2 / 43.5; 16 adapters 4096 x 11008, rank 32, 512 rows 20.9 / 26.9,
+// 1024 36.4 / 36.7, 2048 55.3 / 45.6; rank 64, 64 adapters 4096 x 4096, 400 rows 33.9 / 36.8, 1024 62.2 / 46.4).
+static bool few_rows(int64_t rows, int64_t rank) { return rows <= (rank <= 32 ? 1024 : 512); }
+
 size_t low_rank_scratch_bytes(int64_t rows, int64_t rank) {
-    if (rows >= 0 && rows <= LOW_RANK_FEW) return 0;
+    if (rows >= 0 && few_rows(rows, rank < 0 ? LOW_RANK_MAX : rank)) return 0;
     const int64_t blocks = rank < 0 || rank > 64 ? 8 : rank > 32 ? 4 : rank > 16 ? 2 : 1;
     return (size_t)(rows < 0 ? LOW_RANK_CHUNK : std::min<int64_t>(rows, LOW_RANK_CHUNK)) * 16 * blocks * sizeof(float) * LOW_RANK_SPLITS;
 }
@@ -826,7 +857,7 @@ int launch_low_rank(const LowRankArgs &a, void *scratch, int sm_count, cudaStrea
     if (a.rows == 0 || a.out == 0) return 0;
     LowRankPlan p {};
     p.a = a;
-    p.middle = a.rows <= LOW_RANK_FEW ? nullptr : (float *)scratch;
+    p.middle = few_rows(a.rows, a.rank) ? nullptr : (float *)scratch;
     if (a.dt == DT_BF16)
         return a.dst_dt == DT_F32 ? launch_typed<__nv_bfloat16, float>(p, sm_count, st) : launch_typed<__nv_bfloat16, __nv_bfloat16>(p, sm_count, st);
     if (a.dt == DT_F16) return a.dst_dt == DT_F32 ? launch_typed<__half, float>(p, sm_count, st) : launch_typed<__half, __half>(p, sm_count, st);

@@ -122,7 +122,6 @@ struct LowRankArgs {
     void *dst;
     int64_t dst_ld;
 };
-constexpr int LOW_RANK_FEW = 64; // rows that one launch serves
 constexpr int LOW_RANK_CHUNK = 8192; // rows whose sums are in the scratchpad at a time
 constexpr int LOW_RANK_SPLITS = 4; // of the columns that these sums run over, at most
 int launch_low_rank(const LowRankArgs &a, void *scratch, int sm_count, cudaStream_t st);

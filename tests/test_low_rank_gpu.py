@@ -77,8 +77,11 @@ def verify(got, x, index, down, up, scale, base, dtype, out):
 # rows, adapters, columns in, rank, columns out: one row; ranks on both sides of every block; widths that are no multiple of
 # anything; more rows than a window; tiles that are full, ragged, of one row
 SIZES = [(1, 1, 64, 8, 64), (1, 5, 4096, 16, 4096), (3, 2, 8, 4, 8), (17, 2, 520, 16, 264), (64, 3, 256, 32, 128), (65, 1, 256, 24, 200), (130, 4, 192, 64, 96),
-         (100, 3, 136, 128, 72), (33, 2, 64, 100, 40), (61, 64, 1024, 16, 1024), (513, 7, 128, 8, 136), (1100, 40, 64, 12, 64), (600, 1, 72, 32, 80)]
-ODD = [(1, 1, 1, 1, 1), (5, 2, 31, 3, 17), (40, 3, 1001, 16, 333), (70, 2, 40, 5, 99), (20, 2, 257, 33, 129), (9, 2, 77, 127, 55), (530, 9, 63, 7, 65)]
+         (100, 3, 136, 128, 72), (33, 2, 64, 100, 40), (61, 64, 1024, 16, 1024), (513, 7, 128, 8, 136), (1100, 40, 64, 12, 64), (600, 1, 72, 32, 80),
+         # both sides of what one launch serves, more rows than the scratchpad holds at a time, as many adapters as there can be
+         (1024, 5, 64, 16, 72), (1025, 5, 64, 32, 72), (512, 3, 96, 64, 136), (513, 3, 96, 33, 136), (1200, 2, 96, 128, 136), (8300, 5, 64, 8, 72),
+         (1300, 1024, 64, 16, 64), (700, 1024, 64, 16, 64)]
+ODD = [(1100, 3, 33, 5, 41), (600, 2, 70, 77, 50), (1, 1, 1, 1, 1), (5, 2, 31, 3, 17), (40, 3, 1001, 16, 333), (70, 2, 40, 5, 99), (20, 2, 257, 33, 129), (9, 2, 77, 127, 55), (530, 9, 63, 7, 65)]
 
 
 @pytest.mark.parametrize("T,n,K,r,N", SIZES)
@@ -229,6 +232,71 @@ def test_open_dims_and_a_captured_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         verify(R.host(t["y"]), a[0], index, *a[2:], None, "bf16", "bf16")
+
+
+@pytest.mark.parametrize("T,out", [(1500, "bf16"), (1500, "f32"), (300, "bf16")])
+def test_in_place_with_a_scratchpad_of_the_program(gpu, T, out):
+    import torch
+    from onednn_b200 import api
+    n, K, r, N = 4, 128, 16, 200
+    x, index, down, up, scale, g = make(T, n, K, r, N, "bf16", none=0.3)
+    base = L.rounded(g.standard_normal((T, N)), out)
+    attr = api.primitive_attr()
+    attr.set_scales(api.ARG_WEIGHTS, 1)
+    attr.set_scratchpad_mode(api.SCRATCHPAD_MODE_USER)
+    c = L.Call(gpu[0])
+    y = R.device_matrix(base, out)
+    c.bind(api.ARG_ATTR_SCALES | api.ARG_WEIGHTS, R.device_matrix(scale[None], "f32")[0])
+    ymd = c.bind(api.ARG_DST, y)
+    c.bind(api.ARG_SRC_2, y)
+    pd = api.low_rank_adapter.primitive_desc(
+        gpu[0], c.bind(api.ARG_SRC, R.device_matrix(x, "bf16")), c.bind(api.ARG_SRC_1, torch.from_numpy(index.astype(np.int32)).cuda()),
+        c.bind(api.ARG_WEIGHTS, factor(down, "bf16", "middle")), c.bind(api.ARG_WEIGHTS_1, factor(up, "bf16", "last")), ymd, base_md=ymd, attr=attr)
+    md = pd.query_md(255, api.ARG_SCRATCHPAD)
+    if T <= 512:
+        assert md.get_ndims() == 0
+    else:
+        prim, need = api.low_rank_adapter(pd), md.get_dims()[0]
+        with pytest.raises(api.error) as e:
+            prim.execute(c.strm, c.args)  # none
+        assert e.value.status == api.invalid_arguments
+        room = torch.full((need + 32,), 0xff, dtype=torch.uint8, device="cuda:0")
+        c.bind(api.ARG_SCRATCHPAD, room[4:4 + need])  # not on a 16-byte boundary
+        with pytest.raises(api.error) as e:
+            prim.execute(c.strm, c.args)
+        assert e.value.status == api.invalid_arguments
+        c.bind(api.ARG_SCRATCHPAD, room[:need])
+    c.run(api.low_rank_adapter, pd)
+    c.strm.wait()
+    verify(R.host(y), x, index, down, up, scale, base, "bf16", out)
+    assert np.array_equal(R.host(y)[index < 0], base[index < 0])
+
+
+def test_calls_in_a_row(gpu):
+    """each call's rows are what the call before wrote, with no wait in between: kernels that start early read behind their wait"""
+    import torch
+    from onednn_b200 import api
+    T, n, K, r = 1400, 3, 256, 16
+    x, index, down, up, scale, g = make(T, n, K, r, K, "bf16")
+    a, b = R.device_matrix(x, "bf16"), torch.zeros((T, K), dtype=torch.bfloat16, device="cuda:0")
+    i, d, u = torch.from_numpy(index.astype(np.int32)).cuda(), factor(down, "bf16", "middle"), factor(up, "bf16", "middle")
+    calls = []
+    for step in range(6):
+        src, dst = (a, b) if step % 2 == 0 else (b, a)
+        c = L.Call(gpu[0])
+        pd = api.low_rank_adapter.primitive_desc(gpu[0], c.bind(api.ARG_SRC, src), c.bind(api.ARG_SRC_1, i), c.bind(api.ARG_WEIGHTS, d),
+                                                 c.bind(api.ARG_WEIGHTS_1, u), c.bind(api.ARG_DST, dst), base_md=c.bind(api.ARG_SRC_2, src))
+        calls.append((api.low_rank_adapter(pd), c))
+    torch.cuda.synchronize()
+    for prim, c in calls:
+        prim.execute(c.strm, c.args)
+    c.strm.wait()
+    got = R.host(a)
+    a.copy_(torch.from_numpy(x))  # the same, one at a time
+    for prim, c in calls:
+        prim.execute(c.strm, c.args)
+        c.strm.wait()
+    assert np.array_equal(got, R.host(a))
 
 
 def test_two_runs_give_the_same_bits_and_a_row_does_not_depend_on_its_neighbours(gpu):
