@@ -37,9 +37,9 @@ def norm(x, epsilon, weights=None, residual=None):
     return (y if weights is None else y * weights), h
 
 
-# Relative error of y before it is rounded to its type, in units of 2^-24: the sum (1), squares added by a thread (at most 32
-# of them), a warp (5) and a CTA (4), each square off by that of the sum twice (2): 43; the division, epsilon and, at half of
-# all that, the root: 24; the quotient (1) and two products (2).
+# Relative error of y before it is rounded to its type, in units of 2^-24, an upper bound: the sum (1), squares added by a thread (at
+# most 32 of them, in two sums or one), a warp (5) and a CTA (4), each square off by that of the sum twice (2): 43; the mean, epsilon
+# and, at half of all that, the root: 24; its inverse (1) and two products (2).
 NORM_UNITS = 28
 
 
