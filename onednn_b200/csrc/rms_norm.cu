@@ -548,15 +548,15 @@ template <typename T, bool VEC> int launch_form(NormArgs &a, bool backward, int 
     }
     if (chunks <= 32) return launch_forward<T, VEC, 32, 1>(a, sm_count, st);
     if (chunks <= 64) return launch_forward<T, VEC, 32, 2>(a, sm_count, st);
-    if (VEC && sizeof(T) == 2 && !a.residual) {
-        if (chunks <= 128) return launch_forward<T, VEC, 32, 4>(a, sm_count, st);
-        if (chunks <= 256) return launch_forward<T, VEC, 64, 4>(a, sm_count, st);
-        if (chunks <= 512) return launch_forward<T, VEC, 128, 4>(a, sm_count, st);
-    } else {
-        if (chunks <= 128) return launch_forward<T, VEC, 64, 2>(a, sm_count, st);
-        if (chunks <= 256) return launch_forward<T, VEC, 128, 2>(a, sm_count, st);
-        if (chunks <= 512) return launch_forward<T, VEC, 256, 2>(a, sm_count, st);
-    }
+    if constexpr (VEC && sizeof(T) == 2)
+        if (!a.residual) {
+            if (chunks <= 128) return launch_forward<T, VEC, 32, 4>(a, sm_count, st);
+            if (chunks <= 256) return launch_forward<T, VEC, 64, 4>(a, sm_count, st);
+            if (chunks <= 512) return launch_forward<T, VEC, 128, 4>(a, sm_count, st);
+        }
+    if (chunks <= 128) return launch_forward<T, VEC, 64, 2>(a, sm_count, st);
+    if (chunks <= 256) return launch_forward<T, VEC, 128, 2>(a, sm_count, st);
+    if (chunks <= 512) return launch_forward<T, VEC, 256, 2>(a, sm_count, st);
     if (chunks <= 768) return launch_forward<T, VEC, 256, 3>(a, sm_count, st);
     if (chunks <= 1024) return launch_forward<T, VEC, 256, 4>(a, sm_count, st);
     return launch_forward<T, VEC, 512, 4>(a, sm_count, st);

@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 
 EPSILON = 1e-5
 # every number of threads and chunks that a row can have, odd widths, single columns
-WIDTHS = [1, 8, 40, 255, 256, 264, 512, 513, 1000, 1367, 2048, 2047, 4096, 4104, 8192, 8200, 16384, 16383]
+WIDTHS = [1, 8, 40, 255, 256, 264, 512, 513, 1000, 1367, 2048, 2047, 4096, 4104, 8192, 8200, 16384, 16383, 5001, 7001]
 
 
 def values(seed, shape, dtype, scale=1.0):
@@ -102,6 +102,30 @@ def test_norm(gpu, H, dtype):
     close(got, L.norm(x, EPSILON, values(H + 2, (H,), "f32"))[0], L.NORM_UNITS, "f32")
     got, _, _ = run_norm(gpu, x, dtype, dtype)
     close(got, L.norm(x, EPSILON)[0], L.NORM_UNITS, dtype)
+
+
+@pytest.mark.parametrize("T,H", [(5001, 24), (9000, 200), (4000, 520), (2500, 1000), (3001, 1367), (1500, 2048), (1300, 3000), (700, 4096), (650, 5001),
+                                 (600, 5120), (500, 7001), (450, 8192)])
+@pytest.mark.parametrize("dtype,residual", [("bf16", True), ("bf16", False), ("f32", True)])
+def test_norm_of_many_rows(gpu, T, H, dtype, residual):
+    """more rows than CTAs: each takes several, with the next on its way"""
+    x, w = values(1, (T, H), dtype), values(3, (H,), "f32")
+    res = values(2, (T, H), dtype) if residual else None
+    got, scale, total = run_norm(gpu, x, dtype, "s8", w, residual=res, total=residual, scaling="row")
+    y, h = L.norm(x, EPSILON, w, res)
+    v, s = L.quantized(y, "s8", 0)
+    close(scale, s, L.NORM_UNITS + 1, "f32")
+    L.check_8bit(got, v, 2 * L.NORM_UNITS + 4, "s8")
+    if residual:
+        close(total, h, 1, dtype)
+    if H % 8 == 0:
+        got, _, _ = run_norm(gpu, x, dtype, dtype, w, residual=res)
+        close(got, y, L.NORM_UNITS, dtype)
+    if H % 128 == 0:
+        got, scale, _ = run_norm(gpu, x, dtype, "e4m3", w, residual=res, scaling="group", group=128)
+        v, s = L.quantized(y, "e4m3", 128)
+        close(scale, s, L.NORM_UNITS + 1, "f32")
+        L.check_8bit(got, v, 2 * L.NORM_UNITS + 4, "e4m3")
 
 
 @pytest.mark.parametrize("pitch,offset,out_pitch,out_offset", [(0, 1, 0, 0), (1003, 0, 0, 0), (0, 0, 1001, 0), (0, 0, 0, 3),
