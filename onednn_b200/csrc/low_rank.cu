@@ -11,7 +11,8 @@
 //     a row, which stay in L2); then a CTA takes 64 rows and a run of dst's columns through the second.  No CTA waits for another;
 //     the second kernel starts as the first one's CTAs end, and finds its rows and asks for its first base and weights meanwhile
 //     (777 rows of 37 adapters 20.1 us without, 17.4 with).
-// Measured: 8192 rows, 4096 x 11008, rank 32, 16 adapters 112.7 us (3.9 TB/s); 61 rows of 64 adapters, 4096 x 4096, rank 16 8.9 us.  The
+// Measured: 8192 rows, 4096 x 11008, rank 32, 16 adapters 112.7 us (3.9 TB/s; 213 with 11009 columns, 179 with 4097: rows that start
+// anywhere); 61 rows of 64 adapters, 4096 x 4096, rank 16 8.9 us.  The
 // second product's kernel takes the same time without its MMAs: latency of 16 warps an SM (128 registers) bounds it.  Deeper
 // prefetch through shared memory (cp.async, three blocks a warp), 64 columns a warp and 256 contiguous bytes a row were slower or the same
 // (119, 169, 130 us at a rank of 32; 108, 102, 118 for 106 at 16).
@@ -102,16 +103,31 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t halves(uint32_t lo, uint32_t hi, bool upper) { return __byte_perm(lo, hi, upper ? 0x7632 : 0x5410); }
 
-// eight 16-bit values of a row, of which `left` more columns are there; zeros behind them
-template <bool VEC> __device__ __forceinline__ uint4 load_8(const uint16_t *at, int left) {
+// Eight 16-bit values of a row from its column `col` on, of which `left` more are there; zeros behind them.  Rows that start
+// anywhere: the two aligned blocks of 16 bytes that hold them, where both lie in the row, shifted; one by one at its ends.
+template <bool VEC> __device__ __forceinline__ uint4 load_8(const uint16_t *at, int col, int left) {
     if constexpr (VEC) {
         return left > 0 ? ptx::ld_dependent((const uint4 *)at) : make_uint4(0, 0, 0, 0);
     } else {
-        uint32_t w[4];
+        uint32_t w[8];
+        if (col >= 8 && left >= 16) {
+            const uint32_t off = (uint32_t)(uintptr_t)at & 15u; // bytes
+            const uint4 *block = (const uint4 *)((uintptr_t)at - off);
+            const uint4 x = ptx::ld_dependent(block), y = ptx::ld_dependent(block + 1);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = 2 * i < left ? ld_u16(at + 2 * i) : 0u, hi = 2 * i + 1 < left ? ld_u16(at + 2 * i + 1) : 0u;
-            w[i] = lo | hi << 16;
+            for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __byte_perm(w[i], w[i + 1], off & 2 ? 0x5432 : 0x3210);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t lo = 2 * i < left ? ld_u16(at + 2 * i) : 0u, hi = 2 * i + 1 < left ? ld_u16(at + 2 * i + 1) : 0u;
+                w[i] = lo | hi << 16;
+            }
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -157,6 +173,11 @@ __device__ __forceinline__ void load_down(uint32_t (&w)[J][4], const LowRankPlan
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const bool there = 8 * (j0 + j) + g < a.rank;
+            if (a.down_in == 1) { // rows that start anywhere
+                const uint4 v = load_8<false>(at + 8 * (j0 + j) * a.down_rank, (int)a.in - left, there ? left : 0);
+                w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint16_t *from = at + 8 * (j0 + j) * a.down_rank + 2 * i * a.down_in;
@@ -235,12 +256,12 @@ template <int RB> __device__ __forceinline__ void order_up(uint32_t (&w)[4][RB][
     }
 }
 
-// eight values of a row of base or dst, of which `left` more columns are there
+// eight values of a row of base or dst from its column `col` on, of which `left` more are there
 template <typename D, bool VEC> struct Eight {
     uint4 raw[sizeof(D) / 2];
-    __device__ __forceinline__ void load(const D *at, int left) {
+    __device__ __forceinline__ void load(const D *at, int col, int left) {
         if constexpr (sizeof(D) == 2) {
-            raw[0] = load_8<VEC>((const uint16_t *)at, left);
+            raw[0] = load_8<VEC>((const uint16_t *)at, col, left);
         } else if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) raw[i] = left > 0 ? ptx::ld_dependent((const uint4 *)at + i) : make_uint4(0, 0, 0, 0);
@@ -268,9 +289,23 @@ template <typename D, bool VEC> struct Eight {
             unpack2(raw[0].w, v[6], v[7], D());
         }
     }
+    static __device__ __forceinline__ void store_pair(D *at, float lo, float hi) {
+        if constexpr (sizeof(D) == 2) *reinterpret_cast<uint32_t *>(at) = pack2(lo, hi, D());
+    }
     static __device__ __forceinline__ void store(D *at, int left, const float (&v)[8]) {
         if constexpr (VEC) {
             if (left > 0) Cols<D, true>::store_ragged(at, 8, v);
+        } else if (sizeof(D) == 2 && left >= 8) { // in words of two, where they are aligned
+            const bool odd = (uintptr_t)at & 2;
+            if (odd) {
+                at[0] = from_f32<D>(v[0]);
+                at[7] = from_f32<D>(v[7]);
+#pragma unroll
+                for (int i = 1; i < 7; i += 2) store_pair(at + i, v[i], v[i + 1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) store_pair(at + i, v[i], v[i + 1]);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -302,7 +337,7 @@ __device__ __forceinline__ void first_product(float (&acc)[M][2 * RB][4], const 
 #pragma unroll
             for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) v[u][m][h] = load_8<VEC>(x[m][h] + 32 * u * step, left - 32 * u * step);
+                for (int h = 0; h < 2; ++h) v[u][m][h] = load_8<VEC>(x[m][h] + 32 * u * step, (int)a.in - left + 32 * u * step, left - 32 * u * step);
             load_down<RB, J, VEC>(w[u], p, down + (32 * (s + u * step) + 8 * t) * a.down_in, left - 32 * u * step, 0, lane);
         }
 #pragma unroll
@@ -422,7 +457,7 @@ __device__ __forceinline__ void copy_rows(const LowRankArgs &a, const unsigned s
             float v[8] = {};
             if (a.base) {
                 Eight<D, VEC> e;
-                e.load((const D *)a.base + row * a.base_ld + col, left);
+                e.load((const D *)a.base + row * a.base_ld + col, col, left);
                 e.get(v);
             }
             Eight<D, VEC>::store((D *)a.dst + row * a.dst_ld + col, left, v);
@@ -527,7 +562,7 @@ template <typename T, typename D, int RB, bool VEC, int M, int GROUPS> struct Se
         this->up = up + (32 * first + 4 * (lane >> 2)) * p.a.up_out + rank_column<RB>(p.up_mode, 0, lane & 3, 0) * p.a.up_rank;
     }
     __device__ __forceinline__ void load_base(int m, int h, int col) {
-        base[m][h].load(ld_address<const D>(bases + 8 * (16 * m + 8 * h)) + col, (int)p.a.out - col);
+        base[m][h].load(ld_address<const D>(bases + 8 * (16 * m + 8 * h)) + col, col, (int)p.a.out - col);
     }
     __device__ __forceinline__ void load_weights(int b) {
         load_up<RB, VEC>(raw, p, up, (int)p.a.out - 32 * b - 4 * (lane >> 2), lane);
@@ -627,7 +662,7 @@ __global__ void __launch_bounds__(THREADS) low_rank_few_kernel(const __grid_cons
         }
         find_addresses<D>(sh.window, a, window, count);
         float acc[1][2 * RB][4] = {};
-        first_product<T, RB, VEC, 1, (!VEC || RB > 2) ? 1 : 4 / RB>(acc, p, (const uint16_t *)a.down + id * a.down_adapter, sh.window.rows,
+        first_product<T, RB, VEC, 1, (RB > 2 ? 1 : (VEC ? 4 : 2) / RB)>(acc, p, (const uint16_t *)a.down + id * a.down_adapter, sh.window.rows,
                 window, count, lane, rank * WARPS + warp, p.cluster * WARPS);
         __syncthreads();
         SecondProduct<T, D, RB, VEC, 1, 1> second(p, (const uint16_t *)a.up + id * a.up_adapter, sh.window, count, lane, 0, first, end, WARPS);
@@ -667,7 +702,7 @@ __global__ void __launch_bounds__(THREADS) low_rank_few_kernel(const __grid_cons
 template <int RB> constexpr int DOWN_GROUPS = RB == 8 ? 1 : 2; // of 16 rows
 
 template <typename T, int RB, bool VEC>
-__global__ void __launch_bounds__(THREADS, VEC && RB <= 2 ? 2 : 1) low_rank_down_kernel(const __grid_constant__ LowRankPlan p) {
+__global__ void __launch_bounds__(THREADS, RB <= 2 ? 2 : 1) low_rank_down_kernel(const __grid_constant__ LowRankPlan p) {
     constexpr int M = DOWN_GROUPS<RB>;
     __shared__ union {
         uint4 counts[LOW_RANK_MAX_ADAPTERS + 1];
@@ -686,7 +721,7 @@ __global__ void __launch_bounds__(THREADS, VEC && RB <= 2 ? 2 : 1) low_rank_down
         const int id = find_rows(rows, tile, count);
         if (id == a.adapters) continue;
         float acc[M][2 * RB][4] = {};
-        first_product<T, RB, VEC, M, (!VEC || RB > 2) ? 1 : 2>(acc, p, (const uint16_t *)a.down + id * a.down_adapter, rows.rows, window, count,
+        first_product<T, RB, VEC, M, (!VEC || RB > 2 ? 1 : 2)>(acc, p, (const uint16_t *)a.down + id * a.down_adapter, rows.rows, window, count,
                 threadIdx.x & 31, split * WARPS + threadIdx.x / 32, p.splits * WARPS);
         sh.slabs.add(acc, p.down_mode);
         const float scale = a.scales ? ptx::ld_dependent(a.scales + id) : 1.f;
@@ -710,7 +745,7 @@ template <typename T, typename D, int RB> struct UpShared {
 };
 
 template <typename T, typename D, int RB, bool VEC>
-__global__ void __launch_bounds__(THREADS, VEC ? UP_CTAS<RB> : 1) low_rank_up_kernel(const __grid_constant__ LowRankPlan p) {
+__global__ void __launch_bounds__(THREADS, UP_CTAS<RB>) low_rank_up_kernel(const __grid_constant__ LowRankPlan p) {
     extern __shared__ __align__(16) unsigned char shared[];
     UpShared<T, D, RB> &sh = *reinterpret_cast<UpShared<T, D, RB> *>(shared);
     // What this kernel reads before it waits for the first product's end - indices, base, weights - the first product's kernel has
@@ -780,18 +815,21 @@ template <typename Kernel> int launch_cluster(Kernel kernel, const LowRankPlan &
     return rc;
 }
 
-template <typename T, typename D, int RB, bool VEC> int launch_form(LowRankPlan &p, int sm_count, cudaStream_t st) {
+template <typename T, typename D, int RB, bool VEC> int launch_few(LowRankPlan &p, int sm_count, cudaStream_t st) {
     const LowRankArgs &a = p.a;
-    if (!p.middle) {
-        const int64_t windows = (a.rows + WINDOW - 1) / WINDOW, most = std::min<int64_t>(a.rows, WINDOW);
-        p.end_row = a.rows;
-        p.cluster = 4;
-        p.window_tiles = (int)std::min<int64_t>(most, std::max<int64_t>(WINDOW / 16 + 2, 2 * sm_count / (windows * p.cluster)));
-        if (windows * p.window_tiles * p.cluster > 0x7fffffff) return 3;
-        return launch_cluster(low_rank_few_kernel<T, D, RB, VEC>, p, (unsigned)(windows * p.window_tiles * p.cluster), st);
-    }
-    static std::atomic<unsigned long long> done;
-    if (!opt_in_dynamic_smem(low_rank_up_kernel<T, D, RB, VEC>, (int)sizeof(UpShared<T, D, RB>), done)) return 5;
+    const int64_t windows = (a.rows + WINDOW - 1) / WINDOW, most = std::min<int64_t>(a.rows, WINDOW);
+    p.end_row = a.rows;
+    p.cluster = 4;
+    p.window_tiles = (int)std::min<int64_t>(most, std::max<int64_t>(WINDOW / 16 + 2, 2 * sm_count / (windows * p.cluster)));
+    return launch_cluster(low_rank_few_kernel<T, D, RB, VEC>, p, (unsigned)(windows * p.window_tiles * p.cluster), st);
+}
+
+template <typename T, typename D, int RB> int launch_many(LowRankPlan &p, bool in, bool out, int sm_count, cudaStream_t st) {
+    const LowRankArgs &a = p.a;
+    static std::atomic<unsigned long long> done, done_any;
+    if (!opt_in_dynamic_smem(low_rank_up_kernel<T, D, RB, true>, (int)sizeof(UpShared<T, D, RB>), done)
+            || !opt_in_dynamic_smem(low_rank_up_kernel<T, D, RB, false>, (int)sizeof(UpShared<T, D, RB>), done_any))
+        return 5;
     for (p.first_row = 0; p.first_row < a.rows; p.first_row = p.end_row) {
         p.end_row = std::min<int64_t>(a.rows, p.first_row + LOW_RANK_CHUNK);
         const int64_t rows = p.end_row - p.first_row, windows = (rows + WINDOW - 1) / WINDOW, most = std::min<int64_t>(rows, WINDOW);
@@ -801,7 +839,8 @@ template <typename T, typename D, int RB, bool VEC> int launch_form(LowRankPlan 
         const int64_t ends = windows * (std::min<int64_t>(most, a.adapters) / 2 + 1);
         p.splits = (int)std::min<int64_t>(LOW_RANK_SPLITS, std::max<int64_t>(1, sm_count / (ends + rows / (16 * DOWN_GROUPS<RB>))));
         p.window_tiles = (int)std::min<int64_t>(most, std::max<int64_t>(WINDOW / (16 * DOWN_GROUPS<RB>) + 2, 2 * sm_count / (windows * p.splits)));
-        int rc = launch_dependent(low_rank_down_kernel<T, RB, VEC>, p, (unsigned)(windows * p.window_tiles * p.splits), THREADS, 0, st);
+        int rc = launch_dependent(in ? low_rank_down_kernel<T, RB, true> : low_rank_down_kernel<T, RB, false>, p,
+                (unsigned)(windows * p.window_tiles * p.splits), THREADS, 0, st);
         if (rc != 0) return rc;
         count_launch();
         // Three rounds of CTAs, of at least three blocks of columns a warp (us a call, four / six / eight chunks: the first of those
@@ -809,7 +848,8 @@ template <typename T, typename D, int RB, bool VEC> int launch_form(LowRankPlan 
         p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((a.out + 31) / 32 / (3 * WARPS + 4), 6 * sm_count / (windows + rows / 64)));
         p.window_tiles = (int)std::min<int64_t>(most, std::max<int64_t>(WINDOW / 64 + 2, 4 * sm_count / (windows * p.chunks)));
         if (windows * p.window_tiles * p.chunks > 0x7fffffff) return 3;
-        rc = launch_dependent(low_rank_up_kernel<T, D, RB, VEC>, p, (unsigned)(windows * p.window_tiles * p.chunks), THREADS, sizeof(UpShared<T, D, RB>), st);
+        rc = launch_dependent(out ? low_rank_up_kernel<T, D, RB, true> : low_rank_up_kernel<T, D, RB, false>, p,
+                (unsigned)(windows * p.window_tiles * p.chunks), THREADS, sizeof(UpShared<T, D, RB>), st);
         if (rc != 0) return rc;
         count_launch();
     }
@@ -827,10 +867,12 @@ template <typename T, typename D, int RB> int launch_rank(LowRankPlan &p, int sm
     p.up_mode = a.up_out == 1 && a.out % 4 == 0 && aligned(a.up, 8, a.up_adapter, a.up_rank) ? VECTOR_OUTER
             : a.up_rank == 1 && a.rank % (4 * RB) == 0 && aligned(a.up, std::min(8 * RB, 16), a.up_adapter, a.up_out) ? VECTOR_RANK
                                                                                                                    : ELEMENTS;
-    const bool vec = a.in % 8 == 0 && a.out % 8 == 0 && rows_aligned(a.src, a.src_ld * 2, a.rows)
-            && rows_aligned(a.dst, a.dst_ld * (int)sizeof(D), a.rows) && (!a.base || rows_aligned(a.base, a.base_ld * (int)sizeof(D), a.rows))
-            && p.down_mode != ELEMENTS && p.up_mode != ELEMENTS;
-    return vec ? launch_form<T, D, RB, true>(p, sm_count, st) : launch_form<T, D, RB, false>(p, sm_count, st);
+    // whether each side is read and written in wide accesses
+    const bool in = a.in % 8 == 0 && rows_aligned(a.src, a.src_ld * 2, a.rows) && p.down_mode != ELEMENTS;
+    const bool out = a.out % 8 == 0 && rows_aligned(a.dst, a.dst_ld * (int)sizeof(D), a.rows)
+            && (!a.base || rows_aligned(a.base, a.base_ld * (int)sizeof(D), a.rows)) && p.up_mode != ELEMENTS;
+    if (!p.middle) return in && out ? launch_few<T, D, RB, true>(p, sm_count, st) : launch_few<T, D, RB, false>(p, sm_count, st);
+    return launch_many<T, D, RB>(p, in, out, sm_count, st);
 }
 
 template <typename T, typename D> int launch_typed(LowRankPlan &p, int sm_count, cudaStream_t st) {
