@@ -754,7 +754,8 @@ dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_pri
  * set by dnnl_primitive_attr_set_scales for DNNL_ARG_WEIGHTS with mask 1: f32 [n] in device memory; without them 1.
  *   1 <= r <= 128, n <= 1024; weights have any strides (neighbours along K, r or N on 16-byte boundaries are fastest), the matrices
  * any row pitch; T, K and N may be zero, and any dim open.  Rows in any order; a batch of prompts and single tokens of many requests
- * are the same call.  All sums are f32; the middle product is rounded to 17 bits (27 where DST is f32) before the second.  A row of
+ * are the same call.  All sums are f32; the middle product is rounded to 17 bits or more before
+ * the second (22 with f16; 27 with bf16 and a DST of f32).  A row of
  * SRC with an infinity or a NaN gives infinities or NaN.
  *   Calls of more than 512 rows (or of open T) have a scratchpad, which holds the middle product: executions of one primitive that
  * overlap on the GPU need the user scratchpad mode and a buffer each (16-byte aligned), as moe_dispatch has it.
