@@ -10,10 +10,10 @@
 //   More: two launches.  A CTA takes a tile of 32 rows through the first product, and the sums go to the scratchpad (4 r bytes
 //     a row, which stay in L2); then a CTA takes 64 rows and a run of dst's columns through the second.  No CTA waits for another;
 //     the second kernel starts as the first one's CTAs end, and finds its rows and asks for its first base and weights meanwhile
-//     (777 rows of 37 adapters 20.1 us without, 17.4 with).
-// Measured: 8192 rows, 4096 x 11008, rank 32, 16 adapters 112.7 us (3.9 TB/s; 213 with 11009 columns, 179 with 4097: rows that start
-// anywhere); 61 rows of 64 adapters, 4096 x 4096, rank 16 8.9 us.  The
-// second product's kernel takes the same time without its MMAs: latency of 16 warps an SM (128 registers) bounds it.  Deeper
+//     (777 rows of 37 adapters, in two launches, 20.1 us without, 17.4 with).
+// Measured: 8192 rows, 4096 x 11008, rank 32, 16 adapters 106 to 132 us by the draw of the requests, 123 over eight draws (3.5 TB/s);
+// at the draw that takes 113, 213 with 11009 columns, 179 with 4097: rows that start anywhere; 61 rows of 64 adapters,
+// 4096 x 4096, rank 16 8.9 us.  The second product's kernel takes the same time without its MMAs: latency of 16 warps an SM (128 registers) bounds it.  Deeper
 // prefetch through shared memory (cp.async, three blocks a warp), 64 columns a warp and 256 contiguous bytes a row were slower or the same
 // (119, 169, 130 us at a rank of 32; 108, 102, 118 for 106 at 16).
 // Operands go from global memory to the registers of an MMA without shared memory: a lane reads 8 or 16 bytes, and which of the
@@ -834,8 +834,8 @@ template <typename T, typename D, int RB> int launch_many(LowRankPlan &p, bool i
         p.end_row = std::min<int64_t>(a.rows, p.first_row + LOW_RANK_CHUNK);
         const int64_t rows = p.end_row - p.first_row, windows = (rows + WINDOW - 1) / WINDOW, most = std::min<int64_t>(rows, WINDOW);
         // Full tiles, and half of the adapters once more a window.  The columns of src are split where tiles are too few for the SMs
-        // (us a call, one / two / four splits: 777 rows, 37 adapters, 2048 x 5504 23.2 / 21.0 / 21.7; 8192 rows, 16 adapters,
-        // 4096 x 11008 118.4 / 118.2 / 122.9).
+        // (us a call, one / two / four splits: 777 rows, 37 adapters, 2048 x 5504, in two launches, 23.2 / 21.0 / 21.7; 8192 rows,
+        // 16 adapters, 4096 x 11008, one draw of requests, 118.4 / 118.2 / 122.9).
         const int64_t ends = windows * (std::min<int64_t>(most, a.adapters) / 2 + 1);
         p.splits = (int)std::min<int64_t>(LOW_RANK_SPLITS, std::max<int64_t>(1, sm_count / (ends + rows / (16 * DOWN_GROUPS<RB>))));
         p.window_tiles = (int)std::min<int64_t>(most, std::max<int64_t>(WINDOW / (16 * DOWN_GROUPS<RB>) + 2, 2 * sm_count / (windows * p.splits)));
@@ -843,8 +843,8 @@ template <typename T, typename D, int RB> int launch_many(LowRankPlan &p, bool i
                 (unsigned)(windows * p.window_tiles * p.splits), THREADS, 0, st);
         if (rc != 0) return rc;
         count_launch();
-        // Three rounds of CTAs, of at least three blocks of columns a warp (us a call, four / six / eight chunks: the first of those
-        // calls 21.0 / 17.5 / 18.7, the second 113.2 / 112.7 / 114.8).
+        // Three rounds of CTAs, of at least three blocks of columns a warp (us a call, four / six / eight / twelve chunks: the second of
+        // those calls, mean of eight draws of requests, 131 / 123 / 121 / 121; its rows in any order, all with adapters, 134 / 137 / 139 / 141).
         p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((a.out + 31) / 32 / (3 * WARPS + 4), 6 * sm_count / (windows + rows / 64)));
         p.window_tiles = (int)std::min<int64_t>(most, std::max<int64_t>(WINDOW / 64 + 2, 4 * sm_count / (windows * p.chunks)));
         if (windows * p.window_tiles * p.chunks > 0x7fffffff) return 3;
