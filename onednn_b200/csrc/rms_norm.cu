@@ -209,7 +209,7 @@ template <int THREADS> __device__ __forceinline__ uint32_t row_max(uint32_t v, u
 }
 
 // What brings h w to its 8-bit value, and the scale, of which h w `most` is the largest magnitude (in the bits of a float, those of
-// a NaN are above all others): limit / most, and most r / limit with r the row's norm.  reciprocal: of limit.
+// a NaN are above all others): limit / most, and most r / limit with r what h w lacks of the norm.  reciprocal: of limit.
 __device__ __forceinline__ float make_scale(uint32_t most, float r, float limit, float reciprocal, float &factor) {
     const float m = __uint_as_float(most), y = m * r, q = y * reciprocal;
     float inverse; // off by one unit at most, subnormal results too
@@ -222,6 +222,12 @@ __device__ __forceinline__ float make_scale(uint32_t most, float r, float limit,
 __device__ __forceinline__ float inverse_root(float v) {
     const float r = rsqrtf(v);
     return v < INFINITY ? fmaf(r * 0.5f, fmaf(-v * r, r, 1.f), r) : r;
+}
+// the power of two above the root of a row, and the root over it, 1/2 to 1 (a root of 0: 0; of a NaN: NaN)
+__device__ __forceinline__ float power_of_two(float root, float &rest) {
+    const uint32_t bits = __float_as_uint(root); // (never subnormal: the mean and epsilon are below 2^128)
+    rest = __uint_as_float((bits & 0x007fffffu) | 0x3f000000u);
+    return root > 0.f ? __uint_as_float((bits & 0x7f800000u) + 0x00800000u) : root;
 }
 
 __device__ __forceinline__ float largest(const Pair (&v)[4]) { // magnitude, or NaN
@@ -363,25 +369,34 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
         float total[1] = {sum[0] + sum[1]};
         row_sum<THREADS, 1>(total, sums[turn]);
         const float root = inverse_root(fmaf(total[0], per_column, a.epsilon));
+        // The root before the weights: h is then below 2 sqrt(columns) (0 where the squares exceeded 32 bits), and its product with
+        // the weight finite where the result is.  With made scales only a power of two of it, which leaves h as exact as it was; what
+        // is left of the root goes into the scale.
+        const bool made = a.scaling == NORM_SCALE_ROW || a.scaling == NORM_SCALE_GROUP;
+        float rest;
+        const Pair first = both(made ? power_of_two(root, rest) : root);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] * w[c][i];
-        float factor = root * given;
+            for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] * first * w[c][i];
         if (a.scaling == NORM_SCALE_ROW) {
             float m = 0.f;
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) m = max_nan(m, largest(h[c]));
-            const float s = make_scale(row_max<THREADS>(__float_as_uint(m) & 0x7fffffffu, most[turn]), root, limit, reciprocal, factor);
+            float factor;
+            const float s = make_scale(row_max<THREADS>(__float_as_uint(m) & 0x7fffffffu, most[turn]), rest, limit, reciprocal, factor);
             if (thread == 0) a.scales[t] = s;
-        }
-        if (a.scaling == NORM_SCALE_GROUP) {
-            scale_groups<VEC, THREADS>(a, a.scales + (int64_t)t * (cols / a.group), thread, root, limit, reciprocal, h);
-        } else {
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] * both(factor);
+        } else if (a.scaling == NORM_SCALE_GROUP) {
+            scale_groups<VEC, THREADS>(a, a.scales + (int64_t)t * (cols / a.group), thread, rest, limit, reciprocal, h);
+        } else if (a.scaling == NORM_SCALE_GIVEN) {
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] * both(given);
         }
         switch (a.dst_dt) {
             case DT_F32: store_row<float, VEC, THREADS>((float *)a.dst + t * a.dst_ld, thread, cols, h); break;

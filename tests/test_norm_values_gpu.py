@@ -1,0 +1,54 @@
+"""The norm on a device where values are special: ties of the 8-bit rounding, magnitudes at both ends of 32 bits."""
+import numpy as np
+import pytest
+
+import layer_ref as L
+from test_norm_gpu import close, run_norm
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype,offset", [("f32", 0), ("bf16", 0), ("bf16", 1)])
+def test_rows_whose_squares_exceed_32_bits_are_zeros(gpu, dtype, offset):
+    """whatever the weights are; other rows are not touched by them"""
+    H = 96
+    r = np.random.Generator(np.random.PCG64(5))
+    x = r.standard_normal((4, H))
+    x[1] = r.choice([-1, 1], H) * r.uniform(1e37, 3.3e38, H)
+    x[3] = 0
+    x[3, 40] = 3e38
+    x, w = L.rounded(x, dtype), L.rounded(r.uniform(1.2, 300, H) * r.choice([-1, 1], H), "f32")
+    want = L.norm(x, 1e-5, w)[0]
+    want[[1, 3]] = 0
+    got, _, _ = run_norm(gpu, x, dtype, dtype, w, offset=offset)
+    close(got, want, L.NORM_UNITS, dtype)
+    for out in ("s8", "e4m3"):
+        for scaling, group in (("", 0), ("tensor", 0), ("row", 0), ("group", 32)):
+            got, scale, _ = run_norm(gpu, x, dtype, out, w, scaling=scaling, group=group, given=2.0, offset=offset)
+            assert (got[[1, 3]] == 0).all() and np.isfinite(got).all()
+            if scaling in ("row", "group"):
+                assert (scale[[1, 3]] == 0).all()
+                v, s = L.quantized(want[[0, 2]], out, group)
+                close(scale[[0, 2]], s, L.NORM_UNITS + 1, "f32")
+                L.check_8bit(got[[0, 2]], v, 2 * L.NORM_UNITS + 4, out)
+
+
+@pytest.mark.parametrize("h,weight", [(1e18, 1e21), (1e18, 1e30), (1e-30, 1e-9), (1e-38, 1e-4), (1e-20, 1e25)])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_large_and_small_weights(gpu, h, weight, offset):
+    """where the product of h and its weight is not what 32 bits hold, but the norm times the weight is"""
+    H = 64
+    r = np.random.Generator(np.random.PCG64(6))
+    x, w = L.rounded(r.uniform(0.5, 1, (5, H)) * h, "f32"), L.rounded(r.uniform(0.5, 1, H) * weight, "f32")
+    y = L.norm(x, 1e-5, w)[0]
+    got, _, _ = run_norm(gpu, x, "f32", "f32", w, offset=offset)
+    close(got, y, L.NORM_UNITS, "f32")
+    for scaling, group in (("row", 0), ("group", 32)):
+        for out in ("s8", "e4m3"):
+            got, scale, _ = run_norm(gpu, x, "f32", out, w, scaling=scaling, group=group, offset=offset)
+            v, s = L.quantized(y, out, group)
+            if np.abs(y).max() < 1.4e-36:
+                assert (scale == 0).all() and (got == 0).all()
+                continue
+            close(scale, s, L.NORM_UNITS + 1, "f32")
+            L.check_8bit(got, v, 2 * L.NORM_UNITS + 4, out)
