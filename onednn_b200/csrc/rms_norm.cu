@@ -25,7 +25,7 @@ namespace qmm {
 
 namespace {
 
-constexpr float SMALLEST_MAX = 1e-36f; // 448 / this is still finite
+constexpr float SMALLEST_MAX = 1.4e-36f; // 448 / this is still finite
 
 __device__ __forceinline__ uint32_t cvt_s8(float v) { // saturated, to nearest even; 0 for a NaN
     int r;
@@ -209,7 +209,8 @@ template <int THREADS> __device__ __forceinline__ uint32_t row_max(uint32_t v, u
 }
 
 // What brings h w to its 8-bit value, and the scale, of which h w `most` is the largest magnitude (in the bits of a float, those of
-// a NaN are above all others): limit / most, and most r / limit with r what h w lacks of the norm.  reciprocal: of limit.
+// a NaN are above all others): limit / most, and most r / limit with r what h w lacks of the norm, at most 1: where the scale is not
+// zero, `most` is SMALLEST_MAX at least and the quotient finite.  reciprocal: of limit.
 __device__ __forceinline__ float make_scale(uint32_t most, float r, float limit, float reciprocal, float &factor) {
     const float m = __uint_as_float(most), y = m * r, q = y * reciprocal;
     float inverse; // off by one unit at most, subnormal results too

@@ -52,3 +52,32 @@ def test_large_and_small_weights(gpu, h, weight, offset):
                 continue
             close(scale, s, L.NORM_UNITS + 1, "f32")
             L.check_8bit(got, v, 2 * L.NORM_UNITS + 4, out)
+
+
+@pytest.mark.parametrize("scaling,group", [("row", 0), ("group", 32)])
+@pytest.mark.parametrize("out", ["s8", "e4m3"])
+@pytest.mark.parametrize("dtype,offset", [("f32", 0), ("f32", 1), ("bf16", 0)])
+@pytest.mark.parametrize("epsilon", [1e-5, 1.0, 1e-12])
+def test_small_rows_and_groups_have_scales_of_their_own(gpu, epsilon, dtype, offset, out, scaling, group):
+    """Largest values from below 1.4e-36, where the scale is zero, to 1e-30, in rows whose squares vanish beside epsilon and in groups
+    of ordinary rows; every row holds zeros."""
+    H = 96
+    most = np.concatenate([10.0 ** np.arange(-36.55, -30, 0.25), [1.3e-36, 1.36e-36, 1.44e-36, 1.6e-36, 2e-36, 2.6e-36]])  # after the norm
+    r = np.random.Generator(np.random.PCG64(4))
+    x = r.uniform(-1, 1, (2 * most.size, H))
+    x[:, ::3] = 0
+    x[:, 1::32] = np.where(r.random((2 * most.size, 3)) < 0.5, 1.0, -1.0)
+    x[:most.size] *= most[:, None] * epsilon ** 0.5
+    x[most.size:, 32:] *= most[:, None]  # and one group of ordinary values
+    x = L.rounded(x, dtype)
+    got, scale, _ = run_norm(gpu, x, dtype, out, None, scaling=scaling, group=group, offset=offset, epsilon=epsilon)
+    y = L.norm(x, epsilon)[0]
+    with np.errstate(all="ignore"):
+        v, s = L.quantized(y, out, group)
+    none = s * L.LIMIT[out] < 1.4e-36
+    assert (np.abs(s * L.LIMIT[out] / 1.4e-36 - 1) > 100 * L.EPS).all()  # (none on the border)
+    assert none.any() and (scale[none] == 0).all()
+    close(scale[~none], s[~none], L.NORM_UNITS + 1, "f32")
+    v = np.where(none.repeat(group or H, 1), 0, v)
+    assert not np.isnan(got).any() and (got[v == 0] == 0).all()
+    L.check_8bit(got, v, 2 * L.NORM_UNITS + 4, out)
