@@ -242,6 +242,33 @@ __device__ __forceinline__ float largest(const Pair (&v)[4]) { // magnitude, or 
     return m;
 }
 
+// The eight columns of a thread, 32 apart: a group is the same GROUP / 32 of them in all lanes (or one in half of them).  One group after
+// the other: 4099 x 4096 bf16 that start anywhere, groups of 128, take 24 us instead of the 47 of all eight maxima at once, whose registers
+// spill.  (That form also came out of ptxas 12.9 wrong at -O3, though not at -O1, once the quotient had more parts than one: in the kernels of
+// four chunks every group had the first one's maximum.)
+template <int GROUP>
+__device__ __forceinline__ void scale_spread(float *scales, int col, int cols, float r, float limit, float reciprocal, float (&each)[8]) {
+    constexpr int N = GROUP < 32 ? 1 : GROUP / 32;
+#pragma unroll
+    for (int k = 0; k < 8; k += N) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = k; i < k + N; ++i) m = max_nan(m, fabsf(each[i]));
+        uint32_t most = __float_as_uint(m) & 0x7fffffffu;
+        if constexpr (GROUP == 16) {
+#pragma unroll
+            for (int s = 1; s < 16; s *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, s));
+        } else {
+            most = __reduce_max_sync(0xffffffffu, most);
+        }
+        float factor;
+        const float s = make_scale(most, r, limit, reciprocal, factor);
+        if (col + 32 * k < cols && (col + 32 * k) % GROUP == 0) scales[(col + 32 * k) / GROUP] = s;
+#pragma unroll
+        for (int i = k; i < k + N; ++i) each[i] *= factor;
+    }
+}
+
 // h w to 8 bits by the scales of its groups, and the scales.  Groups of 16 to 256 columns, a power of two: in a warp's 256 columns
 // they are whole lanes' (VEC), or one to eight times 32 columns of all lanes, or half of them.
 template <bool VEC, int THREADS, int CHUNKS>
@@ -266,39 +293,23 @@ __device__ __forceinline__ void scale_groups(const NormArgs &a, float *scales, i
             for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] * both(factor);
         }
     } else {
+        auto all = [&](auto spread) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int col = chunk_column<VEC>(c * THREADS + thread);
-            float each[8], factor[8];
-            uint32_t m[8];
+            for (int c = 0; c < CHUNKS; ++c) {
+                float each[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) split(v[c][i], each[2 * i], each[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) split(v[c][i], each[2 * i], each[2 * i + 1]);
+                scale_spread<decltype(spread)::value>(scales, chunk_column<VEC>(c * THREADS + thread), cols, r, limit, reciprocal, each);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                m[i] = __float_as_uint(each[i]) & 0x7fffffffu;
-                if (a.group == 16) {
-#pragma unroll
-                    for (int s = 1; s < 16; s *= 2) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], s));
-                } else {
-                    m[i] = __reduce_max_sync(0xffffffffu, m[i]);
-                }
+                for (int i = 0; i < 4; ++i) v[c][i] = pair(each[2 * i], each[2 * i + 1]);
             }
-#pragma unroll
-            for (int step = 1; step < 8; step *= 2) // (pairs, fours, all eight of the 32 columns)
-                if (a.group > 32 * step) {
-                    uint32_t other[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) other[i] = m[i ^ step];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) m[i] = max(m[i], other[i]);
-                }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float s = make_scale(m[i], r, limit, reciprocal, factor[i]);
-                if (col + 32 * i < cols && ((col + 32 * i) & (a.group - 1)) == 0) scales[(col + 32 * i) >> shift] = s;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[c][i] = pair(each[2 * i] * factor[2 * i], each[2 * i + 1] * factor[2 * i + 1]);
+        };
+        switch (a.group) {
+            case 16: all(std::integral_constant<int, 16>()); break;
+            case 32: all(std::integral_constant<int, 32>()); break;
+            case 64: all(std::integral_constant<int, 64>()); break;
+            case 128: all(std::integral_constant<int, 128>()); break;
+            default: all(std::integral_constant<int, 256>());
         }
     }
 }

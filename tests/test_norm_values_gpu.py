@@ -81,3 +81,21 @@ def test_small_rows_and_groups_have_scales_of_their_own(gpu, epsilon, dtype, off
     v = np.where(none.repeat(group or H, 1), 0, v)
     assert not np.isnan(got).any() and (got[v == 0] == 0).all()
     L.check_8bit(got, v, 2 * L.NORM_UNITS + 4, out)
+
+
+@pytest.mark.parametrize("H", [512, 1024, 4096, 5120, 8192, 16384])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_scales_of_groups_in_rows_that_start_anywhere(gpu, H, dtype, residual):
+    """every number of threads and chunks, every size of a group"""
+    r = np.random.Generator(np.random.PCG64([H, residual]))
+    x = L.rounded(r.standard_normal((4, H)) * np.exp(r.standard_normal((4, H // 16))).repeat(16, 1), dtype)
+    res = L.rounded(r.standard_normal((4, H)), dtype) if residual else None
+    w = L.rounded(r.standard_normal(H), "f32")
+    y = L.norm(x, 1e-5, w, res)[0]
+    for group in (16, 32, 64, 128, 256):
+        for out in ("s8", "e4m3"):
+            got, scale, _ = run_norm(gpu, x, dtype, out, w, residual=res, scaling="group", group=group, offset=1)
+            v, s = L.quantized(y, out, group)
+            close(scale, s, L.NORM_UNITS + 1, "f32")
+            L.check_8bit(got, v, 2 * L.NORM_UNITS + 4, out)
