@@ -208,14 +208,23 @@ template <int THREADS> __device__ __forceinline__ uint32_t row_max(uint32_t v, u
     return v;
 }
 
-// What brings h w to its 8-bit value, and the scale, of which h w `most` is the largest magnitude (in the bits of a float, those of
-// a NaN are above all others): limit / most, and most r / limit with r what h w lacks of the norm, at most 1: where the scale is not
-// zero, `most` is SMALLEST_MAX at least and the quotient finite.  reciprocal: of limit.
-__device__ __forceinline__ float make_scale(uint32_t most, float r, float limit, float reciprocal, float &factor) {
+// h w -> its 8-bit value before rounding, h w limit / most, where `most` is the largest |h w|.  The root cancels in this quotient, so
+// it is often a tie of the rounding to 8 bits, and a unit's error decides which way that goes (5 of 100000 e4m3 values).  So the factor
+// limit / most has two parts, which together are off by 2^-44 of it: quotients that 32 bits hold, as they do ties, come out exact.
+struct Quotient {
+    float high, low;
+    __device__ __forceinline__ Pair operator()(Pair v) const { return fma(v, both(high), v * both(low)); }
+    __device__ __forceinline__ float operator()(float v) const { return fmaf(v, high, v * low); }
+};
+// The scale, most r / limit with r what h w lacks of the norm, and that factor.  r is at most 1: where the scale is not zero, `most` is
+// SMALLEST_MAX at least and the factor finite.  (most: the bits of a float, those of a NaN are above all others; reciprocal: of limit.)
+__device__ __forceinline__ float make_scale(uint32_t most, float r, float limit, float reciprocal, Quotient &to) {
     const float m = __uint_as_float(most), y = m * r, q = y * reciprocal;
-    float inverse; // off by one unit at most, subnormal results too
+    float inverse; // off by one unit at most
     asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(m));
-    factor = y < SMALLEST_MAX ? 0.f : y == y ? inverse * limit : y;
+    const float high = inverse * limit, low = fmaf(-high, m, limit) * inverse;
+    to.high = y < SMALLEST_MAX ? 0.f : y == y ? high : y;
+    to.low = y < SMALLEST_MAX ? 0.f : low;
     // the quotient, with what is left of the division put back; an infinity stays one
     return y < SMALLEST_MAX ? 0.f : y < INFINITY ? fmaf(fmaf(-q, limit, y), reciprocal, q) : y;
 }
@@ -261,11 +270,11 @@ __device__ __forceinline__ void scale_spread(float *scales, int col, int cols, f
         } else {
             most = __reduce_max_sync(0xffffffffu, most);
         }
-        float factor;
-        const float s = make_scale(most, r, limit, reciprocal, factor);
+        Quotient to;
+        const float s = make_scale(most, r, limit, reciprocal, to);
         if (col + 32 * k < cols && (col + 32 * k) % GROUP == 0) scales[(col + 32 * k) / GROUP] = s;
 #pragma unroll
-        for (int i = k; i < k + N; ++i) each[i] *= factor;
+        for (int i = k; i < k + N; ++i) each[i] = to(each[i]);
     }
 }
 
@@ -286,11 +295,11 @@ __device__ __forceinline__ void scale_groups(const NormArgs &a, float *scales, i
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = chunk_column<VEC>(c * THREADS + thread);
-            float factor;
-            const float s = make_scale(m[c], r, limit, reciprocal, factor);
+            Quotient to;
+            const float s = make_scale(m[c], r, limit, reciprocal, to);
             if (col < cols && (col & (a.group - 1)) == 0) scales[col >> shift] = s;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] * both(factor);
+            for (int i = 0; i < 4; ++i) v[c][i] = to(v[c][i]);
         }
     } else {
         auto all = [&](auto spread) {
@@ -395,13 +404,13 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
             float m = 0.f;
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) m = max_nan(m, largest(h[c]));
-            float factor;
-            const float s = make_scale(row_max<THREADS>(__float_as_uint(m) & 0x7fffffffu, most[turn]), rest, limit, reciprocal, factor);
+            Quotient to;
+            const float s = make_scale(row_max<THREADS>(__float_as_uint(m) & 0x7fffffffu, most[turn]), rest, limit, reciprocal, to);
             if (thread == 0) a.scales[t] = s;
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) h[c][i] = h[c][i] * both(factor);
+                for (int i = 0; i < 4; ++i) h[c][i] = to(h[c][i]);
         } else if (a.scaling == NORM_SCALE_GROUP) {
             scale_groups<VEC, THREADS>(a, a.scales + (int64_t)t * (cols / a.group), thread, rest, limit, reciprocal, h);
         } else if (a.scaling == NORM_SCALE_GIVEN) {

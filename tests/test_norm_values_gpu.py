@@ -99,3 +99,34 @@ def test_scales_of_groups_in_rows_that_start_anywhere(gpu, H, dtype, residual):
             v, s = L.quantized(y, out, group)
             close(scale, s, L.NORM_UNITS + 1, "f32")
             L.check_8bit(got, v, 2 * L.NORM_UNITS + 4, out)
+
+
+def nearest_8bit(v, out):
+    """`v` in 8 bits, to nearest, ties to even, saturated"""
+    step = 1.0 if out == "s8" else L.step_e4m3(v)
+    return np.clip(np.round(v / step) * step, -128.0 if out == "s8" else -448.0, L.LIMIT[out])
+
+
+# every number of threads and chunks that a row can have
+@pytest.mark.parametrize("H,groups", [(40, ()), (255, ()), (512, (16, 32, 64, 128, 256)), (1024, (16, 32, 64, 128, 256)), (2048, (32, 128, 256)),
+                                      (4096, (16, 32, 64, 128, 256)), (5120, (16, 32, 64, 128, 256)), (8192, (16, 32, 64, 128, 256)),
+                                      (16384, (16, 32, 64, 128, 256))])
+@pytest.mark.parametrize("out", ["s8", "e4m3"])
+@pytest.mark.parametrize("dtype,offset", [("bf16", 0), ("bf16", 1), ("f16", 0), ("f16", 1), ("f32", 0), ("f32", 1)])
+def test_values_between_two_of_8_bits_go_to_the_even_one(gpu, H, groups, out, dtype, offset):
+    """A made scale is the largest |h w| over the limit, so that the root cancels in the quotient: many quotients are ties.  h and w
+    are whole numbers below 2^6 and 2^4 here: h w, of ten bits, and h w times the limit, of 17, are exact in 32 bits.  A quotient
+    limit h w / m that is not a tie is at least 1 / (255 x 2^10) of itself away from one, more than 32 bits can be off: every value
+    has to be the nearest one."""
+    T = max(5, min(200, 80000 // H))
+    r = np.random.Generator(np.random.PCG64([T, H]))
+    x = np.round(r.integers(-63, 64, (T, H)) * r.random((T, 1)))
+    w = r.integers(1, 16, H).astype(float)
+    for group in (0,) + groups:
+        got, scale, _ = run_norm(gpu, x, dtype, out, w, dtype, scaling="group" if group else "row", group=group, offset=offset)
+        hw = (x * w).reshape(T, -1, group or H)
+        most = np.maximum(np.abs(hw).max(2, keepdims=True), 1)
+        want = nearest_8bit((hw * L.LIMIT[out] / most).reshape(T, H), out)
+        bad = got != want
+        assert not bad.any(), (group, bad.sum(), np.argwhere(bad)[:5], got[bad][:5], want[bad][:5])
+        close(scale, np.abs(L.norm(x, 1e-5, w)[0]).reshape(T, -1, group or H).max(2) / L.LIMIT[out], L.NORM_UNITS + 1, "f32")
