@@ -491,7 +491,8 @@ __global__ void __launch_bounds__(BACKWARD_BLOCK<THREADS>, BACKWARD_CTAS<THREADS
         s[1] += odd[1];
         row_sum<THREADS, ROWS>(s, sums[turn][team]);
         const float r = inverse_root(fmaf(s[0], per_column, a.epsilon));
-        const Pair root = both(r), inner = both(-(s[1] * per_column * r * r)); // dh = r (z - h inner)
+        // dh = r (z - h inner); where the squares exceeded 32 bits r is 0, and the products may have exceeded them too
+        const Pair root = both(r), inner = both(r > 0.f ? -(s[1] * per_column * r * r) : 0.f);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             Pair x[4], g[4], d[4];

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import layer_ref as L
-from test_norm_gpu import close, run_norm
+from test_norm_gpu import check_backward, close, run_backward, run_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,19 @@ def test_values_between_two_of_8_bits_go_to_the_even_one(gpu, H, groups, out, dt
         bad = got != want
         assert not bad.any(), (group, bad.sum(), np.argwhere(bad)[:5], got[bad][:5], want[bad][:5])
         close(scale, np.abs(L.norm(x, 1e-5, w)[0]).reshape(T, -1, group or H).max(2) / L.LIMIT[out], L.NORM_UNITS + 1, "f32")
+
+
+@pytest.mark.parametrize("dtype,offset", [("f32", 0), ("bf16", 0), ("bf16", 1)])
+@pytest.mark.parametrize("T,H", [(5, 96), (700, 40)])
+def test_gradient_of_rows_whose_squares_exceed_32_bits(gpu, T, H, dtype, offset):
+    """zeros besides what comes along the residual path, and nothing in the weights' gradient"""
+    r = np.random.Generator(np.random.PCG64(7))
+    h, dy, dsum = r.standard_normal((T, H)), r.standard_normal((T, H)) * 3, r.standard_normal((T, H))
+    over = np.arange(T) % 4 == 1
+    h[over] = r.choice([-1, 1], (over.sum(), H)) * r.uniform(1e37, 3.3e38, (over.sum(), H))
+    h, dy, dsum = (L.rounded(v, dtype) for v in (h, dy, dsum))
+    w = L.rounded(r.uniform(1.2, 300, H), "f32")
+    for add in (None, dsum):
+        got, gotw = run_backward(gpu, h, dy, dtype, w, "f32", add, "f32", offset=offset)
+        assert np.array_equal(got[over], np.zeros_like(got[over]) if add is None else dsum[over])
+        check_backward(got[~over], gotw, h[~over], dy[~over], dtype, w, None if add is None else dsum[~over], "f32")
