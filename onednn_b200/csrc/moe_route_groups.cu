@@ -37,6 +37,9 @@ __host__ __device__ inline int group_lanes(int groups) {
 // softmax: the argument is off by 2^-24 of itself, which is at most 104 where the exponential is not zero; its sum has at most
 // 32 + 5 roundings, the exponential and the quotient are as above.
 __device__ __forceinline__ float score_error(int scoring) { return scoring == SCORING_SIGMOID ? 0x1p-21f : 0x1p-16f; }
+// And its error besides, where the score is too small for a relative one: a sigmoid below 2^-126 may come out as 0 (its quotient with
+// a divisor above 2^126 does), a softmax's is off by a few of the least numbers, 2^-149.  Two scores on either side of a comparison.
+constexpr float LEAST_SCORES = 4.f * 0x1p-126f;
 
 // exp(x), x <= 0, in 64 bits without a branch, so that several run at once: x = n log 2 + r with log 2 in two parts of which the
 // first has zeros enough that its product with n is exact (Cody and Waite: Software manual for the elementary functions; 1980),
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_groups_kernel(const __grid_c
         const uint32_t ends = __ballot_sync(0xffffffffu, real && better == a.groups_kept - 1), next = __ballot_sync(0xffffffffu, real && better == a.groups_kept);
         if (next) {
             const float l = __shfl_sync(0xffffffffu, rank, __ffs(ends) - 1), n = __shfl_sync(0xffffffffu, rank, __ffs(next) - 1);
-            close = !(l - n > 2.f * (score_error(a.scoring) + 0x1p-22f) * (fabsf(l) + 4.f * most_bias));
+            close = !(l - n > 2.f * (score_error(a.scoring) + 0x1p-22f) * (fabsf(l) + 4.f * most_bias) + LEAST_SCORES);
         }
 #pragma unroll
         for (int i = 0; i < PER_LANE; ++i) {
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_groups_kernel(const __grid_c
     auto near = [&] {
         const uint32_t down = __shfl_down_sync(0xffffffffu, mine, 1), after = lane == found - 1 ? left_out : down;
         const float c = key_value<float>(mine & ~SLOT), n = key_value<float>(after & ~SLOT);
-        return lane < found && after && !(c - n > 2.f * (score_error(a.scoring) + (PER_LANE + 1) * 0x1p-23f) * (fabsf(c) + most_bias));
+        return lane < found && after && !(c - n > 2.f * (score_error(a.scoring) + (PER_LANE + 1) * 0x1p-23f) * (fabsf(c) + most_bias) + LEAST_SCORES);
     };
     const bool tight = near();
     const bool some = !close && __any_sync(0xffffffffu, tight);
