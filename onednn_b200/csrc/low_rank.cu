@@ -495,9 +495,6 @@ template <int RB, int M> struct Slabs {
 
 template <typename T, typename D> constexpr int PARTS = sizeof(D) == 4 && std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
 
-// (unit, 1 / unit) of a row
-__device__ __forceinline__ float2 with_inverse(float unit) { return make_float2(unit, 1.f / unit); }
-
 // The second product's left operand, for a row of which this thread (of four, t = threadIdx.x % 4) has the middle's columns
 // rank_column(mode, s, t, 0..3): operand[part][group of rows][s][lane].  f16: returns the power of two it was divided by.
 template <typename T, int RB, int P>
@@ -545,7 +542,11 @@ __device__ __forceinline__ float make_operand(uint4 *operand, int groups, float 
 // columns of dst at a time, every `stride` of these blocks; its rows' base is asked for one block ahead, the weights too where
 // registers allow it (a rank of up to 32).  start() asks for the first block's, and may be called long before.
 template <typename T, typename D, int RB, bool VEC, int M, int GROUPS> struct SecondProduct {
-    static constexpr bool AHEAD = RB <= 2;
+    static constexpr bool AHEAD = RB <= 2, UNITS = std::is_same<T, __half>::value;
+    // With units the next base can be asked for behind the products only; the weights in front of it where registers allow it (8192 rows of
+    // 37 adapters, 2048 x 5504, f16, us a call, in front / behind: rank 64 to f32 250 / 280; to f16, 16 adapters 4096 x 11008, 192 / 181;
+    // rank 128 to f32 433 / 426).
+    static constexpr bool WEIGHTS_FIRST = UNITS && RB == 4 && sizeof(D) == 4;
     const LowRankPlan &p;
     const uint16_t *up; // of the lane, in the block that is asked for next
     uint32_t bases, dsts; // shared memory, of the lane's first row
@@ -579,7 +580,7 @@ template <typename T, typename D, int RB, bool VEC, int M, int GROUPS> struct Se
         }
         load_weights(first);
     }
-    __device__ __forceinline__ void run(int first, const uint4 *operand, const float2 *units) {
+    __device__ __forceinline__ void run(int first, const uint4 *operand, const float *units) {
         for (int b = first; b < end; b += stride) {
             const int col = 32 * b + 8 * (lane & 3);
             const bool more = b + stride < end;
@@ -589,20 +590,19 @@ template <typename T, typename D, int RB, bool VEC, int M, int GROUPS> struct Se
 #pragma unroll
             for (int m = 0; m < M; ++m) {
                 if (16 * (group + m) >= count) break;
+                // The base is where the sums begin (bf16), or is added to them behind their unit (f16: in that unit a finite base might be infinite).
                 float out[4][4];
-                float2 unit[2]; // (f16)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if constexpr (std::is_same<T, __half>::value) unit[h] = units[16 * (group + m) + 8 * h + (lane >> 2)];
                     float v[8] = {};
-                    if (p.a.base) {
+                    if (!UNITS && p.a.base) {
                         base[m][h].get(v);
                         if (more) load_base(m, h, col + 32 * stride);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) out[j][2 * h + i] = std::is_same<T, __half>::value ? v[4 * i + j] * unit[h].y : v[4 * i + j];
+                        for (int i = 0; i < 2; ++i) out[j][2 * h + i] = v[4 * i + j];
                 }
 #pragma unroll
                 for (int q = PARTS<T, D> - 1; q >= 0; --q) // the smallest first
@@ -612,18 +612,24 @@ template <typename T, typename D, int RB, bool VEC, int M, int GROUPS> struct Se
 #pragma unroll
                         for (int j = 0; j < 4; ++j) mma_16816<T>(out[j], f.x, f.y, f.z, f.w, w[j][s][0], w[j][s][1]);
                     }
+                if (WEIGHTS_FIRST && more && (m == M - 1 || 16 * (group + m + 1) >= count)) load_weights(b + stride);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float v[8];
+                    float v[8] = {};
+                    if (UNITS && p.a.base) {
+                        base[m][h].get(v);
+                        if (more) load_base(m, h, col + 32 * stride);
+                    }
+                    const float unit = UNITS ? units[16 * (group + m) + 8 * h + (lane >> 2)] : 1.f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) v[4 * i + j] = std::is_same<T, __half>::value ? out[j][2 * h + i] * unit[h].x : out[j][2 * h + i];
+                        for (int i = 0; i < 2; ++i) v[4 * i + j] = UNITS ? fmaf(out[j][2 * h + i], unit, v[4 * i + j]) : out[j][2 * h + i];
                     if (16 * (group + m) + 8 * h + (lane >> 2) < count)
                         Eight<D, VEC>::store(ld_address<D>(dsts + 8 * (16 * m + 8 * h)) + col, (int)p.a.out - col, v);
                 }
             }
-            if (!AHEAD && more) load_weights(b + stride);
+            if (!AHEAD && !WEIGHTS_FIRST && more) load_weights(b + stride);
         }
     }
 };
@@ -637,7 +643,7 @@ template <typename T, typename D, int RB> struct FewShared {
         uint4 operand[PARTS<T, D> * RB * 32];
     };
     alignas(16) float part[16][16 * RB]; // this CTA's sums, which the whole cluster reads
-    float2 unit[16];
+    float unit[16];
     Window<16> window;
 };
 
@@ -687,7 +693,7 @@ __global__ void __launch_bounds__(THREADS) low_rank_few_kernel(const __grid_cons
                 v[s][0] = sum.x * scale; v[s][1] = sum.y * scale; v[s][2] = sum.z * scale; v[s][3] = sum.w * scale;
             }
             const float unit = make_operand<T, RB, PARTS<T, D>>(sh.operand, 1, v, p, row, true);
-            if (threadIdx.x % 4 == 0) sh.unit[row] = with_inverse(unit);
+            if (threadIdx.x % 4 == 0) sh.unit[row] = unit;
         }
         cluster_arrive();
         arrived = true;
@@ -740,7 +746,7 @@ template <typename T, typename D, int RB> struct UpShared {
         uint4 counts[LOW_RANK_MAX_ADAPTERS + 1];
         uint4 operand[PARTS<T, D> * 4 * RB * 32];
     };
-    float2 unit[64];
+    float unit[64];
     Window<64> window;
 };
 
@@ -789,7 +795,7 @@ __global__ void __launch_bounds__(THREADS, UP_CTAS<RB>) low_rank_up_kernel(const
                 }
         }
         const float unit = make_operand<T, RB, PARTS<T, D>>(sh.operand, 4, v, p, row, row < (count + 15) / 16 * 16);
-        if (threadIdx.x % 4 == 0) sh.unit[row] = with_inverse(unit);
+        if (threadIdx.x % 4 == 0) sh.unit[row] = unit;
         __syncthreads();
         second.run(first, sh.operand, sh.unit);
     }
