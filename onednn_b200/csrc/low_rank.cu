@@ -508,10 +508,10 @@ __device__ __forceinline__ float make_operand(uint4 *operand, int groups, float 
             if (rank_column<RB>(p.up_mode, s, t, i) >= p.a.rank) v[s][i] = 0.f; // (whatever src holds)
             most = fmaxf(most, fabsf(v[s][i]));
         }
-    if constexpr (std::is_same<T, __half>::value) { // the largest of the row into [2^13, 2^14)
+    if constexpr (std::is_same<T, __half>::value) { // the largest of the row into [2^13, 2^14), by a normal number
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        if (most > 0.f && most < INFINITY) unit = __uint_as_float(max(__float_as_uint(most) & 0x7f800000u, 87u << 23)) * 0x1p-13f;
+        if (most > 0.f && most < INFINITY) unit = __uint_as_float(max(__float_as_uint(most) & 0x7f800000u, 14u << 23)) * 0x1p-13f;
     }
     if (!there) return unit;
     const float inverse = 1.f / unit;

@@ -22,3 +22,13 @@ def test_a_large_base_beside_small_products(gpu, T, r, dtype, offset):
     got = run(gpu, x, index, down, up, dtype, "f32", scale, base, "middle", "middle", offset, offset)
     assert np.isfinite(got).all()
     verify(got, x, index, down, up, scale, base, dtype, "f32")
+
+
+@pytest.mark.parametrize("T,r", [(40, 8), (600, 128)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_small_products_keep_their_bits(gpu, T, r, dtype):
+    """the first product times an adapter's scale down to 1e-30: in 32-bit results as exact as any other"""
+    x, index, down, up, scale, g = make(T, 8, 64, r, 72, dtype)
+    scale = L.rounded(scale * 10.0 ** -g.uniform(10, 30, 8), "f32")
+    got = run(gpu, x, index, down, up, dtype, "f32", scale, None, "middle", "middle")
+    verify(got, x, index, down, up, scale, None, dtype, "f32")
