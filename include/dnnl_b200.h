@@ -757,8 +757,9 @@ dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_pri
  * are the same call.  All sums are f32; the middle product is rounded to 17 bits or more before
  * the second (22 with f16; 27 with bf16 and a DST of f32).  A row of
  * SRC with an infinity or a NaN gives infinities or NaN.
- *   Calls of more than 512 rows (or of open T) have a scratchpad, which holds the middle product: executions of one primitive that
- * overlap on the GPU need the user scratchpad mode and a buffer each (16-byte aligned), as moe_dispatch has it.
+ *   Calls of more than 1024 rows (512 with r above 32; open dims count as large ones) have a scratchpad, which holds the middle product:
+ * executions of one primitive that overlap on the GPU need the user scratchpad mode and a buffer each (16-byte aligned), as
+ * moe_dispatch has it.
  *   The gradient of SRC is this primitive on the gradient of DST, with WEIGHTS_1 transposed as WEIGHTS and WEIGHTS as WEIGHTS_1 (their
  * strides say so), and the projection's own gradient as base. */
 dnnl_status_t dnnl_cuda_interop_low_rank_adapter_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
