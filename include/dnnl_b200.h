@@ -730,8 +730,11 @@ dnnl_status_t dnnl_cuda_interop_dropout_primitive_desc_create(dnnl_primitive_des
  *     row over 127 (s8) or 448 (f8_e4m3);
  *   mask 3 with groups {1, g}, dynamic_fp: the same per g neighbouring columns, [T, H / g]; g a power of two from 16 to 256 that
  *     divides H.
- * They are what dnnl_matmul takes as scales of its src.  Where the largest |value| is below 1.4e-36 (whose
- * quotient with 448 is no longer finite) the scale is 0 and so are the values; where a value is NaN the scale is NaN. */
+ * Where the largest |value| is below 1.4e-36 (whose quotient with 448 is no longer finite) the scale is 0 and so are the values;
+ * where a value is NaN the scale is NaN.
+ *   dnnl_matmul takes, as scales of its src (set there as static ones), one scale for s8 (cuda:tcgen05:int8) and f8_e4m3
+ * (cuda:tcgen05:fp8), a scale per row for s8 (cuda:tcgen05:int8), and scales of groups in its reference kernels only
+ * (cuda:ref_int8:any, cuda:ref:any); f8_e4m3 with a scale per row it does not take. */
 dnnl_status_t dnnl_cuda_interop_rms_norm_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
         const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t residual_desc, const_dnnl_memory_desc_t weights_desc,
         const_dnnl_memory_desc_t dst_desc, const_dnnl_memory_desc_t sum_desc, float epsilon, const_dnnl_primitive_attr_t attr);

@@ -1,5 +1,35 @@
-"""What the operators around a quantized projection promise, without a device: when the adapters have a scratchpad."""
-BF16, S32 = 2, 4
+"""What the operators around a quantized projection promise of one another, without a device: which of the norm's outputs the products
+take and by which kernel, and when the adapters have a scratchpad."""
+import pytest
+
+BF16, F32, S32, S8, E4M3 = 2, 3, 4, 5, 10
+
+
+@pytest.mark.parametrize("out,mask,groups,impl", [(S8, 0, (), "cuda:tcgen05:int8"), (S8, 1, (), "cuda:tcgen05:int8"), (E4M3, 0, (), "cuda:tcgen05:fp8"),
+                                                  (E4M3, 1, (), None), (S8, 3, (1, 128), "cuda:ref_int8:any"), (E4M3, 3, (1, 128), "cuda:ref:any")])
+def test_products_of_what_the_norm_writes(host_engine, out, mask, groups, impl):
+    """the scales that the norm takes for its dst, given to the product for its src"""
+    from onednn_b200 import api
+    md, eng = api.memory.desc, host_engine
+    T, H, N = 256, 1024, 512
+    attr = api.primitive_attr()
+    attr.set_scales(api.ARG_DST, mask, groups, qmode=api.quantization_mode.dynamic_fp if mask else api.quantization_mode.static_sazp)
+    x, q = md((T, H), BF16, (H, 1)), md((T, H), out, (H, 1))
+    norm = api.rms_norm.primitive_desc(eng, x, q, 1e-5, attr=attr)
+    assert norm.query_md(255, api.ARG_ATTR_SCALES | api.ARG_DST).get_dims() == ((T if mask & 1 else 1), (H // groups[1] if groups else 1))
+    attr = api.primitive_attr()
+    attr.set_scales(api.ARG_SRC, mask, groups)
+    attr.set_scales(api.ARG_WEIGHTS, 2)
+
+    def product():
+        return api.matmul.primitive_desc(eng, q, md((H, N), out, (N, 1)), md((T, N), F32, (N, 1)), None, attr)
+
+    if impl is None:
+        with pytest.raises(api.error) as e:
+            product()
+        assert e.value.status == api.unimplemented
+    else:
+        assert product().impl_info_str() == impl
 
 
 def test_scratchpad_of_the_adapters(host_engine):
