@@ -663,10 +663,10 @@ dnnl_status_t dnnl_cuda_interop_moe_route_primitive_desc_create(dnnl_primitive_d
  * (0; f32 [E], neighbouring values): the bias moves the choice, not the weights, which are made from the scores of the chosen
  * as above.  The experts are `groups` (1 to 32, a divisor of E) runs of neighbours; only those of the groups_kept groups take part
  * whose group_best (1 or 2) largest c have the largest sum (of those that are there, where a group has fewer); K <= E / groups x groups_kept.
- * The choice is by the values of c and of their sums in 64 bits, ties to the lowest group and expert.  A masked logit is masked here
- * too; an expert with a bias of -inf or NaN is never chosen; +inf counts as the largest finite value.  With no bias and one group
- * this is the router above, which chooses by the logits (scores that 64 bits hold as the same number differ there).  Its gradient is
- * moe_route_backward with the indices that this primitive chose; the bias has none. */
+ * The choice is by the values of c and of their sums in 64 bits (scores below 2^-1022 as 0), ties to the lowest group and expert.  A
+ * masked logit is masked here too; an expert with a bias of -inf or NaN is never chosen; +inf counts as the largest finite value.
+ * With no bias and one group this is the router above, which chooses by the logits (scores that 64 bits hold as the same number differ
+ * there).  Its gradient is moe_route_backward with the indices that this primitive chose; the bias has none. */
 dnnl_status_t dnnl_cuda_interop_moe_route_v2_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,
         const_dnnl_memory_desc_t logits_desc, const_dnnl_memory_desc_t bias_desc, const_dnnl_memory_desc_t weights_desc,
         const_dnnl_memory_desc_t indices_desc, dnnl_cuda_interop_scoring_t scoring, int normalize, float scale, int groups,
@@ -722,16 +722,17 @@ dnnl_status_t dnnl_cuda_interop_dropout_primitive_desc_create(dnnl_primitive_des
  * -> DST [T, H] = h / sqrt(mean over the row of h^2 + epsilon) x WEIGHTS [H] (f32 or SRC's type; NULL: 1), and, where sum_desc
  * is given, DST_1 = h, of SRC's type.  (DST is made from the sum before it is rounded.)  DST is f32, of SRC's type, s8 or
  * f8_e4m3.  DST_1 may be the residual's or SRC's memory, DST SRC's where the types agree.  Squares are summed in 32 bits: a
- * row whose sum of squares exceeds them comes out as zeros, one with an infinity or a NaN as NaN.
+ * row whose sum of squares exceeds them comes out as zeros, so does one with an infinity, with a NaN where that is; one with a NaN
+ * comes out as NaN.
  *   An 8-bit DST holds round(value / scale), to nearest even, saturated (a NaN is 0 in s8).  Its scales are set by
  * dnnl_primitive_attr_set_scales_v3 for DNNL_ARG_DST, f32, in device memory; without them the scale is 1:
- *   mask 0, static: one scale, an input;
+ *   mask 0, static: one scale, an input, 2^-126 or more;
  *   mask 1, dnnl_quantization_mode_dynamic_fp: a scale per row, [T, 1], which this primitive writes: the largest |value| of the
  *     row over 127 (s8) or 448 (f8_e4m3);
  *   mask 3 with groups {1, g}, dynamic_fp: the same per g neighbouring columns, [T, H / g]; g a power of two from 16 to 256 that
  *     divides H.
  * Where the largest |value| is below 1.4e-36 (whose quotient with 448 is no longer finite) the scale is 0 and so are the values;
- * where a value is NaN the scale is NaN.
+ * where a value is NaN or infinite so is the scale, and the values are NaN.
  *   dnnl_matmul takes, as scales of its src (set there as static ones), one scale for s8 (cuda:tcgen05:int8) and f8_e4m3
  * (cuda:tcgen05:fp8), a scale per row for s8 (cuda:tcgen05:int8), and scales of groups in its reference kernels only
  * (cuda:ref_int8:any, cuda:ref:any); f8_e4m3 with a scale per row it does not take. */
@@ -740,8 +741,10 @@ dnnl_status_t dnnl_cuda_interop_rms_norm_primitive_desc_create(dnnl_primitive_de
         const_dnnl_memory_desc_t dst_desc, const_dnnl_memory_desc_t sum_desc, float epsilon, const_dnnl_primitive_attr_t attr);
 /* Its gradient.  DIFF_DST [T, H], SRC the sum h, SRC_2 the gradient that reaches h along the residual path (diff_sum_desc may be
  * NULL), all of one type, WEIGHTS as forward -> DIFF_SRC [T, H], of the same type: the gradient of h, which is that of src and
- * that of the residual alike; DIFF_WEIGHTS [H] (f32 or SRC's type; diff_weights_desc may be NULL), summed in the same order
- * every time.  DIFF_SRC may be the memory of DIFF_DST, SRC_2 or SRC.  Quantization of the output counts as the identity.
+ * that of the residual alike; DIFF_WEIGHTS [H] (f32 or SRC's type; diff_weights_desc may be NULL), summed in 32 bits in
+ * the same order every time, as are the products h w diff_dst of a row.  Rows whose squares exceed 32 bits, and rows with an infinity, have
+ * a gradient of zeros (NaN where the infinity is) besides SRC_2.  DIFF_SRC may be the memory of DIFF_DST, SRC_2 or SRC.  Quantization of
+ * the output counts as the identity.
  *   With DIFF_WEIGHTS, H may not be open, and there is a scratchpad, which holds sums between its kernels: executions of one
  * primitive that overlap on the GPU need the user scratchpad mode and a buffer each (16-byte aligned), as moe_dispatch has it. */
 dnnl_status_t dnnl_cuda_interop_rms_norm_backward_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc, dnnl_engine_t engine,

@@ -146,3 +146,35 @@ def test_gradient_of_rows_whose_squares_exceed_32_bits(gpu, T, H, dtype, offset)
         got, gotw = run_backward(gpu, h, dy, dtype, w, "f32", add, "f32", offset=offset)
         assert np.array_equal(got[over], np.zeros_like(got[over]) if add is None else dsum[over])
         check_backward(got[~over], gotw, h[~over], dy[~over], dtype, w, None if add is None else dsum[~over], "f32")
+
+
+@pytest.mark.parametrize("H,offset", [(96, 0), (96, 1), (2048, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_infinities_and_nan_stay_where_they_are(gpu, H, offset, dtype):
+    """rows with an infinity are zeros but for a NaN where it is, those with a NaN are NaN; an infinite value makes an infinite scale"""
+    r = np.random.Generator(np.random.PCG64(8))
+    x, w = L.rounded(r.standard_normal((5, H)), dtype), L.rounded(r.standard_normal(H), "f32")
+    x[1, 7], x[2, 40], x[3, 50] = np.inf, -np.inf, np.nan
+    want = L.norm(x[[0, 4]], 1e-5, w)[0]
+    got, _, _ = run_norm(gpu, x, dtype, dtype, w, offset=offset)
+    close(got[[0, 4]], want, L.NORM_UNITS, dtype)
+    at = np.isnan(got)
+    assert at[3].all() and at[1].sum() == at[2].sum() == 1 and at[1, 7] and at[2, 40] and (got[1:3][~at[1:3]] == 0).all()
+    got, scale, _ = run_norm(gpu, x, dtype, "e4m3", w, scaling="group", group=32, offset=offset)
+    of = np.arange(H) // 32
+    assert np.array_equal(np.isnan(got[1]), of == 0) and np.array_equal(np.isnan(got[2]), of == 1) and np.isnan(got[3]).all()
+    assert np.array_equal(np.isnan(scale[1]), np.arange(H // 32) == 0) and (scale[1, 1:] == 0).all() and np.isnan(scale[3]).all()
+    # the gradient: the same, besides what comes along the residual path
+    dy, dsum = (L.rounded(r.standard_normal((5, H)), dtype) for _ in range(2))
+    got, gotw = run_backward(gpu, x, dy, dtype, w, "f32", dsum, "f32", offset=offset)
+    at = np.isnan(got)
+    assert at[3].all() and at[1].sum() == at[2].sum() == 1 and at[1, 7] and at[2, 40] and np.array_equal(got[1:3][~at[1:3]], dsum[1:3][~at[1:3]])
+    # a weight that takes the value beyond 32 bits
+    x, w = np.where(np.isfinite(x), x, 0), w.copy()
+    x[0, 3], w[3] = 100.0, 3.4e38
+    w = L.rounded(w, "f32")
+    for out in ("s8", "e4m3"):
+        got, scale, _ = run_norm(gpu, x, dtype, out, w, scaling="group", group=32, offset=offset)
+        assert scale[0, 0] == np.inf and np.isfinite(scale[0, 1:]).all()
+        assert np.isnan(got[0, :32]).all() if out == "e4m3" else (got[0, :32] == 0).all()
+        assert np.isfinite(got[0, 32:]).all()
