@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(BLOCK<THREADS>, FORWARD_CTAS<T, VEC, THREADS, 
 template <typename T, bool VEC, int THREADS, int CHUNKS>
 __global__ void __launch_bounds__(BACKWARD_BLOCK<THREADS>, BACKWARD_CTAS<THREADS>) rms_norm_backward_kernel(const __grid_constant__ NormArgs a) {
     constexpr int ROWS = BACKWARD_TEAMS<THREADS>;
-    extern __shared__ float gathered[]; // several rows at a time: [ROWS][columns]
+    extern __shared__ __align__(16) float gathered[]; // several rows at a time: [ROWS][columns]
     __shared__ float sums[2][ROWS][64];
     ptx::grid_dependency_wait();
     const int thread = threadIdx.x % THREADS, team = threadIdx.x / THREADS, cols = (int)a.cols;

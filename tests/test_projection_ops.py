@@ -1,5 +1,8 @@
 """What the operators around a quantized projection promise of one another, without a device: which of the norm's outputs the products
 take and by which kernel, and when the adapters have a scratchpad."""
+import os
+import re
+
 import pytest
 
 BF16, F32, S32, S8, E4M3 = 2, 3, 4, 5, 10
@@ -48,3 +51,12 @@ def test_scratchpad_of_the_adapters(host_engine):
 
     assert bytes_(1024, 32) == bytes_(512, 33) == bytes_(512, 128) == bytes_(512, O) == bytes_(1, 1) == 0
     assert all(bytes_(T, r) for T, r in ((1025, 1), (1025, 32), (513, 33), (513, 128), (513, O), (O, 8), (O, O)))
+
+
+@pytest.mark.parametrize("file", ["rms_norm.cu", "low_rank.cu"])
+def test_shared_memory_of_wide_accesses_is_aligned(file):
+    """what a launch sizes stands on a 16-byte boundary by its declaration, not by what happens to lie in front of it"""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "onednn_b200", "csrc")
+    with open(os.path.join(csrc, file)) as f:
+        declared = re.findall(r"extern __shared__ ([^;]*);", f.read())
+    assert declared and all(d.startswith("__align__(16) ") for d in declared), declared
