@@ -13,14 +13,15 @@
 //     (777 rows of 37 adapters, in two launches, 20.1 us without, 17.4 with).
 // Measured: 8192 rows, 4096 x 11008, rank 32, 16 adapters 106 to 132 us by the draw of the requests, 123 over eight draws (3.5 TB/s);
 // at the draw that takes 113, 213 with 11009 columns, 179 with 4097: rows that start anywhere; 61 rows of 64 adapters,
-// 4096 x 4096, rank 16 8.9 us.  The second product's kernel takes the same time without its MMAs: latency of 16 warps an SM (128 registers) bounds it.  Deeper
-// prefetch through shared memory (cp.async, three blocks a warp), 64 columns a warp and 256 contiguous bytes a row were slower or the same
+// 4096 x 4096, rank 16 8.9 us.  The second product's kernel takes the same time without its MMAs, and with twice the bytes in flight, so that
+// neither bounds it alone; its 960 CTAs are 3.2 rounds of the 296 that fit, and each finds its rows, makes its operand and fills its
+// loads anew.  Deeper prefetch through shared memory (cp.async, three blocks a warp), 64 columns a warp and 256 contiguous bytes a row were slower or the same
 // (119, 169, 130 us at a rank of 32; 108, 102, 118 for 106 at 16).
 // Operands go from global memory to the registers of an MMA without shared memory: a lane reads 8 or 16 bytes, and which of the
 // summed (or of the output's) columns these are is decided alike for both operands, so any order serves.
 // The middle is a 32-bit sum.  The second product takes it as a sum of 16-bit parts, most significant first: two (what is left
 // out is 2^-18 of a value), or three where dst has 32 bits and the parts are bf16 (2^-27).  f16 parts are made of values that a
-// power of two brings just below the type's largest, row by row.
+// power of two brings just below the type's largest, row by row; what it divides is only the products, the base is added behind it.
 #include <algorithm>
 
 #include "launch.h"
@@ -892,7 +893,10 @@ template <typename T, typename D> int launch_typed(LowRankPlan &p, int sm_count,
 
 // What one launch serves: above, tiles of 16 rows read the weights too often (us a call, one launch / two: 64 adapters 4096 x 4096, rank
 // 16, 100 rows 9.1 / 9.9, 400 10.6 / 15.9, 1024 20.9 / 29.0, 2048 38.2 / 43.5; 16 adapters 4096 x 11008, rank 32, 512 rows 20.9 / 26.9,
-// 1024 36.4 / 36.7, 2048 55.3 / 45.6; rank 64, 64 adapters 4096 x 4096, 400 rows 33.9 / 36.8, 1024 62.2 / 46.4).
+// 1024 36.4 / 36.7, 2048 55.3 / 45.6; rank 64, 64 adapters 4096 x 4096, 400 rows 33.9 / 36.8, 1024 62.2 / 46.4).  What decides is how many
+// rows share an adapter and how large its factors are, which is not known before the call (the indices are in device memory): the
+// limit is where the two are even for 16 adapters, and for 64 some 14 % are lost at 2048 rows.  (The cluster of four CTAs was
+// compared with two and eight on the 61 rows above only.)
 static bool few_rows(int64_t rows, int64_t rank) { return rows <= (rank <= 32 ? 1024 : 512); }
 
 size_t low_rank_scratch_bytes(int64_t rows, int64_t rank) {

@@ -3,17 +3,17 @@
 //   h = src + residual            (written in src's type where that is wanted; what follows takes the unrounded sum)
 //   y = h r w,  r = 1 / sqrt(mean h^2 + eps)
 //   8 bits: q = round(y / s), saturated; s is given (one for all), or made: largest |y| of the row, or of each group of
-//   its columns, over 127 (s8) or 448 (e4m3).  A largest value below 1e-36 makes s = 0 and q = 0; a NaN makes s NaN.
+//   its columns, over 127 (s8) or 448 (e4m3).  A largest value below 1.4e-36 makes s = 0 and q = 0; a NaN makes s NaN.
 // Gradient, with z = w dy:
 //   dh = r z - h r^3 mean(h z) (+ the gradient that comes along the residual path),  dw = sum over the rows of dy h r
 //
 // Bound by memory where rows are many and aligned.  A row stays in the registers of a CTA (of a warp where it is short), so each
 // tensor crosses memory once; sums are f32: in a thread (two columns an instruction), over the warp, over the CTA.  A thread holds
 // chunks of eight columns: neighbours in 16-byte accesses, or 32 apart where rows start anywhere.
-// us a call (floor): 8192 x 4096 bf16 with residual and sum to e4m3 37.6 (35.8, 6.25 TB/s); 4099 x 4096 bf16 to e4m3 with scales of
-// 128 columns 15.7 (7.8; some 560 instructions a warp and row), with one scale 13.0; 3001 x 2047 f16 at odd starts 14.3 (7.5; accesses
-// of two bytes).  Gradient: 8192 x 4096 bf16 with the residual's 48 (40.9), 8192 x 1024 17.0 (10.2), 1021 x 1367 f32 at odd starts 8.3
-// (2.6), of which 2 to 3 are the second kernel.
+// us a call (floor): 8192 x 4096 bf16 with residual and sum to e4m3 37.7 (35.8, 6.2 TB/s); 4099 x 4096 bf16 to e4m3 with scales of
+// 128 columns 17.2 (7.8; some 630 instructions a warp and row, at odd starts 25.6), with one scale 13.2; 2048 x 5120 bf16 with residual and
+// sum, a scale a row 15.5 (11.2); 3001 x 2047 f16 at odd starts 14.6 (7.5; accesses of two bytes).  Gradient: 8192 x 4096 bf16 with the
+// residual's 48 (40.9), 8192 x 1024 17.2 (10.2), 1021 x 1367 f32 at odd starts 8.3 (2.6), of which 2 to 3 are the second kernel.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -210,7 +210,8 @@ template <int THREADS> __device__ __forceinline__ uint32_t row_max(uint32_t v, u
 
 // h w -> its 8-bit value before rounding, h w limit / most, where `most` is the largest |h w|.  The root cancels in this quotient, so
 // it is often a tie of the rounding to 8 bits, and a unit's error decides which way that goes (5 of 100000 e4m3 values).  So the factor
-// limit / most has two parts, which together are off by 2^-44 of it: quotients that 32 bits hold, as they do ties, come out exact.
+// limit / most has two parts, which together are off by 2^-44 of it: quotients that 32 bits hold, as they do ties, come out exact (16.2 -> 17.2 us with scales of 128
+// columns, 15.2 -> 15.3 with a scale a row).
 struct Quotient {
     float high, low;
     __device__ __forceinline__ Pair operator()(Pair v) const { return fma(v, both(high), v * both(low)); }
@@ -570,8 +571,8 @@ template <typename T, bool VEC, int THREADS, int CHUNKS> int launch_backward(Nor
             BACKWARD_TEAMS<THREADS> > 1 ? BACKWARD_TEAMS<THREADS> * a.cols * sizeof(float) : 0, st);
 }
 // Threads of a row and its chunks of eight columns each: two chunks where a residual doubles what is in flight, four without one, which
-// halves what is done once a thread (8192 x 4096 with residual 37.6 us with two, 39.2 with four; 4099 x 4096 without, scales of
-// 128 columns 19.8 / 15.7; 8192 x 1024 with 12.2 / 13.2), and more where the row needs them.
+// halves what is done once a thread (us with two / four: 8192 x 4096 with residual 37.7 / 39.2, 8192 x 1024 with 12.2 / 13.4; 4099 x 4096
+// without, scales of 128 columns 17.6 / 17.2, one scale 13.0 / 13.2), and more where the row needs them.
 template <typename T, bool VEC> int launch_form(NormArgs &a, bool backward, int sm_count, cudaStream_t st) {
     const int64_t chunks = VEC ? (a.cols + 7) / 8 : (a.cols + 255) / 256 * 32;
     if (backward) {
