@@ -320,7 +320,8 @@ __global__ void __launch_bounds__(WARPS * 32) route_groups_kernel(const __grid_c
             second = __shfl_sync(0xffffffffu, s, lane * lanes);
         }
         const bool real = lane < a.groups && first > -INFINITY;
-        const float rank = !real ? -INFINITY : a.group_best == 2 && second > -INFINITY ? first + second : first;
+        // (two of the lowest biases exceed 32 bits: their group is still in front of those without an expert)
+        const float rank = !real ? -INFINITY : a.group_best == 2 && second > -INFINITY ? fmaxf(first + second, -LARGEST<float>) : first;
         int better = 0;
         for (int g = 0; g < a.groups; ++g) {
             const float other = __shfl_sync(0xffffffffu, rank, g);

@@ -42,3 +42,25 @@ def test_many_rows_of_the_smallest_scores(gpu, scoring, dtype, E, groups, kept, 
     want = L.choose(R.host(logits), None, scoring, 4, groups, kept, best)
     bad = (idx != want).any(1)
     assert not bad.any(), (bad.sum(), np.argwhere(bad)[:5], idx[bad][:3], want[bad][:3])
+
+
+@pytest.mark.parametrize("scoring,dtype", [("softmax", "f32"), ("sigmoid", "f16"), ("sigmoid", "bf16")])
+@pytest.mark.parametrize("E,groups,kept", [(16, 8, 3), (20, 5, 3), (24, 8, 6), (32, 16, 11), (256, 8, 4)])
+@pytest.mark.parametrize("lowest", [-np.finfo(np.float32).max, -1e38, -1e30])
+def test_biases_that_mask_by_a_low_value(gpu, scoring, dtype, E, groups, kept, lowest):
+    """Groups whose best two have such a bias come behind all others, and in front of those in which every expert is masked: their
+    sum of two is beyond 32 bits."""
+    r = np.random.Generator(np.random.PCG64([E, groups]))
+    T, size = 300, E // groups
+    x = r.standard_normal((T, E))
+    x[(r.random((T, groups)) < 0.4).repeat(size, 1)] = -np.inf
+    x[r.random((T, E)) < 0.2] = np.nan
+    logits = R.device_matrix(x, dtype)
+    for share in (0.3, 0.9, 1.0):
+        bias = (0.1 * r.standard_normal(E)).astype(np.float32).astype(np.float64)
+        bias[(r.random(groups) < share).repeat(size)] = float(np.float32(lowest))
+        for best in (1, 2):
+            _, idx = run(gpu, logits, bias, kept * size if E <= 32 else 8, scoring, True, 1.0, groups, kept, best)
+            want = L.choose(R.host(logits), bias, scoring, kept * size if E <= 32 else 8, groups, kept, best)
+            bad = (idx != want).any(1)
+            assert not bad.any(), (share, best, bad.sum(), np.argwhere(bad)[:3].ravel(), idx[bad][:2], want[bad][:2])
